@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256) void clip_bwd_fused_kernel(const BwdFusedBatch
           const f32x4 l4 = *reinterpret_cast<const f32x4*>(lc + 8 * q4);
           bf16x4 g4;
 #pragma unroll
-          for (int u2 = 0; u2 < 2; ++u2) {   // two elements at a time: packed f32 multiply-adds (v_pk_fma_f32), half the VALU issue slots
+          for (int u2 = 0; u2 < 2; ++u2) {   // two elements at a time (independent chains; the build makes no packed f32 of them)
             const int e = 4 * q4 + 2 * u2;
             const f32x2 tv = {sacc[e], sacc[e + 1]};
             const f32x2 nl = {l4[2 * u2], l4[2 * u2 + 1]};
