@@ -47,7 +47,8 @@ enum {
   MMK_K_SIM_GRAD, MMK_K_GRAD_GEMM, MMK_K_GRAD_FINALIZE, MMK_K_L2NORM, MMK_K_IJEPA_LOSS_FWD,
   MMK_K_IJEPA_LOSS_BWD, MMK_K_GATHER_ROWS, MMK_K_SCATTER_ROWS, MMK_K_PRED_ASSEMBLE, MMK_K_PRED_ASSEMBLE_BWD,
   MMK_K_EMA, MMK_K_MASK_INDEX, MMK_K_LAYERNORM_FWD, MMK_K_LAYERNORM_BWD, MMK_K_ACT, MMK_K_ATTN_FWD,
-  MMK_K_ATTN_BWD, MMK_K_WGRAD, MMK_K_RECALL, MMK_K_CLIP_FUSED, MMK_K_MLP_GEMM, MMK_K_WIN_ATTN_FWD, MMK_K_WIN_ATTN_BWD, MMK_K_CLIP_BWD_FUSED, MMK_K_COUNT
+  MMK_K_ATTN_BWD, MMK_K_WGRAD, MMK_K_RECALL, MMK_K_CLIP_FUSED, MMK_K_MLP_GEMM, MMK_K_WIN_ATTN_FWD, MMK_K_WIN_ATTN_BWD, MMK_K_CLIP_BWD_FUSED,
+  MMK_K_QK_NORM, MMK_K_COUNT
 };
 int mmk_profile_enable(int on);          /* on=1 start recording (clears), on=0 stop */
 /* resolve recorded events (synchronises on them); fills count[k] and total_ms[k] for k < MMK_K_COUNT */
@@ -546,6 +547,26 @@ int mmk_cls_attn_fwd(const void* q, const void* k, const void* v, void* o, float
 int mmk_cls_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const float* lse2, void* dq, void* dk, void* dv, int B,
                      int H, int L, int dh, int64_t kv_sb, int64_t kv_sl, int64_t g_sb, int64_t g_sl, float scale, float dropout_p,
                      uint64_t seed, const float* key_bias, void* stream);
+
+/* Per-head RMS norm of queries and keys and the position rotation in one pass (no reference lines: the reference's blocks,
+ * mmlearn/modules/layers/attention.py:60-75, have neither; this is the form of later towers):
+ *   y = R(pos) (w * x / sqrt(mean(x^2) + eps)) for every (token, head) row of q [B, L, H, D] and k [B, L, Hk, D].
+ * q / k: element strides {batch, token, head}, last dim contiguous; qo / ko: contiguous.  D even, <= 256.  qw / kw: [D] of w_dtype (f32 or
+ * the operands' type), NULL = ones.  table: f32 [table_rows][rot], rot / 2 cosines then rot / 2 sines of a position; rot = 0: no
+ * rotation.  Of the first `rot` values of a head, (i, i + rot / 2) turn together, or with `interleaved` (2 i, 2 i + 1); the others pass.
+ * positions: NULL (0 .. L-1; L <= table_rows), or int32 (pos64 = 0) / int64 (pos64 = 1) [.., L] with batch stride pos_sb (0: one row for
+ * all).  A position outside the table makes its rows NaN.
+ * Backward: dq / dk contiguous; dqw / dkw [D] of w_dtype with the workspaces q_part / k_part, f32
+ * [mmk_qk_norm_rotary_part_rows(B * L * H, D)][D] (k: Hk); NULL pairs: not wanted.  Sums in a fixed order. */
+int mmk_qk_norm_rotary_fwd(const void* q, const void* k, const void* qw, const void* kw, const float* table, int table_rows,
+                           const void* positions, int pos64, int64_t pos_sb, void* qo, void* ko, int B, int L, int H, int Hk, int D, int rot,
+                           int interleaved, const int64_t* q_strides, const int64_t* k_strides, float eps, int dtype, int w_dtype, void* stream);
+int mmk_qk_norm_rotary_part_rows(int64_t rows, int D);
+int mmk_qk_norm_rotary_bwd(const void* q, const void* k, const void* qw, const void* kw, const float* table, int table_rows,
+                           const void* positions, int pos64, int64_t pos_sb, const void* dqo, const void* dko, void* dq, void* dk, void* dqw,
+                           void* dkw, float* q_part, float* k_part, int B, int L, int H, int Hk, int D, int rot, int interleaved,
+                           const int64_t* q_strides, const int64_t* k_strides, const int64_t* dq_strides, const int64_t* dk_strides, float eps,
+                           int dtype, int w_dtype, void* stream);
 
 #ifdef __cplusplus
 }

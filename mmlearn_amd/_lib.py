@@ -7,6 +7,7 @@ loudly (``RuntimeError``) when it is missing.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import subprocess
@@ -30,7 +31,7 @@ KERNEL_NAMES = [
     "match_ids", "pack_rows", "transpose", "sim_stats", "lse_reduce", "loss_combine", "sim_grad", "grad_gemm",
     "grad_finalize", "l2norm", "ijepa_loss_fwd", "ijepa_loss_bwd", "gather_rows", "scatter_rows", "pred_assemble",
     "pred_assemble_bwd", "ema_update", "mask_to_index", "layernorm_fwd", "layernorm_bwd", "activation", "attn_fwd", "attn_bwd", "wgrad", "recall_ranks", "clip_fused", "mlp_gemm",
-    "win_attn_fwd", "win_attn_bwd", "clip_bwd_fused",
+    "win_attn_fwd", "win_attn_bwd", "clip_bwd_fused", "qk_norm",
 ]
 
 
@@ -163,6 +164,12 @@ _SIGNATURES = {
     "mmk_cls_attn_bwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _f, _f, C.c_uint64, _vp, _vp],
     "mmk_attn_bwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _f, _f, C.c_uint64, _vp, _vp, _i, _vp],
 }
+_i64 = C.c_int64
+_SIGNATURES.update({
+    "mmk_qk_norm_rotary_fwd": [_vp] * 5 + [_i, _vp, _i, _i64, _vp, _vp] + [_i] * 7 + [_vp, _vp, _f, _i, _i, _vp],
+    "mmk_qk_norm_rotary_part_rows": [_i64, _i],
+    "mmk_qk_norm_rotary_bwd": [_vp] * 5 + [_i, _vp, _i, _i64] + [_vp] * 8 + [_i] * 7 + [_vp] * 4 + [_f, _i, _i, _vp],
+})
 _STR_FUNCS = {"mmk_last_error": [], "mmk_kernel_name": [_i]}
 EXPORTED_SYMBOLS = sorted(list(_SIGNATURES) + list(_STR_FUNCS))
 
@@ -234,6 +241,14 @@ def stream() -> int:
         return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     except AttributeError:  # private API moved: fall back to the public one
         return torch.cuda.current_stream().cuda_stream
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """``with on_device_of(t):`` -- make ``t``'s device current for a launch (``stream()`` is the current device's); free when it is."""
+    return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 # ------------------------------------------------------------------ profiling

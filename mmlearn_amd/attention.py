@@ -162,3 +162,75 @@ def register_hf_attention(name: str = "mmlearn_hip") -> str:
 
     AttentionInterface.register(name, hf_attention_forward)
     return name
+
+
+# ------------------------------------------------------------------ per-head norm of queries and keys with the position rotation
+def rotary_table(positions: int, dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """f32 ``[positions, dim]`` table for :func:`qk_norm_rotary`: ``dim / 2`` cosines, then ``dim / 2`` sines, of the angles
+    ``position * base ** (-2 i / dim)``, formed in float64 (in float32 the angle of position 100,000 is off by thousandths of a turn)."""
+    if positions < 0 or dim < 0 or dim % 2 or not base > 0:
+        raise ValueError("mmlearn_amd.rotary_table: need positions >= 0, an even dim >= 0 and base > 0")
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / max(dim, 1))
+    return torch.cat((angle.cos(), angle.sin()), 1).float().to(device)
+
+
+class _QKNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, table, positions, interleaved, eps):
+        ctx.save_for_backward(q, k, qw, kw, table, positions)
+        ctx.interleaved, ctx.eps = interleaved, eps
+        return K.qk_norm_rotary_fwd(q, k, qw, kw, table, positions, interleaved, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dqo, dko):
+        q, k, qw, kw, table, positions = ctx.saved_tensors
+        dqo, dko = (g if g.stride(-1) == 1 or g.shape[-1] == 1 else g.contiguous() for g in (dqo.to(q.dtype), dko.to(k.dtype)))
+        grads = K.qk_norm_rotary_bwd(q, k, qw, kw, table, positions, dqo, dko, ctx.interleaved, ctx.eps, ctx.needs_input_grad[2],
+                                     ctx.needs_input_grad[3])
+        return (*grads, None, None, None, None)
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                   rotary: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, interleaved: bool = False,
+                   eps: float = 1e-6):
+    """Per-head RMS norm of queries and keys and the rotation by their positions, one launch forward and one (plus the sum of the weights'
+    gradients) backward.  ``q`` ``[B, L, H, D]`` and ``k`` ``[B, L, Hk, D]`` (f32 / bf16 / f16, any strides with a contiguous last dim --
+    slices of a packed projection --, ``D`` even, at most 256) -> contiguous ``(q', k')`` of the same shapes, with
+    ``q' = R(position) (q_weight * q / sqrt(mean(q ** 2) + eps))``.  Weights: ``[D]``, f32 or of the operands' type, None = ones.
+    ``rotary``: a :func:`rotary_table` of even width ``<= D``; of a head's first ``rotary.shape[1]`` values the pairs ``(i, i + width / 2)``
+    turn (``interleaved``: ``(2 i, 2 i + 1)``), the others pass.  None: no rotation.  ``positions``: int32 / int64 ``[L]`` or ``[B, L]``, rows of
+    the table; None: ``0 .. L - 1``.  They are read on the device: a position outside the table makes its rows NaN.
+    Both passes may be captured into a HIP graph.  As with every autograd function, no output of an eager pass over the same leaves may be
+    alive then: it would keep the leaves' gradient nodes on that pass's stream."""
+    K.require_gpu(q, "query")
+    name = "mmlearn_amd.qk_norm_rotary"
+    if not (q.dim() == k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3] and q.dtype == k.dtype
+            and q.dtype in (torch.float32, torch.bfloat16, torch.float16)):
+        raise ValueError(f"{name}: need q [B, L, H, D] and k [B, L, Hk, D] of one type (float32, bfloat16 or float16)")
+    B, L, _, D = q.shape
+    if D % 2 or not 2 <= D <= 256 or any(t.stride(3) != 1 for t in (q, k)):
+        raise ValueError(f"{name}: the head dim must be even, at most 256, and contiguous")
+    for w in (q_weight, k_weight):
+        if w is not None and not (w.shape == (D,) and w.is_contiguous() and w.dtype in (torch.float32, q.dtype)):
+            raise ValueError(f"{name}: weights are contiguous [D] tensors, float32 or of the operands' type")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"{name}: both weights must have one type")
+    if rotary is not None:
+        if not (rotary.dim() == 2 and rotary.dtype == torch.float32 and rotary.is_contiguous() and rotary.shape[1] % 2 == 0
+                and rotary.shape[1] <= D and not rotary.requires_grad):
+            raise ValueError(f"{name}: rotary is a contiguous float32 [positions, width] table without gradient, its width even and at most the head dim")
+        if positions is None and rotary.shape[0] < L:
+            raise ValueError(f"{name}: the rotary table holds {rotary.shape[0]} positions, the sequence has {L}")
+        if rotary.shape[1] == 0:
+            rotary = None
+    elif positions is not None:
+        raise ValueError(f"{name}: positions are rows of a rotary table, and there is none")
+    if rotary is None:
+        positions = None
+    if positions is not None and not (positions.dtype in (torch.int32, torch.int64) and tuple(positions.shape) in ((L,), (B, L))
+                                      and (L <= 1 or positions.stride(-1) == 1)):
+        raise ValueError(f"{name}: positions are int32 or int64 [L] or [B, L] with a contiguous last dim")
+    if any(t is not None and t.device != q.device for t in (k, q_weight, k_weight, rotary, positions)):
+        raise ValueError(f"{name}: all operands must be on one device")
+    return _QKNormRotary.apply(q, k, q_weight, k_weight, rotary, positions, bool(interleaved), float(eps))

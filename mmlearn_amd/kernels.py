@@ -18,7 +18,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import COMPUTE_BF16, COMPUTE_F32, ClipDir, check, dtype_tag, ptr, require_gpu, stream
+from ._lib import COMPUTE_BF16, COMPUTE_F32, ClipDir, check, dtype_tag, on_device_of, ptr, require_gpu, stream
 
 MAX_DIRS_PER_CALL = 8
 
@@ -1304,3 +1304,56 @@ def attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tenso
     if packed:
         return dqkv
     return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2)
+
+
+# ------------------------------------------------------------------ per-head norm of queries and keys with the position rotation
+def _strides_blh(t: torch.Tensor):
+    """Element strides {batch, token, head} of a [B, L, H, D] view."""
+    return (C.c_int64 * 3)(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _qk_norm_operands(q, qw, kw, table, positions):
+    rot = 0 if table is None else table.shape[1]
+    rows = 0 if table is None else table.shape[0]
+    pos64 = int(positions is not None and positions.dtype == torch.int64)
+    pos_sb = positions.stride(0) if positions is not None and positions.dim() == 2 else 0
+    w = qw if qw is not None else kw
+    return rot, rows, pos64, pos_sb, dtype_tag(q.dtype if w is None else w.dtype)
+
+
+def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, qw: Optional[torch.Tensor], kw: Optional[torch.Tensor], table: Optional[torch.Tensor],
+                       positions: Optional[torch.Tensor], interleaved: bool, eps: float):
+    """q [B, L, H, D], k [B, L, Hk, D] views (last dim contiguous) -> contiguous (q', k').  csrc/qk_norm.hip."""
+    require_gpu(q)
+    B, L, H, D = q.shape
+    rot, rows, pos64, pos_sb, wdt = _qk_norm_operands(q, qw, kw, table, positions)
+    with on_device_of(q):
+        qo = torch.empty((B, L, H, D), dtype=q.dtype, device=q.device)
+        ko = torch.empty((B, L, k.shape[2], D), dtype=q.dtype, device=q.device)
+        check(_lib.lib().mmk_qk_norm_rotary_fwd(ptr(q), ptr(k), ptr(qw), ptr(kw), ptr(table), rows, ptr(positions), pos64, pos_sb, ptr(qo), ptr(ko),
+                                                B, L, H, k.shape[2], D, rot, int(interleaved), _strides_blh(q), _strides_blh(k), float(eps),
+                                                dtype_tag(q.dtype), wdt, stream()))
+    return qo, ko
+
+
+def qk_norm_rotary_bwd(q: torch.Tensor, k: torch.Tensor, qw: Optional[torch.Tensor], kw: Optional[torch.Tensor], table: Optional[torch.Tensor],
+                       positions: Optional[torch.Tensor], dqo: torch.Tensor, dko: torch.Tensor, interleaved: bool, eps: float,
+                       need_qw: bool = True, need_kw: bool = True):
+    """Backward of ``qk_norm_rotary_fwd`` -> (dq, dk contiguous, dqw, dkw or None), the weight gradients in the weights' type."""
+    require_gpu(q)
+    B, L, H, D = q.shape
+    Hk = k.shape[2]
+    rot, rows, pos64, pos_sb, wdt = _qk_norm_operands(q, qw, kw, table, positions)
+    with on_device_of(q):
+        dq = torch.empty((B, L, H, D), dtype=q.dtype, device=q.device)
+        dk = torch.empty((B, L, Hk, D), dtype=q.dtype, device=q.device)
+        dw, part = [None, None], [None, None]
+        for n, (w, need, h) in enumerate(((qw, need_qw, H), (kw, need_kw, Hk))):
+            if w is not None and need:
+                dw[n] = torch.empty_like(w) if B * L * (H + Hk) else torch.zeros_like(w)
+                part[n] = torch.empty((max(1, _lib.lib().mmk_qk_norm_rotary_part_rows(B * L * h, D)), D), dtype=torch.float32, device=q.device)
+        check(_lib.lib().mmk_qk_norm_rotary_bwd(ptr(q), ptr(k), ptr(qw), ptr(kw), ptr(table), rows, ptr(positions), pos64, pos_sb, ptr(dqo), ptr(dko),
+                                                ptr(dq), ptr(dk), ptr(dw[0]), ptr(dw[1]), ptr(part[0]), ptr(part[1]), B, L, H, Hk, D, rot,
+                                                int(interleaved), _strides_blh(q), _strides_blh(k), _strides_blh(dqo), _strides_blh(dko),
+                                                float(eps), dtype_tag(q.dtype), wdt, stream()))
+    return dq, dk, dw[0], dw[1]
