@@ -48,7 +48,7 @@ enum {
   MMK_K_IJEPA_LOSS_BWD, MMK_K_GATHER_ROWS, MMK_K_SCATTER_ROWS, MMK_K_PRED_ASSEMBLE, MMK_K_PRED_ASSEMBLE_BWD,
   MMK_K_EMA, MMK_K_MASK_INDEX, MMK_K_LAYERNORM_FWD, MMK_K_LAYERNORM_BWD, MMK_K_ACT, MMK_K_ATTN_FWD,
   MMK_K_ATTN_BWD, MMK_K_WGRAD, MMK_K_RECALL, MMK_K_CLIP_FUSED, MMK_K_MLP_GEMM, MMK_K_WIN_ATTN_FWD, MMK_K_WIN_ATTN_BWD, MMK_K_CLIP_BWD_FUSED,
-  MMK_K_QK_NORM, MMK_K_COUNT
+  MMK_K_QK_NORM, MMK_K_REL_ATTN_FWD, MMK_K_REL_ATTN_BWD, MMK_K_COUNT
 };
 int mmk_profile_enable(int on);          /* on=1 start recording (clears), on=0 stop */
 /* resolve recorded events (synchronises on them); fills count[k] and total_ms[k] for k < MMK_K_COUNT */
@@ -567,6 +567,47 @@ int mmk_qk_norm_rotary_bwd(const void* q, const void* k, const void* qw, const v
                            void* dkw, float* q_part, float* k_part, int B, int L, int H, int Hk, int D, int rot, int interleaved,
                            const int64_t* q_strides, const int64_t* k_strides, const int64_t* dq_strides, const int64_t* dk_strides, float eps,
                            int dtype, int w_dtype, void* stream);
+
+/* Attention with a learned relative position bias by buckets, any length (the reference's text towers are any HF model,
+ * mmlearn/modules/encoders/text.py:20-178; those with relative_attention_bias materialise [1, H, Lq, Lk] for it):
+ *   out = softmax(scale * q k^T + table[bucket(j - i - q_offset), h]) v  over the keys j that the mask (and with `causal`, j <= i + q_offset)
+ * keeps; a row without keys gives zeros.  q [B, H, Lq, D], k / v [B, Hk, Lk, D] (H a multiple of Hk): bf16 / f16 views by element strides
+ * {batch, head, row}, multiples of 8, 16-byte aligned; D 64 or 128.  out [B, Lq, H, D] contiguous; lse f32 [B, H, Lq] (base 2; NULL: not
+ * wanted) feeds the backward.
+ * Buckets: with bidirectional, distances j - i > 0 use the second half of them; else positive distances count as 0.  Within a side the
+ * first near_buckets hold one distance each, the next n_borders + 1 begin at near_buckets, borders[0], borders[1], .. (HOST memory,
+ * ascending); all distances from max_distance (1 .. 512) on fall into one bucket.  table: [buckets][H], f32 or the operands' type.
+ * mask: one of MMK_REL_MASK_* -- LEN: int [B] leading keys are kept; 8 / 32 / 64: [B, Lk] integers of that width with batch stride
+ * mask_stride, nonzero = kept.  Masked keys and values may hold anything.  q_offsets (int32 [B], device) overrides q_offset.
+ * ws: mmk_rel_attn_fwd_ws_floats() floats.
+ * Backward: out / dout [B, Lq, H, D] contiguous; dq / dk / dv contiguous [B, L, heads, D]; dtable [buckets][H] in table_dtype, NULL: not
+ * wanted; ws: mmk_rel_attn_bwd_ws_floats() floats.  All sums in a fixed order. */
+#define MMK_REL_MASK_NONE 0
+#define MMK_REL_MASK_LEN32 1
+#define MMK_REL_MASK_LEN64 2
+#define MMK_REL_MASK_8 3
+#define MMK_REL_MASK_32 4
+#define MMK_REL_MASK_64 5
+typedef struct {
+  const void *q, *k, *v;
+  const void* table;
+  const void* mask;
+  const int32_t* q_offsets;
+  const int32_t* borders;
+  int64_t q_strides[3], k_strides[3], v_strides[3];
+  int64_t mask_stride;
+  int32_t B, H, Hk, Lq, Lk, D;
+  int32_t dtype, table_dtype, mask_kind;
+  int32_t buckets, near_buckets, n_borders, max_distance, bidirectional;
+  int32_t causal, q_offset;
+  float scale;
+  int32_t pad;
+} mmk_rel_attn;
+int64_t mmk_rel_attn_fwd_ws_floats(const mmk_rel_attn* p);
+int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, float* lse, float* ws, void* stream);
+int64_t mmk_rel_attn_bwd_ws_floats(const mmk_rel_attn* p, int want_dtable);
+int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dtable,
+                     float* ws, void* stream);
 
 #ifdef __cplusplus
 }

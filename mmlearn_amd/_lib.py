@@ -32,6 +32,7 @@ KERNEL_NAMES = [
     "grad_finalize", "l2norm", "ijepa_loss_fwd", "ijepa_loss_bwd", "gather_rows", "scatter_rows", "pred_assemble",
     "pred_assemble_bwd", "ema_update", "mask_to_index", "layernorm_fwd", "layernorm_bwd", "activation", "attn_fwd", "attn_bwd", "wgrad", "recall_ranks", "clip_fused", "mlp_gemm",
     "win_attn_fwd", "win_attn_bwd", "clip_bwd_fused", "qk_norm",
+    "rel_attn_fwd", "rel_attn_bwd",
 ]
 
 
@@ -77,6 +78,16 @@ class EmaEntry(C.Structure):
 
     _fields_ = [("teacher", C.c_void_p), ("student", C.c_void_p), ("numel", C.c_int64),
                 ("teacher_dtype", C.c_int32), ("student_dtype", C.c_int32)]
+
+
+class RelAttn(C.Structure):
+    """mirror of ``mmk_rel_attn``"""
+
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "table", "mask", "q_offsets", "borders")]
+                + [(n, C.c_int64 * 3) for n in ("q_strides", "k_strides", "v_strides")] + [("mask_stride", C.c_int64)]
+                + [(n, C.c_int32) for n in ("B", "H", "Hk", "Lq", "Lk", "D", "dtype", "table_dtype", "mask_kind", "buckets", "near_buckets",
+                                            "n_borders", "max_distance", "bidirectional", "causal", "q_offset")]
+                + [("scale", C.c_float), ("pad", C.c_int32)])
 
 
 _vp, _i, _f = C.c_void_p, C.c_int, C.c_float
@@ -168,6 +179,10 @@ _i64 = C.c_int64
 _SIGNATURES.update({
     "mmk_qk_norm_rotary_fwd": [_vp] * 5 + [_i, _vp, _i, _i64, _vp, _vp] + [_i] * 7 + [_vp, _vp, _f, _i, _i, _vp],
     "mmk_qk_norm_rotary_part_rows": [_i64, _i],
+    "mmk_rel_attn_fwd_ws_floats": [_vp],
+    "mmk_rel_attn_fwd": [_vp] * 5,
+    "mmk_rel_attn_bwd_ws_floats": [_vp, _i],
+    "mmk_rel_attn_bwd": [_vp] * 10,
     "mmk_qk_norm_rotary_bwd": [_vp] * 5 + [_i, _vp, _i, _i64] + [_vp] * 8 + [_i] * 7 + [_vp] * 4 + [_f, _i, _i, _vp],
 })
 _STR_FUNCS = {"mmk_last_error": [], "mmk_kernel_name": [_i]}
@@ -200,7 +215,8 @@ def lib() -> C.CDLL:
             fn = getattr(l, name)
             fn.argtypes = args
             fn.restype = C.c_int
-        l.mmk_embedding_bwd_scratch_bytes.restype = C.c_int64
+        for name in ("mmk_embedding_bwd_scratch_bytes", "mmk_rel_attn_fwd_ws_floats", "mmk_rel_attn_bwd_ws_floats"):
+            getattr(l, name).restype = C.c_int64
         for name, args in _STR_FUNCS.items():
             fn = getattr(l, name)
             fn.argtypes = args

@@ -234,3 +234,85 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     if any(t is not None and t.device != q.device for t in (k, q_weight, k_weight, rotary, positions)):
         raise ValueError(f"{name}: all operands must be on one device")
     return _QKNormRotary.apply(q, k, q_weight, k_weight, rotary, positions, bool(interleaved), float(eps))
+
+
+# ------------------------------------------------------------------ attention with a learned relative position bias
+class _RelativeAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, key_mask, offsets, how):
+        q_offset = how["q_offset"] if offsets is None else offsets
+        out, lse = K.rel_attn_fwd(q, k, v, table, how["max_distance"], how["bidirectional"], how["scale"], how["causal"], key_mask, q_offset,
+                                  any(ctx.needs_input_grad[:4]))
+        ctx.save_for_backward(q, k, v, table, key_mask, offsets, out, lse)
+        ctx.how = how
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, key_mask, offsets, out, lse = ctx.saved_tensors
+        how = ctx.how
+        dout = dout.to(q.dtype).contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        grads = K.rel_attn_bwd(q, k, v, table, how["max_distance"], how["bidirectional"], how["scale"], how["causal"], key_mask,
+                               how["q_offset"] if offsets is None else offsets, out, lse, dout, ctx.needs_input_grad[3])
+        return (*grads, None, None, None)
+
+
+def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int = 128, bidirectional: bool = True,
+                       scale: Optional[float] = None, causal: bool = False, key_mask: Optional[torch.Tensor] = None, q_offset=0):
+    """``softmax(scale * q k^T + table[bucket(j - i)]) v`` with a learned bias per head for each bucket of distances (key minus query), and
+    its gradients, the table's included.  ``q`` ``[B, H, Lq, D]``, ``k`` / ``v`` ``[B, Hk, Lk, D]``: bf16 or f16, ``D`` 64 or 128, ``H`` a multiple
+    of ``Hk`` (key heads shared by neighbouring query heads), any lengths, any strides that are multiples of 8 with a contiguous last dim.
+    Returns ``[B, Lq, H, D]`` contiguous.
+
+    ``table`` ``[buckets, H]``, f32 or of the operands' type (HF's ``relative_attention_bias.weight``).  With ``bidirectional`` the first half of
+    the buckets serves keys at or before the query, the second half keys behind it; otherwise keys behind it count as distance 0.  Of a
+    side's buckets (at least 2, at most 128) the first half holds one distance each, the others widen with the logarithm up to
+    ``max_distance`` (above the number of single distances where there are more than two, at most 512), beyond which all distances share the last one.
+
+    ``key_mask``: ``[B, Lk]`` bool / uint8 / int32 / int64 with nonzero = attended, or int32 / int64 ``[B]`` numbers of leading keys.  What masked
+    keys and values hold does not matter.  ``causal``: only keys ``j <= i + q_offset``.  ``q_offset``: position of query 0 among the keys, an int
+    or an int32 tensor ``[B]`` (one token against a cache: the number of keys before it).  A row that nothing is left for gives zeros and
+    passes no gradient.
+
+    The table's gradient is summed in f32 from scores whose softmax correction comes from the 16-bit output, so it is as exact as a
+    16-bit gradient also for an f32 table.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive."""
+    K.require_gpu(q, "query")
+    name = "mmlearn_amd.relative_attention"
+    if not (q.dim() == k.dim() == v.dim() == 4 and q.dtype in (torch.bfloat16, torch.float16) and q.dtype == k.dtype == v.dtype):
+        raise ValueError(f"{name}: need 4-dimensional q, k, v of one type, bfloat16 or float16")
+    B, H, _, D = q.shape
+    if not (k.shape == v.shape and k.shape[0] == B and k.shape[3] == D and D in (64, 128) and k.shape[1] >= 1 and H >= 1 and H % k.shape[1] == 0):
+        raise ValueError(f"{name}: need q [B, H, Lq, D], k and v [B, Hk, Lk, D], D 64 or 128, H a multiple of Hk")
+    for t in (q, k, v):
+        if t.stride(3) != 1 or any(s % 8 for s in K._strides_bhl(t)) or t.data_ptr() % 16 or K._strides_bhl(t)[2] > 1 << 23:
+            raise ValueError(f"{name}: operands need a contiguous last dim, strides that are multiples of 8 (rows: at most 2^23) and 16-byte alignment")
+    if max(q.shape[2], k.shape[2]) > 1 << 28:
+        raise ValueError(f"{name}: at most 2^28 rows")
+    buckets = table.shape[0] if table.dim() == 2 else 0
+    if not (table.dim() == 2 and table.shape[1] == H and table.is_contiguous() and table.dtype in (torch.float32, q.dtype)):
+        raise ValueError(f"{name}: table is a contiguous [buckets, H] tensor, float32 or of the operands' type")
+    side = buckets // 2 if bidirectional else buckets
+    if not 2 <= side <= 128 or (bidirectional and buckets % 2):
+        raise ValueError(f"{name}: need 2 to 128 buckets a side, an even number of them if bidirectional; got {buckets}")
+    least = side // 2 + (side > 2)   # (two buckets a side: distance 0 and the rest, no logarithm)
+    if not (isinstance(max_distance, int) and least <= max_distance <= 512):
+        raise ValueError(f"{name}: max_distance must be an int of at least {least} and at most 512")
+    if key_mask is not None:
+        if (key_mask.dim(), key_mask.dtype) not in K._REL_MASKS or tuple(key_mask.shape) != ((B,) if key_mask.dim() == 1 else (B, k.shape[2])):
+            raise ValueError(f"{name}: key_mask is [B, Lk] bool / uint8 / int32 / int64, or int32 / int64 [B] lengths")
+        if key_mask.shape[-1] > 1 and key_mask.stride(-1) != 1:
+            raise ValueError(f"{name}: key_mask needs a contiguous last dim")
+    offsets = q_offset if isinstance(q_offset, torch.Tensor) else None
+    if offsets is not None and not (offsets.dtype == torch.int32 and offsets.shape == (B,) and offsets.is_contiguous()):
+        raise ValueError(f"{name}: q_offset is an int or a contiguous int32 [B] tensor")
+    if offsets is None and not (isinstance(q_offset, int) and abs(q_offset) < 1 << 29):
+        raise ValueError(f"{name}: q_offset is an int below 2^29 in size, or an int32 [B] tensor")
+    if any(t is not None and t.device != q.device for t in (k, v, table, key_mask, offsets)):
+        raise ValueError(f"{name}: all operands must be on one device")
+    scale = D ** -0.5 if scale is None else float(scale)
+    how = {"max_distance": max_distance, "bidirectional": bool(bidirectional), "scale": scale, "causal": bool(causal),
+           "q_offset": 0 if offsets is not None else q_offset}
+    return _RelativeAttention.apply(q, k, v, table, key_mask, offsets, how)

@@ -1,0 +1,1086 @@
+// Attention with a learned relative position bias by buckets, for any length:
+//
+//   s_ij = scale q_i . k_j + table[bucket(j - i - off), h],   P = softmax over the kept keys j,   o_i = sum_j P_ij v_j
+//   backward:  dP = dO V^T,  delta_i = dO_i . o_i,  dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,
+//              dtable[c, h] = sum over all samples and all (i, j) with bucket c of dS
+//
+// The bias depends on the distance alone and is constant beyond max_distance, so it never exists as a matrix: a workgroup keeps one head's
+// bias as a vector over the distances -max_distance .. max_distance in LDS, tiles that lie wholly beyond it take one scalar, and the
+// backward sums dS of near tiles along their diagonals in LDS, of far tiles in registers.
+//
+// Matrix products run on v_mfma_f32_32x32x16 with the softmax axis across the accumulator registers: S^T = K Q^T has the query on the
+// lane, so the running maximum, the sum and the rescale of O^T are lane-local, and the exponentiated accumulators are the B operand
+// of O^T = V^T P^T as they stand (csrc/attention.hip uses the same forms for whole heads on chip; attn_image.h has the images).  K / V (or
+// Q / dO) tiles of 64 rows go to LDS by LDS-DMA, double-buffered, one barrier a tile.  P and dS are rounded to the operands' type for their
+// products -- the matrix unit takes 16-bit operands; statistics, sums, accumulators and the table's gradient stay in f32, and
+// delta is formed from the rounded o, as everything the backward knows of o.
+#include <hip/hip_ext.h>
+#include <limits.h>
+
+#include <algorithm>
+
+#include "attn_image.h"
+#include "common.h"
+
+namespace mmk {
+
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int REL_MAX_BORDERS = 64;
+constexpr int REL_MAX_BUCKETS = 256;
+constexpr int REL_MAX_FAR = 512;
+constexpr float REL_LOG2E = 1.4426950408889634f;
+
+struct RelArgs {
+  const void *q, *k, *v;
+  int64_t q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;   // element strides of [B, H, L, D] views
+  void* out;       // [B, Lq, H, D] contiguous
+  float* lse;      // [B, H, Lq], base 2 of the biased scores; +inf for a row without keys; may be null
+  int B, H, Hk, G, Lq, Lk;   // G = H / Hk query heads share a key head
+  float scale, sl2;          // sl2 = scale log2 e
+  const void* table;         // [buckets][H]
+  int table_f32, buckets, side, near, far, bidir, n_borders;
+  int causal, off;
+  const int32_t* off_ptr;    // per-sample offsets, or null
+  const void* mask;
+  int64_t mask_sb;
+  int mask_kind;             // MMK_REL_MASK_*
+  // backward
+  const void* dout;          // [B, Lq, H, D] contiguous
+  const void* o;
+  void *dq, *dk, *dv;        // contiguous [B, L, heads, D]
+  float *delta, *dtab_part;  // [B, H, Lq]; [workgroups of the dQ kernel][buckets] or null
+  // split forward
+  float* part;               // partial results of the key splits
+  int splits, row_blocks;
+  int borders[REL_MAX_BORDERS];   // smallest distance of the 2nd, 3rd, .. logarithmic bucket
+};
+
+template <typename T>
+__device__ __forceinline__ f32x16 rel_mfma(s16x8 a, s16x8 b, f32x16 c);
+template <>
+__device__ __forceinline__ f32x16 rel_mfma<bf16_t>(s16x8 a, s16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x16 rel_mfma<f16_t>(s16x8 a, s16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ s16x8 rel_row_frag(const char* p) { return *reinterpret_cast<const s16x8*>(p); }
+__device__ __forceinline__ s16x8 rel_tr_frag(const char* img, const ImgLane& il, int off, int ct) {
+  return __builtin_bit_cast(s16x8, lds_tr_frag(img, il, off, ct));
+}
+// eight accumulator registers (one k step) as a B operand
+template <typename T>
+__device__ __forceinline__ s16x8 rel_operand(const f32x16& x, int s) {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  t8 o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = from_f32<T>(x[8 * s + e]);
+  return __builtin_bit_cast(s16x8, o);
+}
+__device__ __forceinline__ f32x16 rel_zero() {
+  f32x16 z;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  return z;
+}
+// accumulator register e of a lane in half h is row (e & 3) + 8 (e >> 2) + 4 h of the tile
+__device__ __forceinline__ constexpr int acc_row(int e) { return (e & 3) + 8 * (e >> 2); }
+
+// the same value of the lane 32 away
+__device__ __forceinline__ float rel_other_half(float v) { return __shfl_xor(v, 32); }
+
+__device__ __forceinline__ int rel_bucket(const RelArgs& a, int rel) {
+  const int dist = a.bidir ? abs(rel) : max(-rel, 0);
+  const int base = a.bidir && rel > 0 ? a.side : 0;
+  if (dist < a.near) return base + dist;
+  int b = base + a.near;
+  for (int t = 0; t < a.n_borders; ++t) b += dist >= a.borders[t];
+  return b;
+}
+__device__ __forceinline__ float rel_table(const RelArgs& a, int bucket, int h, bf16_t) {
+  const int64_t at = (int64_t)bucket * a.H + h;
+  return a.table_f32 ? reinterpret_cast<const float*>(a.table)[at] : (float)reinterpret_cast<const bf16_t*>(a.table)[at];
+}
+__device__ __forceinline__ float rel_table(const RelArgs& a, int bucket, int h, f16_t) {
+  const int64_t at = (int64_t)bucket * a.H + h;
+  return a.table_f32 ? reinterpret_cast<const float*>(a.table)[at] : (float)reinterpret_cast<const f16_t*>(a.table)[at];
+}
+// bias[x] of the distance x - far - ext, in base-2 units; distances beyond `far` on either side (ext of them) repeat the last one, so that a
+// tile that reaches beyond needs no clamp
+template <typename T>
+__device__ __forceinline__ void rel_bias_fill(const RelArgs& a, float* bias, int ext, int h, int tid, int nt) {
+  const int n = 2 * (a.far + ext) + 1;
+  for (int x = tid; x < n; x += nt) {
+    const int rel = min(max(x - a.far - ext, -a.far), a.far);
+    bias[x] = rel_table(a, rel_bucket(a, rel), h, T()) * REL_LOG2E;
+  }
+}
+
+__device__ __forceinline__ int rel_offset(const RelArgs& a, int b) {
+  const int o = a.off_ptr ? a.off_ptr[b] : a.off;
+  return min(max(o, -(1 << 29)), 1 << 29);   // (distances stay within 32 bits; far beyond every bucket border)
+}
+// how many leading keys of the sample can be kept at all
+__device__ __forceinline__ int rel_key_len(const RelArgs& a, int b) {
+  int64_t n = a.Lk;
+  if (a.mask_kind == MMK_REL_MASK_LEN32) n = reinterpret_cast<const int32_t*>(a.mask)[b];
+  if (a.mask_kind == MMK_REL_MASK_LEN64) n = reinterpret_cast<const int64_t*>(a.mask)[b];
+  return (int)(n < 0 ? 0 : n < a.Lk ? n : a.Lk);
+}
+// whether the mask keeps key j (1 where there is no per-key mask); j may lie past the end
+__device__ __forceinline__ int rel_mask_at(const RelArgs& a, int b, int j) {
+  if (a.mask_kind < MMK_REL_MASK_8) return 1;
+  const int64_t at = (int64_t)b * a.mask_sb + min(j, a.Lk - 1);
+  if (a.mask_kind == MMK_REL_MASK_8) return reinterpret_cast<const uint8_t*>(a.mask)[at] != 0;
+  if (a.mask_kind == MMK_REL_MASK_32) return reinterpret_cast<const int32_t*>(a.mask)[at] != 0;
+  return reinterpret_cast<const int64_t*>(a.mask)[at] != 0;
+}
+
+// blockIdx -> work item, so that neighbouring items (the query blocks of one head) run on one XCD and share its L2
+__device__ __forceinline__ int rel_item(int id, int total) {
+  const int per = total >> 3;
+  return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
+}
+
+// One wave's share of a 64-row tile in LDS: CB column blocks of 64 of X, then of Y, 8 pieces of 8 rows each
+template <typename T, int CB, int NW>
+struct RelLoader {
+  uint32_t vx[2], vy[2];
+  __device__ __forceinline__ RelLoader(int64_t x_sl, int64_t y_sl, int wave, int lane) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = 8 * ((wave + NW * u) & 7) + (lane >> 3), ch = (lane & 7) ^ img_swz(row & 15);
+      vx[u] = (uint32_t)(row * (int)x_sl + ch * 8) * 2u;
+      vy[u] = (uint32_t)(row * (int)y_sl + ch * 8) * 2u;
+    }
+  }
+  // rows row0 .. row0 + 63 of X and Y (rows past `rows - 1` repeat that row), to the stage at `lds`
+  __device__ __forceinline__ void issue(const T* x, const T* y, int64_t x_sl, int64_t y_sl, int row0, int rows, uint32_t lds, int wave,
+                                        int lane) const {
+    static_assert(NW == 4, "two pieces of an image per wave");
+    const bool whole = row0 + 64 <= rows;
+#pragma unroll
+    for (int im = 0; im < 2 * CB; ++im) {
+      const int64_t sl = im < CB ? x_sl : y_sl;
+      const T* base = (im < CB ? x : y) + (int64_t)row0 * sl + 64 * (im % CB);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int piece = wave + NW * u;
+        uint32_t vo = im < CB ? vx[u] : vy[u];
+        if (!whole) {
+          const int row = 8 * piece + (lane >> 3), ch = (lane & 7) ^ img_swz(row & 15);
+          vo = (uint32_t)(min(row, rows - 1 - row0) * (int)sl + ch * 8) * 2u;
+        }
+        lds_dma16(base, vo, lds + (uint32_t)(im * 8192 + piece * 1024));
+      }
+    }
+  }
+};
+
+// rows of `img` (CB images of 64 rows) whose bit in `word` is clear become zero: a masked key may hold anything, and 0 * NaN is NaN
+template <int CB>
+__device__ __forceinline__ void rel_zero_rows(char* img, uint64_t word, int wave, int lane) {
+  const int row = 16 * wave + (lane >> 2);
+  if (!((word >> row) & 1)) {
+    const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      uint4* p = reinterpret_cast<uint4*>(img + cb * 8192 + row * 128 + (lane & 3) * 32);
+      p[0] = z;
+      p[1] = z;
+    }
+  }
+}
+
+// D^T accumulators (lane = row, registers = columns) -> row `row` of a contiguous-row tensor
+template <typename T, int D>
+__device__ __forceinline__ void rel_store_row(T* row, const f32x16 (&o)[D / 32], float mul, int h) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      t4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(o[dt][4 * g + e] * mul);
+      *reinterpret_cast<t4*>(row + 32 * dt + 8 * g + 4 * h) = w;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// Workgroup: 4 waves x NQ x 32 queries of one (sample, head); tiles of 64 keys.
+template <typename T, int D, int NQ>
+__global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, QB = 128 * NQ, EXT = 64 + 32 * NQ;
+  float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, hf = lane >> 5;
+  const int nqb = (a.Lq + QB - 1) / QB, item = rel_item(blockIdx.x, gridDim.x);
+  const int bh = item / nqb, b = bh / a.H, h = bh - b * a.H;
+  const int qb = a.causal ? nqb - 1 - (item - bh * nqb) : item - bh * nqb;   // causal: the longest rows first
+  const int off = rel_offset(a, b), klen = rel_key_len(a, b);
+  const int i_wg = qb * QB, i_wave = i_wg + 32 * NQ * wave;
+  int nkt = (klen + 63) / 64;
+  if (a.causal) {
+    const int last = min(klen - 1, min(i_wg + QB, a.Lq) - 1 + off);
+    nkt = last < 0 ? 0 : last / 64 + 1;
+  }
+  const T* kp = reinterpret_cast<const T*>(a.k) + b * a.k_sb + (h / a.G) * a.k_sh;
+  const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + (h / a.G) * a.v_sh;
+  rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
+
+  s16x8 qf[NQ][D / 16];
+  f32x16 o[NQ][D / 32];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int s = 0; s < NQ; ++s) {
+    const int i = min(i_wave + 32 * s + r, a.Lq - 1);
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + i * a.q_sl + 8 * hf;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) qf[s][kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) o[s][dt] = rel_zero();
+    m[s] = -INFINITY;
+    l[s] = 0.f;
+  }
+  const ImgLane il = img_lane(lane);
+  const RelLoader<T, CB, 4> ld(a.k_sl, a.v_sl, wave, lane);
+  const uint32_t lds0 = lds_addr_of(smem);
+  int keep = 1;
+  if (nkt > 0) {
+    ld.issue(kp, vp, a.k_sl, a.v_sl, 0, a.Lk, lds0, wave, lane);
+    keep = rel_mask_at(a, b, lane);
+  }
+  for (int kt = 0; kt < nkt; ++kt) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this tile and its mask are here
+    __syncthreads();
+    const int j0 = 64 * kt;
+    const uint64_t word = __ballot(j0 + lane < klen && keep);
+    if (kt + 1 < nkt) {
+      ld.issue(kp, vp, a.k_sl, a.v_sl, j0 + 64, a.Lk, lds0 + ((kt + 1) & 1) * STAGE, wave, lane);
+      keep = rel_mask_at(a, b, j0 + 64 + lane);
+    }
+    if (word == 0) continue;
+    char* K = smem + (kt & 1) * STAGE;
+    char* V = K + CB * 8192;
+    if (~word) {
+      rel_zero_rows<CB>(V, word, wave, lane);
+      __syncthreads();
+    }
+    if (i_wave >= a.Lq || (a.causal && j0 > i_wave + 32 * NQ - 1 + off)) continue;   // no row, or no key of the tile, for this wave
+    f32x16 s[NQ][2];
+#pragma unroll
+    for (int qs = 0; qs < NQ; ++qs) s[qs][0] = s[qs][1] = rel_zero();
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const s16x8 kf = rel_row_frag(K + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]);
+#pragma unroll
+        for (int qs = 0; qs < NQ; ++qs) s[qs][t] = rel_mfma<T>(kf, qf[qs][kk], s[qs][t]);
+      }
+    const int rel_hi = j0 + 63 - (i_wave + off), rel_lo = j0 - (i_wave + 32 * NQ - 1 + off);
+    const bool masked = ~word || (a.causal && rel_hi > 0);
+    s16x8 pf[NQ][4];
+#pragma unroll
+    for (int qs = 0; qs < NQ; ++qs) {
+      const int ip = i_wave + 32 * qs + r + off;   // this lane's query position
+      if (rel_hi <= -a.far || rel_lo >= a.far) {
+        const float c = bias[rel_hi <= -a.far ? 0 : 2 * (a.far + EXT)];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[qs][t][e] = fmaf(s[qs][t][e], a.sl2, c);
+      } else {
+        const float* bp = bias + (a.far + EXT + j0 + 4 * hf - ip);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[qs][t][e] = fmaf(s[qs][t][e], a.sl2, bp[32 * t + acc_row(e)]);
+      }
+      if (masked) {
+        const int jmax = a.causal ? ip - j0 - 4 * hf : INT_MAX;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t w = (uint32_t)(word >> (32 * t)) >> (4 * hf);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!((w >> acc_row(e)) & 1) || 32 * t + acc_row(e) > jmax) s[qs][t][e] = -INFINITY;
+        }
+      }
+      float mt = s[qs][0][0];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[qs][t][e]);
+      mt = fmaxf(mt, rel_other_half(mt));
+      // the running maximum moves only when it grows by more than 2^8: until then the sums stay exact enough in f32 and the
+      // rescale of O is skipped for the whole wave
+      if (__any(mt > m[qs] + 8.f)) {
+        const float mn = fmaxf(m[qs], mt);
+        const float alpha = mn == m[qs] ? 1.f : att_exp2(m[qs] - mn);
+        m[qs] = mn;
+        l[qs] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[qs][dt][e] *= alpha;
+      }
+      const float nm = m[qs] == -INFINITY ? 0.f : -m[qs];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[qs][t][e] = att_exp2(s[qs][t][e] + nm);
+          l[qs] += s[qs][t][e];
+        }
+        pf[qs][2 * t] = rel_operand<T>(s[qs][t], 0);
+        pf[qs][2 * t + 1] = rel_operand<T>(s[qs][t], 1);
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const s16x8 vf = rel_tr_frag(V + (dt >> 1) * 8192, il, st * 2048, dt & 1);
+#pragma unroll
+        for (int qs = 0; qs < NQ; ++qs) o[qs][dt] = rel_mfma<T>(vf, pf[qs][st], o[qs][dt]);
+      }
+  }
+#pragma unroll
+  for (int qs = 0; qs < NQ; ++qs) {
+    const int i = i_wave + 32 * qs + r;
+    const float sum = l[qs] + rel_other_half(l[qs]);
+    if (i < a.Lq) {
+      rel_store_row<T, D>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + h) * D, o[qs], sum > 0.f ? 1.f / sum : sum, hf);
+      if (a.lse && hf == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : m[qs] + log2f(sum);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ forward, few rows
+// One workgroup per (sample, key head, block of 32 rows, split of the keys).  Row = query head of the group x query; all rows of a block
+// share every key tile, so the keys are read once for the whole group.  The four waves walk tiles of 32 keys of their own, each through
+// LDS of its own without barriers, and are joined at the end; splits are joined by rel_join_kernel.  Bound by the K / V bytes.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int CB = D / 64, IMG = 4096, STAGE = 2 * CB * IMG, EXT = 1;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, hf = lane >> 5;
+  char* mine = smem + wave * 2 * STAGE;
+  float* bias_all = reinterpret_cast<float*>(smem + 8 * STAGE);
+  const int nb = 2 * (a.far + EXT) + 1;
+  const int split = blockIdx.x % a.splits, blk = (blockIdx.x / a.splits) % a.row_blocks, bk = blockIdx.x / a.splits / a.row_blocks;
+  const int b = bk / a.Hk, hk = bk - b * a.Hk;
+  const int rows = a.G * a.Lq, row = blk * 32 + r;
+  const int rc = min(row, rows - 1), g = rc / a.Lq, i = rc - g * a.Lq, h = hk * a.G + g;
+  const int g0 = blk * 32 / a.Lq, g1 = min(blk * 32 + 31, rows - 1) / a.Lq;   // heads of this block
+  const int off = rel_offset(a, b), klen = rel_key_len(a, b), ip = i + off;
+  for (int gg = g0; gg <= g1; ++gg) rel_bias_fill<T>(a, bias_all + (gg - g0) * nb, EXT, hk * a.G + gg, tid, 256);
+  const float* bias = bias_all + (g - g0) * nb + a.far + EXT;
+  // tiles of this split: the sample's own length is divided, so that short samples do not leave splits idle
+  int last = klen - 1;
+  if (a.causal) last = min(last, a.Lq - 1 + off);
+  const int tiles = last < 0 ? 0 : last / 32 + 1, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = split * per + wave, t1 = min((split + 1) * per, tiles);
+  const T* kp = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+  const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+  s16x8 qf[D / 16];
+  f32x16 o[D / 32];
+  {
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + i * a.q_sl + 8 * hf;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) qf[kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_zero();
+  }
+  float m = -INFINITY, l = 0.f;
+  const ImgLane il = img_lane(lane);
+  const uint32_t lds0 = lds_addr_of(mine);
+  auto issue = [&](int t, int stage) {
+#pragma unroll
+    for (int im = 0; im < 2 * CB; ++im) {
+      const int64_t sl = im < CB ? a.k_sl : a.v_sl;
+      const T* base = (im < CB ? kp : vp) + (int64_t)(32 * t) * sl + 64 * (im % CB);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int rw = 8 * p + (lane >> 3), ch = (lane & 7) ^ img_swz(rw & 15);
+        lds_dma16(base, (uint32_t)(min(rw, a.Lk - 1 - 32 * t) * (int)sl + ch * 8) * 2u, lds0 + (uint32_t)(stage * STAGE + im * IMG + p * 1024));
+      }
+    }
+  };
+  __syncthreads();   // the bias vectors
+  int keep = 1;
+  if (t0 < t1) {
+    issue(t0, 0);
+    keep = rel_mask_at(a, b, 32 * t0 + r);
+  }
+  int stage = 0;
+  for (int t = t0; t < t1; t += 4, stage ^= 1) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    asm volatile("" ::: "memory");
+    const int j0 = 32 * t;
+    const uint32_t word = (uint32_t)__ballot(j0 + r < klen && keep);
+    if (t + 4 < t1) {
+      issue(t + 4, stage ^ 1);
+      keep = rel_mask_at(a, b, j0 + 128 + r);
+    }
+    if (word == 0) continue;
+    char* K = mine + stage * STAGE;
+    char* V = K + CB * IMG;
+    if (~word && !((word >> r) & 1)) {   // (both halves of a lane pair clear one half of the row each)
+      const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(V + cb * IMG + r * 128 + hf * 64 + c * 16) = z;
+    }
+    f32x16 s = rel_zero();
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) s = rel_mfma<T>(rel_row_frag(K + (kk >> 2) * IMG + il.row[kk & 3]), qf[kk], s);
+    const uint32_t w = word >> (4 * hf);
+    const int rel0 = j0 + 4 * hf - ip, jmax = a.causal ? -rel0 : INT_MAX;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      s[e] = fmaf(s[e], a.sl2, bias[min(max(rel0 + acc_row(e), -a.far), a.far)]);
+      if (!((w >> acc_row(e)) & 1) || acc_row(e) > jmax) s[e] = -INFINITY;
+      mt = fmaxf(mt, s[e]);
+    }
+    mt = fmaxf(mt, rel_other_half(mt));
+    if (__any(mt > m + 8.f)) {
+      const float mn = fmaxf(m, mt);
+      const float alpha = mn == m ? 1.f : att_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+    }
+    const float nm = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      s[e] = att_exp2(s[e] + nm);
+      l += s[e];
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const s16x8 pf = rel_operand<T>(s, st);
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_mfma<T>(rel_tr_frag(V + (dt >> 1) * IMG, il, st * 2048, dt & 1), pf, o[dt]);
+    }
+  }
+  l += rel_other_half(l);
+  // ---- join the waves: [wave][32 rows] of (m, l), then O row by row
+  __syncthreads();
+  float* ml = reinterpret_cast<float*>(smem);               // [4][2][32]
+  float* ob = reinterpret_cast<float*>(smem + 1024);         // [4][32][D + 4]
+  if (hf == 0) {
+    ml[wave * 64 + r] = m;
+    ml[wave * 64 + 32 + r] = l;
+  }
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+      *reinterpret_cast<float4*>(ob + (wave * 32 + r) * (D + 4) + 32 * dt + 8 * q4 + 4 * hf) =
+          make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
+  __syncthreads();
+  const int n_rows = min(32, rows - blk * 32);
+  for (int x = tid; x < n_rows * (D / 4); x += 256) {
+    const int rr = x / (D / 4), d = 4 * (x - rr * (D / 4));
+    float mm = -INFINITY, ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int wv = 0; wv < 4; ++wv) mm = fmaxf(mm, ml[wv * 64 + rr]);
+#pragma unroll
+    for (int wv = 0; wv < 4; ++wv) {
+      const float mw = ml[wv * 64 + rr];
+      const float f = mw == -INFINITY ? 0.f : att_exp2(mw - mm);
+      const float4 v4 = *reinterpret_cast<const float4*>(ob + (wv * 32 + rr) * (D + 4) + d);
+      ll += f * ml[wv * 64 + 32 + rr];
+      acc.x += f * v4.x;
+      acc.y += f * v4.y;
+      acc.z += f * v4.z;
+      acc.w += f * v4.w;
+    }
+    const int64_t prow = ((int64_t)bk * a.row_blocks + blk) * 32 + rr;
+    if (a.splits > 1) {
+      float* p = a.part + (prow * a.splits + split) * (D + 4);   // [.., D] sums, then (m, l)
+      *reinterpret_cast<float4*>(p + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(p + D) = make_float2(mm, ll);
+    } else {
+      const int ro = blk * 32 + rr, go = ro / a.Lq, io = ro - go * a.Lq, ho = hk * a.G + go;
+      const float f = ll > 0.f ? 1.f / ll : ll;
+      Vec4<T>::store(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Lq + io) * a.H + ho) * D + d,
+                     make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+      if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm + log2f(ll);
+    }
+  }
+}
+
+// one group of D / 4 threads per row
+template <typename T, int D>
+__global__ __launch_bounds__(256) void rel_join_kernel(const RelArgs a) {
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int rows = a.G * a.Lq;
+  const int64_t row = x / (D / 4);
+  const int d = 4 * (int)(x - row * (D / 4));
+  const int bk = (int)(row / rows), ro = (int)(row - (int64_t)bk * rows);
+  if (bk >= a.B * a.Hk) return;
+  const int b = bk / a.Hk, hk = bk - b * a.Hk, go = ro / a.Lq, io = ro - go * a.Lq, ho = hk * a.G + go;
+  const float* p = a.part + ((int64_t)bk * a.row_blocks * 32 + ro) * a.splits * (D + 4);
+  float mm = -INFINITY, ll = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, p[s * (D + 4) + D]);
+  for (int s = 0; s < a.splits; ++s) {
+    const float ms = p[s * (D + 4) + D];
+    const float f = ms == -INFINITY ? 0.f : att_exp2(ms - mm);
+    const float4 v4 = *reinterpret_cast<const float4*>(p + s * (D + 4) + d);
+    ll += f * p[s * (D + 4) + D + 1];
+    acc.x += f * v4.x;
+    acc.y += f * v4.y;
+    acc.z += f * v4.z;
+    acc.w += f * v4.w;
+  }
+  const float f = ll > 0.f ? 1.f / ll : ll;
+  Vec4<T>::store(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm + log2f(ll);
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dQ, delta, dtable
+// As the forward, with the query on the lane: dS^T needs lse and delta of the lane alone, and dQ^T += K^T dS^T takes it from the
+// accumulators.  dtable: the 32 lanes of a half hold 32 consecutive distances in each register, so each wave half adds them to a vector
+// over the distances of its own (one address per lane: the order of the sums is fixed); tiles beyond max_distance add to two
+// registers.
+template <typename T, int D, int NQ>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, QB = 128 * NQ, EXT = 32 + 32 * NQ;
+  float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
+  const int nbias = (2 * (a.far + EXT) + 1 + 3) & ~3;
+  float* diag = bias + nbias;   // [8][nbias]: per wave half
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, hf = lane >> 5;
+  const int nqb = (a.Lq + QB - 1) / QB, item = rel_item(blockIdx.x, gridDim.x);
+  const int bh = item / nqb, b = bh / a.H, h = bh - b * a.H;
+  const int qb = a.causal ? nqb - 1 - (item - bh * nqb) : item - bh * nqb;
+  const int off = rel_offset(a, b), klen = rel_key_len(a, b);
+  const int i_wg = qb * QB, i_wave = i_wg + 32 * NQ * wave;
+  int nkt = (klen + 63) / 64;
+  if (a.causal) {
+    const int last = min(klen - 1, min(i_wg + QB, a.Lq) - 1 + off);
+    nkt = last < 0 ? 0 : last / 64 + 1;
+  }
+  const T* kp = reinterpret_cast<const T*>(a.k) + b * a.k_sb + (h / a.G) * a.k_sh;
+  const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + (h / a.G) * a.v_sh;
+  rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
+  if (a.dtab_part)
+    for (int x = tid; x < 8 * nbias; x += 256) diag[x] = 0.f;
+  float* my_diag = diag + (2 * wave + hf) * nbias;
+
+  s16x8 qf[NQ][D / 16], gf[NQ][D / 16];
+  f32x16 dq[NQ][D / 32];
+  float lse[NQ], delta[NQ], far_l = 0.f, far_r = 0.f;
+#pragma unroll
+  for (int s = 0; s < NQ; ++s) {
+    const int i = i_wave + 32 * s + r, ic = min(i, a.Lq - 1);
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + ic * a.q_sl + 8 * hf;
+    const int64_t orow = (((int64_t)b * a.Lq + ic) * a.H + h) * D + 8 * hf;
+    const T* gp = reinterpret_cast<const T*>(a.dout) + orow;
+    const T* op = reinterpret_cast<const T*>(a.o) + orow;
+    float dl = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      qf[s][kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
+      gf[s][kk] = *reinterpret_cast<const s16x8*>(gp + 16 * kk);
+      const t8 g8 = __builtin_bit_cast(t8, gf[s][kk]), o8 = *reinterpret_cast<const t8*>(op + 16 * kk);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dl = fmaf(to_f32(g8[e]), to_f32(o8[e]), dl);
+    }
+    dl += rel_other_half(dl);
+    const int64_t at = ((int64_t)b * a.H + h) * a.Lq + ic;
+    lse[s] = i < a.Lq ? a.lse[at] : INFINITY;
+    delta[s] = dl;
+    if (i < a.Lq && hf == 0) a.delta[at] = dl;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) dq[s][dt] = rel_zero();
+  }
+  const ImgLane il = img_lane(lane);
+  const RelLoader<T, CB, 4> ld(a.k_sl, a.v_sl, wave, lane);
+  const uint32_t lds0 = lds_addr_of(smem);
+  int keep = 1;
+  if (nkt > 0) {
+    ld.issue(kp, vp, a.k_sl, a.v_sl, 0, a.Lk, lds0, wave, lane);
+    keep = rel_mask_at(a, b, lane);
+  }
+  for (int kt = 0; kt < nkt; ++kt) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    const int j0 = 64 * kt;
+    const uint64_t word = __ballot(j0 + lane < klen && keep);
+    if (kt + 1 < nkt) {
+      ld.issue(kp, vp, a.k_sl, a.v_sl, j0 + 64, a.Lk, lds0 + ((kt + 1) & 1) * STAGE, wave, lane);
+      keep = rel_mask_at(a, b, j0 + 64 + lane);
+    }
+    if (word == 0) continue;
+    char* K = smem + (kt & 1) * STAGE;
+    char* V = K + CB * 8192;
+    if (~word) {
+      rel_zero_rows<CB>(K, word, wave, lane);
+      __syncthreads();
+    }
+    if (i_wave >= a.Lq || (a.causal && j0 > i_wave + 32 * NQ - 1 + off)) continue;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x16 s[NQ], dp[NQ];
+#pragma unroll
+      for (int qs = 0; qs < NQ; ++qs) s[qs] = dp[qs] = rel_zero();
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const s16x8 kf = rel_row_frag(K + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]);
+        const s16x8 vf = rel_row_frag(V + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]);
+#pragma unroll
+        for (int qs = 0; qs < NQ; ++qs) {
+          s[qs] = rel_mfma<T>(kf, qf[qs][kk], s[qs]);
+          dp[qs] = rel_mfma<T>(vf, gf[qs][kk], dp[qs]);
+        }
+      }
+      const int jt = j0 + 32 * t;
+      const int rel_hi = jt + 31 - (i_wave + off), rel_lo = jt - (i_wave + 32 * NQ - 1 + off);
+      const bool left = rel_hi <= -a.far, right = rel_lo >= a.far;
+      const uint32_t wt = (uint32_t)(word >> (32 * t));
+      const bool masked = ~wt || (a.causal && rel_hi > 0);
+      const uint32_t w = wt >> (4 * hf);
+      s16x8 df[NQ][2];
+#pragma unroll
+      for (int qs = 0; qs < NQ; ++qs) {
+        const int ip = i_wave + 32 * qs + r + off;
+        const int at0 = a.far + EXT + jt + 4 * hf - ip;   // (only used where the tile is near: within the vector)
+        if (left || right) {
+          const float c = bias[left ? 0 : 2 * (a.far + EXT)] - lse[qs];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[qs][e] = att_exp2(fmaf(s[qs][e], a.sl2, c));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[qs][e] = att_exp2(fmaf(s[qs][e], a.sl2, bias[at0 + acc_row(e)]) - lse[qs]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[qs][e] *= dp[qs][e] - delta[qs];
+        if (masked) {
+          const int jmax = a.causal ? ip - jt - 4 * hf : INT_MAX;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!((w >> acc_row(e)) & 1) || acc_row(e) > jmax) s[qs][e] = 0.f;
+        }
+        if (a.dtab_part) {
+          if (left || right) {
+            float t4 = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) t4 += s[qs][e];
+            far_l += left ? t4 : 0.f;
+            far_r += left ? 0.f : t4;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) __hip_atomic_fetch_add(my_diag + at0 + acc_row(e), s[qs][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          }
+        }
+        df[qs][0] = rel_operand<T>(s[qs], 0);
+        df[qs][1] = rel_operand<T>(s[qs], 1);
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+          const s16x8 kf = rel_tr_frag(K + (dt >> 1) * 8192, il, t * 4096 + st * 2048, dt & 1);
+#pragma unroll
+          for (int qs = 0; qs < NQ; ++qs) dq[qs][dt] = rel_mfma<T>(kf, df[qs][st], dq[qs][dt]);
+        }
+    }
+  }
+#pragma unroll
+  for (int qs = 0; qs < NQ; ++qs) {
+    const int i = i_wave + 32 * qs + r;
+    if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, dq[qs], a.scale, hf);
+  }
+  if (!a.dtab_part) return;
+  // ---- this workgroup's sums by bucket: the far sums join their wave's vectors at its ends, the eight vectors are added in order, and
+  // a thread per (bucket, slice) collects its distances
+  far_l = wave_sum(far_l);
+  far_r = wave_sum(far_r);
+  __syncthreads();
+  if (lane == 0) {
+    diag[2 * wave * nbias] += far_l;
+    diag[2 * wave * nbias + 2 * (a.far + EXT)] += far_r;
+  }
+  __syncthreads();
+  const int n = 2 * (a.far + EXT) + 1;
+  int* which = reinterpret_cast<int*>(bias);
+  for (int x = tid; x < n; x += 256) {
+    float t = 0.f;
+#pragma unroll
+    for (int v = 0; v < 8; ++v) t += diag[v * nbias + x];
+    diag[x] = t;
+    which[x] = rel_bucket(a, min(max(x - a.far - EXT, -a.far), a.far));
+  }
+  __syncthreads();
+  const int slices = 256 / a.buckets;
+  const int bucket = tid % a.buckets, sl = tid / a.buckets;
+  float t = 0.f;
+  if (sl < slices)
+    for (int x = sl; x < n; x += slices) t += which[x] == bucket ? diag[x] : 0.f;
+  float* red = diag + nbias;
+  __syncthreads();
+  red[tid] = t;
+  __syncthreads();
+  if (tid < a.buckets) {
+    t = 0.f;
+    for (int s = 0; s < slices; ++s) t += red[s * a.buckets + tid];
+    a.dtab_part[(int64_t)item * a.buckets + tid] = t;
+  }
+}
+
+// dtable[c][h] = sum over samples and query blocks of the partials, in order.  One workgroup per head.
+template <typename W>
+__global__ __launch_bounds__(256) void rel_dtable_kernel(const float* part, W* dtable, int B, int H, int nqb, int buckets) {
+  __shared__ float red[256];
+  const int h = blockIdx.x, slices = 256 / buckets, c = threadIdx.x % buckets, sl = threadIdx.x / buckets;
+  float t = 0.f;
+  if (sl < slices)
+    for (int x = sl; x < B * nqb; x += slices) {
+      const int b = x / nqb, qb = x - b * nqb;
+      t += part[(((int64_t)b * H + h) * nqb + qb) * buckets + c];
+    }
+  red[threadIdx.x] = t;
+  __syncthreads();
+  if (threadIdx.x < buckets) {
+    t = 0.f;
+    for (int s = 0; s < slices; ++s) t += red[s * buckets + threadIdx.x];
+    dtable[(int64_t)threadIdx.x * H + h] = from_f32<W>(t);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dK, dV
+// The key on the lane: a wave keeps K and V of its 32 keys as operands, walks the query tiles of all heads of the group, and sums dK^T
+// and dV^T of the group in its accumulators.
+template <typename T, int D>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dkv_kernel(const RelArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int CB = D / 64, STAGE = 2 * CB * 8192 + 512, KB = 128, EXT = 96;
+  float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, hf = lane >> 5;
+  const int nkb = (a.Lk + KB - 1) / KB, item = rel_item(blockIdx.x, gridDim.x);
+  const int bk = item / nkb, kb = item - bk * nkb, b = bk / a.Hk, hk = bk - b * a.Hk;
+  const int off = rel_offset(a, b), klen = rel_key_len(a, b);
+  const int j_wg = kb * KB, j_wave = j_wg + 32 * wave, j = j_wave + r;
+  const bool kept = j < klen && rel_mask_at(a, b, j);
+  f32x16 dk[D / 32], dv[D / 32];
+  s16x8 kf[D / 16], vf[D / 16];
+  {
+    const int jc = min(j, a.Lk - 1);
+    const T* kp = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh + jc * a.k_sl + 8 * hf;
+    const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh + jc * a.v_sl + 8 * hf;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      kf[kk] = *reinterpret_cast<const s16x8*>(kp + 16 * kk);
+      vf[kk] = *reinterpret_cast<const s16x8*>(vp + 16 * kk);
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = rel_zero();
+  }
+  const bool wave_keeps = __any(kept);
+  const bool wg_keeps = __syncthreads_or(kept);
+  // query tiles: causal rows end before i + off = j
+  const int nqt = (a.Lq + 63) / 64;
+  const int first = a.causal ? max(0, j_wg - off) / 64 : 0;
+  const int per = max(nqt - first, 0), total = wg_keeps ? per * a.G : 0;
+  const ImgLane il = img_lane(lane);
+  const int64_t g_sl = (int64_t)a.H * D;
+  const RelLoader<T, CB, 4> ld(a.q_sl, g_sl, wave, lane);
+  const uint32_t lds0 = lds_addr_of(smem);
+  float rowv = 0.f;   // lanes of waves 0, 1: lse, delta of the next tile's rows
+  auto issue = [&](int x) {
+    const int h = hk * a.G + x / per, i0 = 64 * (first + x % per);
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh;
+    const T* gp = reinterpret_cast<const T*>(a.dout) + ((int64_t)b * a.Lq * a.H + h) * D;
+    ld.issue(qp, gp, a.q_sl, g_sl, i0, a.Lq, lds0 + (x & 1) * STAGE, wave, lane);
+    if (wave < 2) {
+      const int i = i0 + lane;
+      const float* src = wave ? a.delta : a.lse;
+      const float past = wave ? 0.f : INFINITY;   // rows past the end: P = 0
+      rowv = i < a.Lq ? src[((int64_t)b * a.H + h) * a.Lq + i] : past;
+    }
+  };
+  int head = -1;
+  if (total > 0) issue(0);
+  for (int x = 0; x < total; ++x) {
+    const int hg = x / per, i0 = 64 * (first + x % per);
+    char* Q = smem + (x & 1) * STAGE;
+    char* Gr = Q + CB * 8192;
+    float* rows = reinterpret_cast<float*>(Q + 2 * CB * 8192);   // [lse 64][delta 64]
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    if (wave < 2) rows[64 * wave + lane] = rowv;
+    if (hg != head) {   // (nobody reads the old bias any more once all are past this barrier)
+      __syncthreads();
+      rel_bias_fill<T>(a, bias, EXT, hk * a.G + hg, tid, 256);
+      head = hg;
+    }
+    __syncthreads();
+    if (x + 1 < total) issue(x + 1);
+    if (!wave_keeps || (a.causal && i0 + 63 + off < j_wave)) continue;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int it = i0 + 32 * t;
+      if (it >= a.Lq || (a.causal && it + 31 + off < j_wave)) continue;
+      f32x16 s = rel_zero(), dp = rel_zero();
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        s = rel_mfma<T>(rel_row_frag(Q + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]), kf[kk], s);
+        dp = rel_mfma<T>(rel_row_frag(Gr + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]), vf[kk], dp);
+      }
+      const int rel_hi = j_wave + 31 - (it + off), rel_lo = j_wave - (it + 31 + off);
+      const bool left = rel_hi <= -a.far, right = rel_lo >= a.far;
+      const float* lr = rows + 32 * t + 4 * hf;
+      const float* bp = bias + (a.far + EXT + j - (it + off) - 4 * hf);   // minus the row (only used where the tile is near)
+      const float c = bias[left ? 0 : 2 * (a.far + EXT)];
+      const int imin = a.causal ? j - off - it - 4 * hf : INT_MIN;
+      f32x16 p;
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 ls = *reinterpret_cast<const float4*>(lr + 8 * q4);
+        const float4 de = *reinterpret_cast<const float4*>(lr + 64 + 8 * q4);
+        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv4[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = 4 * q4 + e;
+          const float bias2 = left || right ? c : bp[-(8 * q4 + e)];
+          const float pv = att_exp2(fmaf(s[k], a.sl2, bias2) - lv[e]);
+          const bool ok = kept && 8 * q4 + e >= imin;
+          p[k] = ok ? pv : 0.f;
+          s[k] = ok ? pv * (dp[k] - dv4[e]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const s16x8 pf = rel_operand<T>(p, st), df = rel_operand<T>(s, st);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+          dv[dt] = rel_mfma<T>(rel_tr_frag(Gr + (dt >> 1) * 8192, il, t * 4096 + st * 2048, dt & 1), pf, dv[dt]);
+          dk[dt] = rel_mfma<T>(rel_tr_frag(Q + (dt >> 1) * 8192, il, t * 4096 + st * 2048, dt & 1), df, dk[dt]);
+        }
+      }
+    }
+  }
+  if (j < a.Lk) {
+    const int64_t at = (((int64_t)b * a.Lk + j) * a.Hk + hk) * D;
+    if (!kept) {   // (a NaN in a row's gradient meets P = 0 here)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = rel_zero();
+    }
+    rel_store_row<T, D>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, hf);
+    rel_store_row<T, D>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, hf);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+// Queries per wave, 32 NQ.
+static int rel_nq(const mmk_rel_attn* p) { return p->D == 64 ? 2 : 1; }
+static int rel_dq_blocks(const mmk_rel_attn* p) { return (p->Lq + 128 * rel_nq(p) - 1) / (128 * rel_nq(p)); }
+
+constexpr int REL_LDS = 160 * 1024;
+static int64_t rel_split_lds(const mmk_rel_attn* p) {   // four waves' double-buffered tiles and the bias vector of every head of the group
+  return std::max(8 * 2 * (p->D / 64) * 4096 + (int64_t)(p->H / p->Hk) * (2 * (p->max_distance + 1) + 1) * 4, (int64_t)1024 + 4 * 32 * (p->D + 4) * 4);
+}
+// The few-rows kernel takes over where one block of 32 rows holds all queries of a group.
+static bool rel_few_rows(const mmk_rel_attn* p) { return (int64_t)(p->H / p->Hk) * p->Lq <= 32 && rel_split_lds(p) <= REL_LDS; }
+// splits of the keys: about two workgroups per CU, at least two tiles of 32 keys per wave
+static int rel_splits(const mmk_rel_attn* p) {
+  const int64_t groups = (int64_t)p->B * p->Hk;
+  const int64_t want = (512 + groups - 1) / groups, most = std::max<int64_t>(1, ((int64_t)p->Lk + 255) / 256);
+  return (int)std::min<int64_t>(std::min(want, most), 64);
+}
+static int rel_check(const mmk_rel_attn* p) {
+  MMK_REQUIRE(p != nullptr, "no geometry");
+  MMK_REQUIRE(p->dtype == MMK_BF16 || p->dtype == MMK_F16, "operands are bf16 or f16");
+  MMK_REQUIRE(p->table_dtype == MMK_F32 || p->table_dtype == p->dtype, "the table is f32 or of the operands' type");
+  MMK_REQUIRE(p->D == 64 || p->D == 128, "head dim must be 64 or 128");
+  MMK_REQUIRE(p->B >= 0 && p->H >= 1 && p->Hk >= 1 && p->H % p->Hk == 0 && p->Lq >= 0 && p->Lk >= 0, "bad sizes");
+  MMK_REQUIRE(p->Lq <= (1 << 28) && p->Lk <= (1 << 28), "sequence too long");
+  MMK_REQUIRE((int64_t)p->B * p->H * (((int64_t)std::max(p->Lq, p->Lk) + 127) / 128) < (1 << 30), "too many workgroups");
+  MMK_REQUIRE(p->buckets >= 1 && p->buckets <= REL_MAX_BUCKETS && p->n_borders >= 0 && p->n_borders <= REL_MAX_BORDERS, "too many buckets");
+  MMK_REQUIRE(p->near_buckets >= 1 && p->max_distance >= 1 && p->max_distance <= REL_MAX_FAR, "max_distance must be 1 .. 512");
+  MMK_REQUIRE((p->bidirectional ? 2 : 1) * (p->near_buckets + p->n_borders + 1) == p->buckets, "near and logarithmic buckets do not add up");
+  for (int i = 0; i < 3; ++i) {
+    MMK_REQUIRE(p->q_strides[i] % 8 == 0 && p->k_strides[i] % 8 == 0 && p->v_strides[i] % 8 == 0, "strides must be multiples of 8 elements");
+    MMK_REQUIRE(p->q_strides[i] >= 0 && p->k_strides[i] >= 0 && p->v_strides[i] >= 0, "negative strides");
+  }
+  // a tile's 64 rows are addressed by 32-bit byte offsets
+  MMK_REQUIRE(p->q_strides[2] <= (1 << 23) && p->k_strides[2] <= (1 << 23) && p->v_strides[2] <= (1 << 23), "row stride too large");
+  MMK_REQUIRE(p->mask_kind >= MMK_REL_MASK_NONE && p->mask_kind <= MMK_REL_MASK_64 && (p->mask_kind == 0) == (p->mask == nullptr), "bad mask");
+  for (const void* x : {p->q, p->k, p->v}) MMK_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "operands must be 16-byte aligned");
+  return 0;
+}
+
+static RelArgs rel_args(const mmk_rel_attn* p) {
+  RelArgs a = {};
+  a.q = p->q;
+  a.k = p->k;
+  a.v = p->v;
+  a.q_sb = p->q_strides[0];
+  a.q_sh = p->q_strides[1];
+  a.q_sl = p->q_strides[2];
+  a.k_sb = p->k_strides[0];
+  a.k_sh = p->k_strides[1];
+  a.k_sl = p->k_strides[2];
+  a.v_sb = p->v_strides[0];
+  a.v_sh = p->v_strides[1];
+  a.v_sl = p->v_strides[2];
+  a.B = p->B;
+  a.H = p->H;
+  a.Hk = p->Hk;
+  a.G = p->H / p->Hk;
+  a.Lq = p->Lq;
+  a.Lk = p->Lk;
+  a.scale = p->scale;
+  a.sl2 = p->scale * REL_LOG2E;
+  a.table = p->table;
+  a.table_f32 = p->table_dtype == MMK_F32;
+  a.buckets = p->buckets;
+  a.side = p->bidirectional ? p->buckets / 2 : p->buckets;
+  a.near = p->near_buckets;
+  a.far = p->max_distance;
+  a.bidir = p->bidirectional != 0;
+  a.n_borders = p->n_borders;
+  a.causal = p->causal != 0;
+  a.off = p->q_offset;
+  a.off_ptr = p->q_offsets;
+  a.mask = p->mask;
+  a.mask_sb = p->mask_stride;
+  a.mask_kind = p->mask_kind;
+  for (int i = 0; i < p->n_borders; ++i) a.borders[i] = p->borders[i];
+  return a;
+}
+
+// lds_most: the largest dynamic LDS any call of this kernel asks for (the opt-in is made once, at its first launch)
+template <typename K>
+static int rel_launch(K kern, int id, int64_t grid, int lds, int lds_most, const RelArgs& a, hipStream_t st) {
+  KernelSetup ks;
+  if (int rc = kernel_setup(reinterpret_cast<const void*>(kern), 256, lds_most, &ks)) return rc;
+  ProfEvents pe(id);
+  hipExtLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, st, pe.start, pe.stop, 0, a);
+  MMK_LAUNCH_CHECK();
+  return 0;
+}
+
+// bytes of a vector over the distances -far - ext .. far + ext
+static constexpr int rel_vec_bytes(int far, int ext) { return ((2 * (far + ext) + 1 + 3) & ~3) * 4; }
+
+template <typename T, int D>
+static int rel_forward(const mmk_rel_attn* p, RelArgs& a, hipStream_t st) {
+  if (rel_few_rows(p)) {
+    a.splits = rel_splits(p);
+    a.row_blocks = 1;
+    if (int rc = rel_launch(rel_split_kernel<T, D>, MMK_K_REL_ATTN_FWD, (int64_t)a.B * a.Hk * a.splits, (int)rel_split_lds(p), REL_LDS, a, st))
+      return rc;
+    if (a.splits == 1) return 0;
+    const int64_t n = (int64_t)a.B * a.H * a.Lq * (D / 4);
+    return rel_launch(rel_join_kernel<T, D>, MMK_K_REL_ATTN_FWD, (n + 255) / 256, 0, 0, a, st);
+  }
+  constexpr int NQ = D == 64 ? 2 : 1, EXT = 64 + 32 * NQ, TILES = 2 * 2 * (D / 64) * 8192;
+  const int64_t grid = (int64_t)a.B * a.H * ((a.Lq + 128 * NQ - 1) / (128 * NQ));
+  return rel_launch(rel_fwd_kernel<T, D, NQ>, MMK_K_REL_ATTN_FWD, grid, TILES + rel_vec_bytes(a.far, EXT), TILES + rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
+}
+
+template <typename T, int D>
+static int rel_backward(const mmk_rel_attn* p, RelArgs& a, void* dtable, hipStream_t st) {
+  constexpr int NQ = D == 64 ? 2 : 1, EXT = 32 + 32 * NQ, TILES = 2 * 2 * (D / 64) * 8192;
+  const int nqb = rel_dq_blocks(p);
+  if (a.Lq > 0) {
+    const int lds = TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 9 : 1);
+    if (int rc = rel_launch(rel_dq_kernel<T, D, NQ>, MMK_K_REL_ATTN_BWD, (int64_t)a.B * a.H * nqb, lds, TILES + 9 * rel_vec_bytes(REL_MAX_FAR, EXT), a, st))
+      return rc;
+  }
+  if (a.Lk > 0) {
+    const int64_t grid = (int64_t)a.B * a.Hk * ((a.Lk + 127) / 128);
+    if (int rc = rel_launch(rel_dkv_kernel<T, D>, MMK_K_REL_ATTN_BWD, grid, TILES + 1024 + rel_vec_bytes(a.far, 96),
+                            TILES + 1024 + rel_vec_bytes(REL_MAX_FAR, 96), a, st))
+      return rc;
+  }
+  if (a.dtab_part) {
+    const int n = a.Lq > 0 ? nqb : 0;
+    if (p->table_dtype == MMK_F32)
+      hipLaunchKernelGGL(rel_dtable_kernel<float>, dim3(a.H), dim3(256), 0, st, a.dtab_part, (float*)dtable, a.B, a.H, n, a.buckets);
+    else
+      hipLaunchKernelGGL(rel_dtable_kernel<T>, dim3(a.H), dim3(256), 0, st, a.dtab_part, (T*)dtable, a.B, a.H, n, a.buckets);
+    MMK_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+template <typename F>
+static int rel_dispatch(const mmk_rel_attn* p, F f) {
+  if (p->dtype == MMK_BF16) return p->D == 64 ? f(bf16_t(), std::integral_constant<int, 64>()) : f(bf16_t(), std::integral_constant<int, 128>());
+  return p->D == 64 ? f(f16_t(), std::integral_constant<int, 64>()) : f(f16_t(), std::integral_constant<int, 128>());
+}
+
+}  // namespace mmk
+
+using namespace mmk;
+
+extern "C" {
+
+int64_t mmk_rel_attn_fwd_ws_floats(const mmk_rel_attn* p) {
+  if (rel_check(p)) return -1;
+  if (!rel_few_rows(p) || (int64_t)p->B * p->Lq == 0) return 0;
+  const int s = rel_splits(p);
+  return s == 1 ? 0 : (int64_t)p->B * p->Hk * 32 * s * (p->D + 4);
+}
+
+int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, float* lse, float* ws, void* stream) {
+  if (int rc = rel_check(p)) return rc;
+  if ((int64_t)p->B * p->Lq == 0) return 0;
+  MMK_REQUIRE(p->q && out && (p->Lk == 0 || (p->k && p->v)) && p->table, "missing operand");
+  MMK_REQUIRE(mmk_rel_attn_fwd_ws_floats(p) == 0 || ws, "missing workspace");
+  RelArgs a = rel_args(p);
+  a.out = out;
+  a.lse = lse;
+  a.part = ws;
+  return rel_dispatch(p, [&](auto t, auto d) { return rel_forward<decltype(t), decltype(d)::value>(p, a, (hipStream_t)stream); });
+}
+
+int64_t mmk_rel_attn_bwd_ws_floats(const mmk_rel_attn* p, int want_dtable) {
+  if (rel_check(p)) return -1;
+  return (int64_t)p->B * p->H * p->Lq + (want_dtable ? (int64_t)p->B * p->H * rel_dq_blocks(p) * p->buckets : 0);
+}
+
+int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dtable,
+                     float* ws, void* stream) {
+  if (int rc = rel_check(p)) return rc;
+  MMK_REQUIRE(p->Lk == 0 || (dk && dv), "missing operand");
+  MMK_REQUIRE(p->Lq == 0 || (p->q && out && lse && dout && dq && ws && p->table), "missing operand");
+  if (p->B == 0) {
+    if (!dtable) return 0;
+    MMK_REQUIRE(false, "the table's gradient of no samples is the caller's zero");
+  }
+  RelArgs a = rel_args(p);
+  a.o = out;
+  a.lse = const_cast<float*>(lse);
+  a.dout = dout;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.delta = ws;
+  a.dtab_part = dtable ? ws + (int64_t)p->B * p->H * p->Lq : nullptr;
+  return rel_dispatch(p, [&](auto t, auto d) { return rel_backward<decltype(t), decltype(d)::value>(p, a, dtable, (hipStream_t)stream); });
+}
+
+}  // extern "C"

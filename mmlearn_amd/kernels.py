@@ -1357,3 +1357,81 @@ def qk_norm_rotary_bwd(q: torch.Tensor, k: torch.Tensor, qw: Optional[torch.Tens
                                                 int(interleaved), _strides_blh(q), _strides_blh(k), _strides_blh(dqo), _strides_blh(dko),
                                                 float(eps), dtype_tag(q.dtype), wdt, stream()))
     return dq, dk, dw[0], dw[1]
+
+
+# ------------------------------------------------------------------ attention with a learned relative position bias by buckets
+@functools.lru_cache(maxsize=64)
+def relative_buckets(buckets: int, max_distance: int, bidirectional: bool):
+    """(near, borders) of one side of the bucket scheme of ``mmk_rel_attn``: half of a side's buckets hold one distance each; step t of the
+    others begins at the smallest distance d with ``(d / near) ** (side - near) >= (max_distance / near) ** t``, decided in integers (a
+    logarithm in float32 can miss a border that a distance stands on exactly)."""
+    side = buckets // 2 if bidirectional else buckets
+    near = side // 2
+    n = side - near
+    borders = [next(d for d in range(near, max_distance + 1) if d ** n * near ** t >= max_distance ** t * near ** n) for t in range(1, n)]
+    return near, (C.c_int32 * max(len(borders), 1))(*borders), len(borders)
+
+
+_REL_MASKS = {(1, torch.int32): 1, (1, torch.int64): 2, (2, torch.bool): 3, (2, torch.uint8): 3, (2, torch.int32): 4, (2, torch.int64): 5}
+
+
+def _strides_bhl(t: torch.Tensor):
+    """Element strides {batch, head, row}; a dim of one entry is never stepped over."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+
+
+def _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset) -> _lib.RelAttn:
+    p = _lib.RelAttn()
+    B, H, Lq, D = q.shape
+    p.q, p.k, p.v, p.table, p.mask = ptr(q), ptr(k), ptr(v), ptr(table), ptr(key_mask)
+    for n, t in (("q_strides", q), ("k_strides", k), ("v_strides", v)):
+        getattr(p, n)[:] = _strides_bhl(t)
+    p.B, p.H, p.Hk, p.Lq, p.Lk, p.D = B, H, k.shape[1], Lq, k.shape[2], D
+    p.dtype, p.table_dtype = dtype_tag(q.dtype), dtype_tag(table.dtype)
+    if key_mask is not None:
+        p.mask_kind = _REL_MASKS[key_mask.dim(), key_mask.dtype]
+        p.mask_stride = key_mask.stride(0) if key_mask.dim() == 2 else 0
+    near, borders, n_borders = relative_buckets(table.shape[0], max_distance, bidirectional)
+    p.buckets, p.near_buckets, p.n_borders, p.max_distance, p.bidirectional = table.shape[0], near, n_borders, max_distance, int(bidirectional)
+    p.borders = C.cast(borders, C.c_void_p)
+    p.keep = borders   # the cache above may drop it meanwhile
+    p.causal, p.scale = int(causal), scale
+    if isinstance(q_offset, torch.Tensor):
+        p.q_offsets = ptr(q_offset)
+    else:
+        p.q_offset = q_offset
+    return p
+
+
+def rel_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int, bidirectional: bool, scale: float,
+                 causal: bool, key_mask: Optional[torch.Tensor], q_offset, want_lse: bool):
+    """q [B, H, Lq, D], k / v [B, Hk, Lk, D] views -> (out [B, Lq, H, D] contiguous, lse f32 [B, H, Lq] or None).  csrc/rel_attention.hip."""
+    require_gpu(q)
+    B, H, Lq, D = q.shape
+    p = _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset)
+    with on_device_of(q):
+        out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+        lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if want_lse else None
+        n = _lib.lib().mmk_rel_attn_fwd_ws_floats(C.byref(p))
+        ws = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
+        check(_lib.lib().mmk_rel_attn_fwd(C.byref(p), ptr(out), ptr(lse), ptr(ws), stream()))
+    return out, lse
+
+
+def rel_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int, bidirectional: bool, scale: float,
+                 causal: bool, key_mask: Optional[torch.Tensor], q_offset, out: torch.Tensor, lse: torch.Tensor, dout: torch.Tensor,
+                 want_dtable: bool = True):
+    """-> (dq, dk, dv as [B, heads, L, D] views of contiguous [B, L, heads, D] buffers, dtable or None)."""
+    require_gpu(q)
+    B, H, Lq, D = q.shape
+    Hk, Lk = k.shape[1], k.shape[2]
+    assert out.is_contiguous() and dout.is_contiguous() and out.shape == (B, Lq, H, D) == dout.shape
+    p = _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset)
+    with on_device_of(q):
+        dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+        dk, dv = (torch.empty((B, Lk, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+        dtable = None if not want_dtable else torch.empty_like(table) if B else torch.zeros_like(table)
+        if B:
+            ws = torch.empty(max(1, _lib.lib().mmk_rel_attn_bwd_ws_floats(C.byref(p), int(want_dtable))), dtype=torch.float32, device=q.device)
+            check(_lib.lib().mmk_rel_attn_bwd(C.byref(p), ptr(out), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws), stream()))
+    return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dtable

@@ -1,0 +1,365 @@
+"""Attention with a learned relative position bias against its float64 definition: lengths, head layouts, types, bucket schemes, masks with
+anything behind them, offsets, strides; gradients (table included) against the definition's and against differences; refusals."""
+
+import ctypes
+import os
+import subprocess
+
+import pytest
+import torch
+
+from mmlearn_amd import kernels as K
+from mmlearn_amd.attention import relative_attention
+from oracle import tower_oracle as oracle
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _case(B, H, Hk, Lq, Lk, D, dtype="bfloat16", table="same", buckets=32, far=128, bidir=True, causal=False, mask=None, offset=0, strides="rows"):
+    return dict(B=B, H=H, Hk=Hk, Lq=Lq, Lk=Lk, D=D, dtype=dtype, table=table, buckets=buckets, far=far, bidir=bidir, causal=causal, mask=mask,
+                offset=offset, strides=strides)
+
+
+CASES = [
+    # one token
+    _case(1, 1, 1, 1, 1, 64),
+    _case(2, 4, 4, 1, 333, 64, causal=True, bidir=False, offset=332),
+    _case(3, 8, 2, 1, 700, 128, mask="lengths", causal=True, bidir=False, offset="tensor"),
+    _case(2, 6, 1, 5, 129, 128, "float16", mask="bool", offset=40),
+    _case(2, 32, 1, 1, 65, 64, mask="int64"),
+    _case(1, 2, 2, 3, 3000, 64, "float16", far=40, buckets=16, offset=2997),
+    _case(2, 3, 3, 4, 31, 128, mask="len64", offset=-7, causal=True),
+    _case(1, 40, 1, 1, 100, 64),                     # 40 query heads on one key head: more rows than the few-rows kernel holds
+    _case(1, 32, 1, 1, 90, 128, far=512, buckets=64),   # bias vectors of 32 heads that its LDS cannot hold
+    # whole sequences
+    _case(2, 3, 3, 33, 33, 64),
+    _case(2, 4, 2, 64, 64, 64, causal=True),
+    _case(1, 2, 1, 65, 63, 128, "float16", "f32", bidir=False),
+    _case(2, 3, 1, 77, 77, 64, "float16", "f32", mask="lengths", strides="heads"),
+    _case(2, 2, 2, 129, 200, 128, mask="bool", strides="packed"),
+    _case(2, 4, 1, 300, 300, 64, "bfloat16", "f32", buckets=16, far=20, causal=True, bidir=False),
+    _case(1, 2, 2, 257, 513, 64, buckets=8, far=9, mask="uint8", offset=200),
+    _case(1, 2, 1, 150, 513, 128, buckets=8, far=17, causal=True, offset=363, mask="int32"),
+    _case(1, 2, 2, 513, 100, 128, "float16", buckets=4, far=2, offset=-300),
+    _case(2, 2, 1, 200, 140, 64, causal=True, offset=-60, mask="lengths", bidir=False),   # early rows see no key
+    _case(1, 1, 1, 130, 700, 64, buckets=256, far=512, offset=300),
+    _case(1, 2, 2, 70, 70, 64, buckets=2, far=1, bidir=False),
+    _case(1, 2, 2, 40, 40, 64, offset=1 << 28),
+    _case(5, 2, 2, 48, 48, 64, mask="tensor of none"),
+]
+
+
+def _layout(x, kind):
+    if kind == "rows":      # [B, L, H, D] behind [B, H, L, D]
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+    if kind == "packed":    # rows of a wider projection
+        B, H, L, D = x.shape
+        wide = torch.full((B, L, H + 2, D), float("nan"), dtype=x.dtype, device=x.device)
+        wide[:, :, 1:1 + H] = x.transpose(1, 2)
+        return wide[:, :, 1:1 + H].transpose(1, 2)
+    return x.contiguous()
+
+
+def _inputs(c, seed=0, spoil=True):
+    g = torch.Generator().manual_seed(seed)
+    dt = getattr(torch, c["dtype"])
+    B, H, Hk, Lq, Lk, D = (c[n] for n in ("B", "H", "Hk", "Lq", "Lk", "D"))
+    q = torch.randn(B, H, Lq, D, generator=g).to(dt)
+    k, v = (torch.randn(B, Hk, Lk, D, generator=g).to(dt) for _ in range(2))
+    table = torch.randn(c["buckets"], H, generator=g).to(torch.float32 if c["table"] == "f32" else dt)
+    dout = torch.randn(B, Lq, H, D, generator=g).to(dt)
+    keep, mask = None, None
+    if c["mask"] in ("lengths", "len64"):
+        n = torch.randint(0, Lk + 1, (B,), generator=g)
+        n[0], n[-1] = Lk, 0
+        keep = torch.arange(Lk)[None] < n[:, None]
+        mask = n.to(torch.int32 if c["mask"] == "lengths" else torch.int64)
+        mask = mask if c["mask"] == "lengths" else mask * 3 - 2 * n   # (the same numbers)
+    elif c["mask"] == "tensor of none":
+        keep = torch.ones(B, Lk, dtype=torch.bool)
+        keep[1] = False
+        keep[2, 1:] = False
+        keep[3, :-1] = False
+        mask = keep
+    elif c["mask"]:
+        keep = torch.rand(B, Lk, generator=g) < 0.6
+        keep[0, 64:128] = False    # a tile that holds nothing
+        if B > 1:
+            keep[-1] = False       # a sample that holds nothing
+        mask = {"bool": keep, "uint8": keep.to(torch.uint8) * 3, "int32": keep.int() * -5, "int64": keep.long() << 40}[c["mask"]]
+        wide = torch.ones(B, Lk + 7, dtype=mask.dtype)
+        wide[:, :Lk] = mask
+        mask = wide[:, :Lk]
+    if keep is not None and spoil:   # what masked keys hold does not matter
+        bad = (~keep)[:, None, :, None]
+        k = torch.where(bad, torch.tensor(float("nan")), k.float()).to(dt)
+        v = torch.where(bad, torch.tensor(float("inf")), v.float()).to(dt)
+    offset = c["offset"]
+    if offset == "tensor":
+        offset = (keep.sum(1) - 1 if keep is not None else torch.arange(B)).int()
+    dev = [_layout(t.cuda(), c["strides"]) for t in (q, k, v)] + [table.cuda(), dout.cuda()]
+    if isinstance(mask, torch.Tensor):
+        cuda_mask = mask.cuda()
+        if mask.dim() == 2:
+            full = torch.ones(B, Lk + 7, dtype=mask.dtype, device="cuda")
+            full[:, :Lk] = cuda_mask
+            cuda_mask = full[:, :Lk]
+        mask = cuda_mask
+    return dev, mask, keep, offset
+
+
+def _bounds(c, q, k, v, table, dout, keep, offset):
+    """Float64 results and, beside each, how far the kernels' roundings may carry them: half a step of the operands' type for P, for dS, for the
+    stored o that delta comes from, and for every output; f32 for the rest."""
+    dt = getattr(torch, c["dtype"])
+    u = torch.finfo(dt).eps / 2
+    tiny = 2.0 ** -25 if dt == torch.float16 else 0.0      # half a step of f16's smallest values
+    B, H, Hk, Lq, Lk, D = (c[n] for n in ("B", "H", "Hk", "Lq", "Lk", "D"))
+    G, scale = H // Hk, D ** -0.5
+    out = {n: [] for n in ("out", "dq")}
+    res = {n: torch.zeros(s, dtype=torch.float64) for n, s in (("out", (B, Lq, H, D)), ("dq", (B, H, Lq, D)), ("dk", (B, Hk, Lk, D)),
+                                                                ("dv", (B, Hk, Lk, D)), ("dtable", (c["buckets"], H)))}
+    err = {n: torch.zeros_like(t) for n, t in res.items()}
+    keep = torch.ones(B, Lk, dtype=torch.bool) if keep is None else keep
+    for b in range(B):
+        off = offset if isinstance(offset, int) else int(offset[b])
+        bm = oracle.bucket_map(Lq, Lk, off, c["buckets"], c["far"], c["bidir"])
+        seen = keep[b][None].expand(Lq, Lk)
+        if c["causal"]:
+            seen = seen & (torch.arange(Lk)[None] <= torch.arange(Lq)[:, None] + off)
+        for h in range(H):
+            Q, Kb, Vb, dO = q[b, h], k[b, h // G] * keep[b][:, None], v[b, h // G] * keep[b][:, None], dout[b, :, h]
+            Kb, Vb = (torch.where(keep[b][:, None], t[b, h // G], torch.zeros(())) for t in (k, v))
+            bias = table[:, h][bm]
+            z = (Q @ Kb.T) * scale + bias
+            p = torch.where(seen, torch.exp(z - torch.where(seen, z, torch.full_like(z, -1e30)).amax(1, keepdim=True)), torch.zeros_like(z)) if Lk else z
+            p = p / p.sum(1, keepdim=True).clamp(min=1e-300)
+            # a score: sums of D products, the scale, the bias, the maximum and the exponential, in f32; then the softmax's sum
+            es = 2.0 ** -24 * ((D + 8) * ((Q.abs() @ Kb.abs().T) * scale).amax(1, keepdim=True) + 16 * bias.abs().max() + Lk / 16 + 32) if Lk else z
+            A = p @ Vb.abs()
+            eo = (u + es) * A + tiny * Vb.abs().sum(0) if Lk else torch.zeros(Lq, D, dtype=torch.float64)
+            o = p @ Vb
+            res["out"][b, :, h] = o
+            err["out"][b, :, h] = u * o.abs() + eo + tiny
+            if not Lk:
+                continue
+            dp = dO @ Vb.T
+            delta = (dO * o).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            edelta = (dO.abs() * (u * o.abs() + eo + tiny)).sum(1, keepdim=True)
+            f32 = p * 2.0 ** -24 * (D + 8) * (dO.abs() @ Vb.abs().T + (dO.abs() * o.abs()).sum(1, keepdim=True))
+            e32 = 2 * es * ds.abs() + p * edelta + f32           # dS before its rounding
+            e16 = e32 + u * ds.abs() + tiny
+            res["dq"][b, h] = ds @ Kb * scale
+            err["dq"][b, h] = e16 @ Kb.abs() * scale
+            res["dk"][b, h // G] += ds.T @ Q * scale
+            err["dk"][b, h // G] += e16.T @ Q.abs() * scale
+            res["dv"][b, h // G] += p.T @ dO
+            err["dv"][b, h // G] += ((u + 2 * es) * p + tiny).T @ dO.abs()
+            res["dtable"][:, h].index_add_(0, bm.reshape(-1), ds.reshape(-1))
+            err["dtable"][:, h].index_add_(0, bm.reshape(-1), (e32 + 2.0 ** -24 * 64 * ds.abs()).reshape(-1))
+    ut = torch.finfo(torch.float32 if c["table"] == "f32" else dt).eps / 2
+    for n in ("dq", "dk", "dv", "dtable"):
+        w = ut if n == "dtable" else u
+        err[n] = err[n] * 1.01 + w * res[n].abs() + (tiny if w == u else 0.0) + 2.0 ** -24 * 32 * res[n].abs().max() if res[n].numel() else err[n]
+    return res, err
+
+
+def _run(c, dev, mask, offset):
+    leaves = [t.detach().requires_grad_(True) for t in dev[:4]]
+    off = offset.cuda() if isinstance(offset, torch.Tensor) else offset
+    out = relative_attention(*leaves, max_distance=c["far"], bidirectional=c["bidir"], causal=c["causal"], key_mask=mask, q_offset=off)
+    grads = torch.autograd.grad(out, leaves, dev[4])
+    return dict(zip(("out", "dq", "dk", "dv", "dtable"), [t.detach() for t in (out, *grads)]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", CASES, ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_against_float64(c):
+    dev, mask, keep, offset = _inputs(c)
+    got = _run(c, dev, mask, offset)
+    res, err = _bounds(c, *(t.double().cpu() for t in dev), keep, offset)
+    assert got["out"].is_contiguous()
+    for n in res:
+        x = got[n].double().cpu()
+        assert x.shape == res[n].shape and torch.isfinite(x).all(), n
+        over = ((x - res[n]).abs() - err[n] * 1.01).max().item() if x.numel() else 0.0
+        assert over <= 0, (n, over, (x - res[n]).norm().item() / max(res[n].norm().item(), 1e-300))
+        # the bounds are sums of absolute values: also hold the whole to what independent roundings leave of them
+        if res[n].norm() > 0 and n != "dtable":
+            assert (x - res[n]).norm() <= 6 * torch.finfo(dev[0].dtype).eps * res[n].norm(), n
+    with torch.no_grad():
+        off = offset.cuda() if isinstance(offset, torch.Tensor) else offset
+        again = relative_attention(*dev[:4], max_distance=c["far"], bidirectional=c["bidir"], causal=c["causal"], key_mask=mask, q_offset=off)
+    assert torch.equal(again, got["out"])
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    c = _case(2, 2, 1, 37, 45, 64, "float16", "f32", buckets=8, far=12, mask="bool", offset=3)
+    dev, mask, keep, offset = _inputs(c, 4)
+    got = _run(c, dev, mask, offset)
+    g = torch.Generator().manual_seed(2)
+    a = [torch.where(torch.isfinite(t), t, torch.zeros((), dtype=t.dtype, device=t.device)).double().cpu() for t in dev]
+    for n, name in enumerate(("dq", "dk", "dv", "dtable")):
+        d = torch.randn(a[n].shape, generator=g, dtype=torch.float64)
+        f = []
+        for t in (1e-4, -1e-4):
+            x = list(a[:4])
+            x[n] = x[n] + t * d
+            f.append((oracle.relative_attention(*x, max_distance=12, keep=keep, q_offset=offset) * a[4]).sum().item())
+        want = (f[0] - f[1]) / 2e-4
+        # every element of the gradient carries a few half steps of f16, independent of the direction's signs
+        tol = 8 * torch.finfo(torch.float16).eps * (got[name].double().cpu() * d).norm().item() * 4 + 1e-5 * abs(want)
+        assert abs((got[name].double().cpu() * d).sum().item() - want) <= tol + 2.0 ** -24 * d.numel(), name
+
+
+@pytest.mark.gpu
+def test_infinite_table_entries_forbid_a_bucket():
+    c = _case(1, 2, 2, 70, 70, 64, "bfloat16", "f32", buckets=8, far=12)
+    dev, mask, keep, offset = _inputs(c, 6)
+    dev[3][4:] = float("-inf")     # nothing behind the query
+    dev[3][0, 1] = float("-inf")   # nor itself, for head 1: row 0 keeps no key
+    got = _run(c, dev, mask, offset)
+    q, k, v, t, do = (x.double().cpu() for x in dev)
+    rel = torch.arange(70)[None] - torch.arange(70)[:, None]
+    b = oracle.bucket_map(70, 70, 0, 8, 12, True)
+    z = (q @ k.transpose(2, 3)) / 8 + t[b].permute(2, 0, 1)
+    p = torch.nan_to_num(torch.softmax(z, -1), nan=0.0)
+    want = (p @ v).transpose(1, 2)
+    assert not got["out"][0, 0, 1].any() and all(torch.isfinite(x).all() for x in got.values())
+    assert (got["out"].double().cpu() - want).norm() <= 6 * 2.0 ** -8 * want.norm()
+    assert not got["dtable"][4:].any() and got["dtable"][0, 1] == 0
+
+
+@pytest.mark.gpu
+def test_no_rows_no_keys_no_samples():
+    table = torch.randn(32, 2, device="cuda", requires_grad=True)
+    for B, Lq, Lk in ((2, 0, 5), (2, 5, 0), (0, 4, 4), (1, 200, 0), (2, 0, 0)):
+        q = torch.randn(B, 2, Lq, 64, device="cuda").bfloat16().requires_grad_(True)
+        k, v = (torch.randn(B, 2, Lk, 64, device="cuda").bfloat16().requires_grad_(True) for _ in range(2))
+        out = relative_attention(q, k, v, table)
+        grads = torch.autograd.grad(out, (q, k, v, table), torch.ones_like(out))
+        assert out.shape == (B, Lq, 2, 64) and not out.any() and all(not g.any() and g.shape == t.shape for g, t in zip(grads, (q, k, v, table)))
+
+
+@pytest.mark.gpu
+def test_rows_more_than_32_bits_apart():
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 22 GiB of device memory")
+    g = torch.Generator().manual_seed(8)
+    L, far = 620, 1 << 23
+    store = torch.empty(L * far, dtype=torch.bfloat16, device="cuda")     # the last rows lie past 2^32 elements
+    rows = torch.randn(2, 1, 1, L, 64, generator=g).bfloat16().cuda()
+    k, v = (store.as_strided((1, 1, L, 64), (0, 0, far, 1), o) for o in (0, 64))
+    k.copy_(rows[0])
+    v.copy_(rows[1])
+    q = torch.randn(1, 1, 200, 64, generator=g).bfloat16().cuda()
+    table = torch.randn(32, 1, generator=g).cuda()
+    for n in (1, 200):
+        a = relative_attention(q[:, :, :n], k, v, table, q_offset=400)
+        assert torch.equal(a, relative_attention(q[:, :, :n], rows[0], rows[1], table, q_offset=400))
+
+
+@pytest.mark.gpu
+def test_repeatable_captured_and_on_two_streams():
+    cs = [_case(4, 8, 2, 130, 130, 64, mask="bool"), _case(4, 8, 2, 1, 900, 64, causal=True, bidir=False, mask="lengths", offset="tensor")]
+    for c in cs:
+        dev, mask, keep, offset = _inputs(c)
+        want = {n: t.clone() for n, t in _run(c, dev, mask, offset).items()}
+        offset = offset.cuda() if isinstance(offset, torch.Tensor) else offset
+        s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+        got = []
+        for s in (s1, s2, s1):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(_run(c, dev, mask, offset))
+        for s in (s1, s2):
+            torch.cuda.current_stream().wait_stream(s)
+        for other in got:
+            assert all(torch.equal(other[n], want[n]) for n in want)
+        graphs = []
+        torch.cuda.synchronize()
+        for _ in range(2):     # two graphs: each has workspaces of its own
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                held = _run(c, dev, mask, offset)
+            graphs.append((graph, held))
+        for _ in range(3):
+            for graph, held in graphs:
+                for t in held.values():
+                    t.fill_(3.0)
+                graph.replay()
+            torch.cuda.synchronize()
+            for graph, held in graphs:
+                assert all(torch.equal(held[n], want[n]) for n in want)
+            fresh = _run(c, dev, mask, offset)
+            assert all(torch.equal(fresh[n], want[n]) for n in want)
+
+
+@pytest.mark.gpu
+def test_only_some_gradients_are_wanted():
+    c = _case(2, 2, 1, 66, 66, 64)
+    dev, mask, keep, offset = _inputs(c)
+    want = _run(c, dev, mask, offset)
+    for n, name in enumerate(("dq", "dk", "dv", "dtable")):
+        leaves = [t.detach() for t in dev[:4]]
+        leaves[n].requires_grad_(True)
+        out = relative_attention(*leaves)
+        (got,) = torch.autograd.grad(out, leaves[n], dev[4].expand(2, *dev[4].shape[1:]))
+        assert torch.equal(got, want[name]), name
+
+
+def test_struct_layout_matches_header():
+    from mmlearn_amd import _lib
+
+    src = '#include <stdio.h>\n#include "mmlearn_hip.h"\nint main(){printf("%zu %zu", sizeof(mmk_rel_attn), offsetof(mmk_rel_attn, scale));return 0;}'
+    exe = "/tmp/_mmk_rel_sizeof"
+    subprocess.run(["gcc", "-x", "c", "-", "-I", os.path.join(ROOT, "include"), "-o", exe], input=src, text=True, check=True)
+    size, scale = map(int, subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split())
+    assert ctypes.sizeof(_lib.RelAttn) == size and _lib.RelAttn.scale.offset == scale
+
+
+def test_bucket_borders():
+    for buckets, far, bidir in ((32, 128, True), (32, 128, False), (64, 256, True), (16, 40, True), (2, 1, False), (4, 2, True), (256, 512, True), (8, 9, True)):
+        near, borders, n = K.relative_buckets(buckets, far, bidir)
+        side = buckets // 2 if bidir else buckets
+        assert near == side // 2 and n == side - near - 1
+        for d in range(far + 5):
+            mine = d if d < near else near + sum(min(d, far) >= borders[t] for t in range(n))
+            assert mine == oracle.bucket(-min(d, far), buckets, far, bidir), (buckets, far, bidir, d)
+
+
+def test_buckets_agree_with_the_hf_text_models():
+    modeling = pytest.importorskip("transformers.models.t5.modeling_t5")
+    rel = torch.arange(-300, 301)
+    for bidir in (True, False):
+        want = modeling.T5Attention._relative_position_bucket(rel, bidir, 32, 128)
+        assert want.tolist() == [oracle.bucket(max(-128, min(128, r)), 32, 128, bidir) for r in rel.tolist()]
+
+
+def test_refusals(monkeypatch):
+    from mmlearn_amd import attention as A
+
+    def bf(*shape):
+        return torch.zeros(*shape, dtype=torch.bfloat16)
+
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        relative_attention(bf(1, 1, 1, 64), bf(1, 1, 1, 64), bf(1, 1, 1, 64), torch.zeros(32, 1))
+    monkeypatch.setattr(A.K, "require_gpu", lambda *a: None)
+    monkeypatch.setattr(A._RelativeAttention, "apply", lambda *a: pytest.fail("reached the kernel"))
+    q, k, t = bf(2, 4, 6, 64), bf(2, 2, 8, 64), torch.zeros(32, 4)
+    flat = bf(2 * 4 * 6 * 64 + 8)
+    for bad in (
+        dict(q=q[0]), dict(q=q.float(), k=k.float(), v=k.float()), dict(k=k.half()), dict(v=k[:, :, :7]), dict(k=k[:1], v=k[:1]), dict(k=bf(2, 3, 8, 64), v=bf(2, 3, 8, 64)),
+        dict(q=bf(2, 4, 6, 32), k=bf(2, 2, 8, 32), v=bf(2, 2, 8, 32)), dict(k=bf(2, 0, 8, 64), v=bf(2, 0, 8, 64)), dict(q=bf(2, 4, 6, 128)[..., ::2]),
+        dict(q=bf(2, 4, 6, 68)[..., :64]), dict(q=flat[1:1 + q.numel()].view(q.shape)), dict(table=t[:, :3]), dict(table=t.bfloat16().half()), dict(table=t[0]),
+        dict(table=torch.zeros(4, 32).t()), dict(table=torch.zeros(31, 4)), dict(table=torch.zeros(2, 4)), dict(table=torch.zeros(258, 4)),
+        dict(table=torch.zeros(1, 4), bidirectional=False), dict(max_distance=8), dict(max_distance=513), dict(max_distance=16.5),
+        dict(key_mask=torch.ones(2, 7, dtype=torch.bool)), dict(key_mask=torch.ones(2, 8)), dict(key_mask=torch.ones(2, 8, dtype=torch.int16)), dict(key_mask=torch.ones(3, dtype=torch.int32)),
+        dict(key_mask=torch.ones(2, dtype=torch.bool)), dict(key_mask=torch.ones(8, 2, dtype=torch.bool).t()), dict(key_mask=torch.ones(1, 8, dtype=torch.bool)),
+        dict(q_offset=1.5), dict(q_offset=1 << 29), dict(q_offset=torch.zeros(2)), dict(q_offset=torch.zeros(3, dtype=torch.int32)), dict(q_offset=torch.zeros(2, dtype=torch.int64)),
+        dict(table=t.to("meta")),
+    ):
+        with pytest.raises(ValueError):
+            relative_attention(**{"q": q, "k": k, "v": k, "table": t, **bad})
