@@ -48,7 +48,7 @@ enum {
   MMK_K_IJEPA_LOSS_BWD, MMK_K_GATHER_ROWS, MMK_K_SCATTER_ROWS, MMK_K_PRED_ASSEMBLE, MMK_K_PRED_ASSEMBLE_BWD,
   MMK_K_EMA, MMK_K_MASK_INDEX, MMK_K_LAYERNORM_FWD, MMK_K_LAYERNORM_BWD, MMK_K_ACT, MMK_K_ATTN_FWD,
   MMK_K_ATTN_BWD, MMK_K_WGRAD, MMK_K_RECALL, MMK_K_CLIP_FUSED, MMK_K_MLP_GEMM, MMK_K_WIN_ATTN_FWD, MMK_K_WIN_ATTN_BWD, MMK_K_CLIP_BWD_FUSED,
-  MMK_K_QK_NORM, MMK_K_REL_ATTN_FWD, MMK_K_REL_ATTN_BWD, MMK_K_COUNT
+  MMK_K_QK_NORM, MMK_K_REL_ATTN_FWD, MMK_K_REL_ATTN_BWD, MMK_K_NEWTON_SCHULZ, MMK_K_COUNT
 };
 int mmk_profile_enable(int on);          /* on=1 start recording (clears), on=0 stop */
 /* resolve recorded events (synchronises on them); fills count[k] and total_ms[k] for k < MMK_K_COUNT */
@@ -608,6 +608,26 @@ int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, float* lse, float* ws, vo
 int64_t mmk_rel_attn_bwd_ws_floats(const mmk_rel_attn* p, int want_dtable);
 int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dtable,
                      float* ws, void* stream);
+
+/* Orthogonalised update of `count` matrices [rows, cols] of one shape by a quintic Newton-Schulz iteration (the step of a Muon-type
+ * optimizer; beside mmk_adamw_update, which serves TrainingTask.configure_optimizers, mmlearn/tasks/base.py:72-155):
+ *   X = G / (|G|_F + eps);  `steps` times  A = X X^T, X <- coef[0] X + (coef[1] A + coef[2] A^2) X   (G transposed where rows > cols).
+ * src / momenta / dst: HOST arrays of `count` device addresses.  src: elements of `dtype` at row_stride / col_stride.  momenta (NULL: G = src):
+ * f32 [rows][cols] contiguous buffers, moved on first: M <- momentum M + src, G = nesterov ? src + momentum M : M.  dst: bf16 [rows][cols]
+ * results; with `weights`, f32 [rows][cols] weights that are stepped instead: W <- W (1 - lr weight_decay) - lr adjust X, lr from *lr_dev
+ * (device) where that is given.  Sides up to 32768.  ws: mmk_newton_schulz_ws_bytes() bytes, 16-byte aligned. */
+typedef struct {
+  const void* const* src;
+  void* const* momenta;
+  void* const* dst;
+  const float* lr_dev;
+  int64_t row_stride, col_stride;
+  int32_t count, rows, cols, dtype, steps, nesterov, weights;
+  float coef[3], eps, momentum, lr, adjust, weight_decay;
+  int32_t pad;
+} mmk_newton_schulz_args;
+int64_t mmk_newton_schulz_ws_bytes(int count, int rows, int cols);
+int mmk_newton_schulz(const mmk_newton_schulz_args* args, void* ws, void* stream);
 
 #ifdef __cplusplus
 }

@@ -32,7 +32,7 @@ KERNEL_NAMES = [
     "grad_finalize", "l2norm", "ijepa_loss_fwd", "ijepa_loss_bwd", "gather_rows", "scatter_rows", "pred_assemble",
     "pred_assemble_bwd", "ema_update", "mask_to_index", "layernorm_fwd", "layernorm_bwd", "activation", "attn_fwd", "attn_bwd", "wgrad", "recall_ranks", "clip_fused", "mlp_gemm",
     "win_attn_fwd", "win_attn_bwd", "clip_bwd_fused", "qk_norm",
-    "rel_attn_fwd", "rel_attn_bwd",
+    "rel_attn_fwd", "rel_attn_bwd", "newton_schulz",
 ]
 
 
@@ -88,6 +88,14 @@ class RelAttn(C.Structure):
                 + [(n, C.c_int32) for n in ("B", "H", "Hk", "Lq", "Lk", "D", "dtype", "table_dtype", "mask_kind", "buckets", "near_buckets",
                                             "n_borders", "max_distance", "bidirectional", "causal", "q_offset")]
                 + [("scale", C.c_float), ("pad", C.c_int32)])
+
+
+class NewtonSchulz(C.Structure):
+    """mirror of ``mmk_newton_schulz_args``"""
+
+    _fields_ = ([(n, C.c_void_p) for n in ("src", "momenta", "dst", "lr_dev")] + [("row_stride", C.c_int64), ("col_stride", C.c_int64)]
+                + [(n, C.c_int32) for n in ("count", "rows", "cols", "dtype", "steps", "nesterov", "weights")]
+                + [("coef", C.c_float * 3)] + [(n, C.c_float) for n in ("eps", "momentum", "lr", "adjust", "weight_decay")] + [("pad", C.c_int32)])
 
 
 _vp, _i, _f = C.c_void_p, C.c_int, C.c_float
@@ -179,6 +187,8 @@ _i64 = C.c_int64
 _SIGNATURES.update({
     "mmk_qk_norm_rotary_fwd": [_vp] * 5 + [_i, _vp, _i, _i64, _vp, _vp] + [_i] * 7 + [_vp, _vp, _f, _i, _i, _vp],
     "mmk_qk_norm_rotary_part_rows": [_i64, _i],
+    "mmk_newton_schulz_ws_bytes": [_i, _i, _i],
+    "mmk_newton_schulz": [_vp, _vp, _vp],
     "mmk_rel_attn_fwd_ws_floats": [_vp],
     "mmk_rel_attn_fwd": [_vp] * 5,
     "mmk_rel_attn_bwd_ws_floats": [_vp, _i],
@@ -215,7 +225,8 @@ def lib() -> C.CDLL:
             fn = getattr(l, name)
             fn.argtypes = args
             fn.restype = C.c_int
-        for name in ("mmk_embedding_bwd_scratch_bytes", "mmk_rel_attn_fwd_ws_floats", "mmk_rel_attn_bwd_ws_floats"):
+        for name in ("mmk_embedding_bwd_scratch_bytes", "mmk_rel_attn_fwd_ws_floats", "mmk_rel_attn_bwd_ws_floats",
+                     "mmk_newton_schulz_ws_bytes"):
             getattr(l, name).restype = C.c_int64
         for name, args in _STR_FUNCS.items():
             fn = getattr(l, name)

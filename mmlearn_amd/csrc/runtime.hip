@@ -147,7 +147,7 @@ const char* mmk_kernel_name(int id) {
       "grad_finalize", "l2norm", "ijepa_loss_fwd", "ijepa_loss_bwd", "gather_rows", "scatter_rows", "pred_assemble",
       "pred_assemble_bwd", "ema_update", "mask_to_index", "layernorm_fwd", "layernorm_bwd", "activation", "attn_fwd",
       "attn_bwd", "wgrad", "recall_ranks", "clip_fused", "mlp_gemm", "win_attn_fwd", "win_attn_bwd", "clip_bwd_fused",
-      "qk_norm", "rel_attn_fwd", "rel_attn_bwd"};
+      "qk_norm", "rel_attn_fwd", "rel_attn_bwd", "newton_schulz"};
   if (id < 0 || id >= MMK_K_COUNT) return "?";
   return names[id];
 }

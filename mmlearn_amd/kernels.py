@@ -1435,3 +1435,25 @@ def rel_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch
             ws = torch.empty(max(1, _lib.lib().mmk_rel_attn_bwd_ws_floats(C.byref(p), int(want_dtable))), dtype=torch.float32, device=q.device)
             check(_lib.lib().mmk_rel_attn_bwd(C.byref(p), ptr(out), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws), stream()))
     return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dtable
+
+
+# ------------------------------------------------------------------ orthogonalised updates (Newton-Schulz)
+def newton_schulz(src: Sequence[int], dst: Sequence[int], rows: int, cols: int, strides: Tuple[int, int], dtype: torch.dtype,
+                  device: torch.device, steps: int, coefficients: Sequence[float], eps: float, momenta: Optional[Sequence[int]] = None,
+                  momentum: float = 0.0, nesterov: bool = False, weights: bool = False, lr: float = 0.0, adjust: float = 1.0,
+                  weight_decay: float = 0.0, lr_dev: Optional[torch.Tensor] = None) -> None:
+    """Device addresses of equally shaped matrices -> their orthogonalised updates (bf16 at ``dst``), or with ``weights`` the step of the f32
+    weights at ``dst``; ``momenta``: f32 buffers moved on first.  ``device`` is the current one.  csrc/newton_schulz.hip."""
+    n = len(src)
+    array = C.c_void_p * max(n, 1)
+    p = _lib.NewtonSchulz()
+    keep = [array(*src), array(*dst), None if momenta is None else array(*momenta)]   # host arrays, read during the call
+    p.src, p.dst, p.momenta = (None if x is None else C.cast(x, C.c_void_p) for x in keep)
+    p.lr_dev = ptr(lr_dev)
+    p.row_stride, p.col_stride = strides
+    p.count, p.rows, p.cols, p.dtype, p.steps, p.nesterov, p.weights = n, rows, cols, dtype_tag(dtype), steps, int(nesterov), int(weights)
+    p.coef[:] = coefficients
+    p.eps, p.momentum, p.lr, p.adjust, p.weight_decay = eps, momentum, lr, adjust, weight_decay
+    size = _lib.lib().mmk_newton_schulz_ws_bytes(n, rows, cols)
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
+    check(_lib.lib().mmk_newton_schulz(C.byref(p), ptr(ws), stream()))

@@ -1,4 +1,6 @@
-"""``AdamW`` with the update as ONE multi-tensor HIP launch per parameter group (``csrc/ijepa.hip::adamw_kernel``).
+"""``AdamW`` and ``Muon`` (with its operator ``orthogonalize``) as HIP launches over whole parameter groups.
+
+``AdamW``: the update as ONE multi-tensor HIP launch per parameter group (``csrc/ijepa.hip::adamw_kernel``).
 
 Same algorithm and hyper-parameters as ``torch.optim.AdamW`` (decoupled weight decay, bias correction, ``amsgrad`` /
 ``maximize`` off) for f32 parameters on the GPU; the foreach implementation makes ~7 passes of 15-25 launches over the
@@ -24,11 +26,13 @@ kept alive for the optimizer's lifetime, so an eager step with other gradient ad
 from __future__ import annotations
 
 import ctypes as C
-from typing import Any, Dict, List
+import math
+from typing import Any, Dict, List, Sequence
 
 import torch
 
 from . import _lib
+from . import kernels as K
 from .kernels import check, dtype_tag, require_gpu, stream
 
 
@@ -188,3 +192,123 @@ class AdamW(torch.optim.Optimizer):
         """The device word a captured step reads its learning rate from (``capturable=True``, after the first eager step):
         ``opt.lr_device(g).fill_(new_lr)`` between replays is what a scheduler's ``group["lr"] = ...`` is for eager steps."""
         return self._dev_words[group_index]["lr"]
+
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # quintic of a steep start: singular values from 1e-2 up end within 0.7 .. 1.2 after 5 steps
+
+
+def _check_iteration(name: str, steps: int, coefficients: Sequence[float], eps: float) -> None:
+    if not (isinstance(steps, int) and 1 <= steps <= 32):
+        raise ValueError(f"{name}: 1 to 32 Newton-Schulz steps")
+    if len(coefficients) != 3 or not all(math.isfinite(c) and abs(c) <= 64 for c in coefficients):
+        raise ValueError(f"{name}: three finite coefficients of at most 64 in size")
+    if not (math.isfinite(eps) and eps > 0):
+        raise ValueError(f"{name}: eps must be positive")
+
+
+@torch.no_grad()
+def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients: Sequence[float] = NS_COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
+    """The matrices of ``update`` ``[..., rows, cols]`` (f32 / bf16 / f16, any strides, sides up to 32768) with their singular values driven towards
+    1: ``X = G / (|G| + eps)``, then ``steps`` times ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``.  Returns bf16, contiguous: the
+    products run on 16-bit operands (csrc/newton_schulz.hip), whose errors of about 1e-3 a finer result would only carry along.  A matrix
+    of zeros stays zero; one that holds a NaN or an infinity becomes NaN.  The coefficients must keep singular values below about 4."""
+    require_gpu(update, "update")
+    name = "mmlearn_amd.optim.orthogonalize"
+    _check_iteration(name, steps, coefficients, eps)
+    if update.dim() < 2 or update.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"{name}: need a [..., rows, cols] tensor of float32, bfloat16 or float16")
+    rows, cols = update.shape[-2:]
+    if max(rows, cols) > 32768:
+        raise ValueError(f"{name}: sides up to 32768")
+    with _lib.on_device_of(update):
+        out = torch.empty(update.shape, dtype=torch.bfloat16, device=update.device)
+        if out.numel():
+            g = update.reshape(-1, rows, cols)
+            first, size = g.data_ptr(), g.element_size()
+            K.newton_schulz([first + i * g.stride(0) * size for i in range(g.shape[0])], [out.data_ptr() + i * rows * cols * 2 for i in range(g.shape[0])],
+                            rows, cols, (g.stride(1), g.stride(2)), g.dtype, g.device, steps, coefficients, eps)
+    return out
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update is orthogonalised, for the weight MATRICES of a tower (``AdamW`` takes the rest): per step
+
+        ``M <- momentum M + g``,  ``u = g + momentum M`` (``nesterov``) or ``M``,
+        ``w <- w (1 - lr weight_decay) - lr adjust orthogonalize(u)``
+
+    with ``adjust = sqrt(max(1, rows / cols))`` (``adjust_lr_fn`` None or ``"original"``) or ``0.2 sqrt(max(rows, cols))``
+    (``"match_rms_adamw"``: the update's root mean square is that of AdamW, whose learning rates then carry over).  Arguments, formulas and
+    state (``momentum_buffer``) as in ``torch.optim.Muon``; parameters are dense contiguous f32 matrices on the GPU.  Momentum,
+    normalisation and the step of the weights are part of the launches; all matrices of one shape run as one batch.
+
+    ``capturable=True``: the learning rate is read from a device word (``lr_device(g)``), so a captured step follows it.  A captured step
+    bakes in the addresses of weights, gradients and momenta: run one eager step before capturing and keep the gradients
+    (``zero_grad(set_to_none=False)``)."""
+
+    def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95, nesterov: bool = True,
+                 ns_coefficients: Sequence[float] = NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5, adjust_lr_fn=None,
+                 capturable: bool = False):
+        if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0:
+            raise ValueError("invalid Muon hyper-parameters")
+        _check_iteration("mmlearn_amd.optim.Muon", ns_steps, ns_coefficients, eps)
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError(f"unknown adjust_lr_fn {adjust_lr_fn!r}")
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=bool(nesterov), ns_coefficients=tuple(ns_coefficients),
+                                      eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn, capturable=bool(capturable)))
+        self._lr_words: Dict[Any, Any] = {}
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                raise ValueError(f"mmlearn_amd.optim.Muon takes matrices; got a parameter of shape {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for gi, group in enumerate(self.param_groups):
+            batches: Dict[Any, List[torch.Tensor]] = {}
+            for p in group["params"]:
+                if p.grad is None or p.numel() == 0:
+                    continue
+                require_gpu(p)
+                if p.dtype != torch.float32 or not p.is_contiguous() or p.grad.is_sparse:
+                    raise RuntimeError("mmlearn_amd.optim.Muon supports dense contiguous f32 parameters")
+                batches.setdefault((p.device, tuple(p.shape), p.grad.dtype, p.grad.stride()), []).append(p)
+            for (device, (rows, cols), dtype, strides), plist in batches.items():
+                with _lib.on_device_of(plist[0]):
+                    self._step_batch(gi, group, plist, rows, cols, strides, dtype, device)
+        return loss
+
+    def _step_batch(self, gi, group, plist, rows, cols, strides, dtype, device) -> None:
+        capturing = torch.cuda.is_current_stream_capturing()
+        for p in plist:
+            st = self.state[p]
+            buf = st.get("momentum_buffer")
+            if buf is None or buf.dtype != torch.float32 or not buf.is_contiguous() or buf.device != p.device:
+                if capturing:
+                    raise RuntimeError("mmlearn_amd.optim.Muon: run one eager step before capturing")
+                st["momentum_buffer"] = (torch.zeros_like(p, memory_format=torch.contiguous_format) if buf is None
+                                         else buf.to(device=p.device, dtype=torch.float32).contiguous())
+        word = None
+        if group.get("capturable", False):
+            word, seen = self._lr_words.get((gi, device), (None, None))
+            if word is None or (not capturing and seen != group["lr"]):
+                if capturing:
+                    raise RuntimeError("mmlearn_amd.optim.Muon(capturable=True): run one eager step before capturing")
+                word = torch.empty(1, dtype=torch.float32, device=device) if word is None else word
+                word.fill_(float(group["lr"]))
+                self._lr_words[gi, device] = (word, group["lr"])
+        adjust = 0.2 * math.sqrt(max(rows, cols)) if group["adjust_lr_fn"] == "match_rms_adamw" else math.sqrt(max(1.0, rows / cols))
+        K.newton_schulz([p.grad.data_ptr() for p in plist], [p.data_ptr() for p in plist], rows, cols, strides, dtype, device, group["ns_steps"],
+                        group["ns_coefficients"], group["eps"], [self.state[p]["momentum_buffer"].data_ptr() for p in plist], group["momentum"],
+                        group["nesterov"], True, float(group["lr"]), adjust, group["weight_decay"], word)
+        torch.autograd.graph.increment_version(plist)
+
+    def lr_device(self, group_index: int = 0, device=None) -> torch.Tensor:
+        """The device word a captured step reads its learning rate from (``capturable=True``, after the first eager step)."""
+        words = {d: w for (g, d), (w, _) in self._lr_words.items() if g == group_index}
+        return words[torch.device(device)] if device is not None else next(iter(words.values()))
