@@ -556,17 +556,47 @@ __global__ __launch_bounds__(256) void rel_join_kernel(const RelArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, dtable
+// Sums of a 32 x 32 tile of dS^T along its diagonals.  Register e of lane (row R of 16 lanes, c = lane & 15, half hf) is key
+// 16 K + n + 4 hf (n = acc_row(e) & 15, K = e >> 3) and query 16 R + c.  Shifting the register by n lanes within its row of 16 puts equal
+// distances into one lane: what stays in the row has distance 16 (K - R) + 4 hf - c, what leaves it on the other side 16 more.  With
+// row shifts that fill with zeros both parts are one DPP add each.  d[k] of a lane: the sum at distance 16 (k - R) + 4 hf - c from the
+// tile's corner.
+template <int N>
+__device__ __forceinline__ void rel_diag_add(float x, float& stay, float& leave) {
+  if (N == 0) {
+    stay += x;
+  } else {
+    const int xi = __builtin_bit_cast(int, x);
+    stay += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, xi, 0x100 + (N & 15), 0xf, 0xf, true));           // lane c takes lane c + N
+    leave += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, xi, 0x110 + ((16 - N) & 15), 0xf, 0xf, true));   // lane c takes lane c + N - 16
+  }
+}
+__device__ __forceinline__ void rel_diagonals(const f32x16& s, float (&d)[3]) {
+  d[0] = d[1] = d[2] = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    rel_diag_add<0>(s[8 * k + 0], d[k], d[k + 1]);
+    rel_diag_add<1>(s[8 * k + 1], d[k], d[k + 1]);
+    rel_diag_add<2>(s[8 * k + 2], d[k], d[k + 1]);
+    rel_diag_add<3>(s[8 * k + 3], d[k], d[k + 1]);
+    rel_diag_add<8>(s[8 * k + 4], d[k], d[k + 1]);
+    rel_diag_add<9>(s[8 * k + 5], d[k], d[k + 1]);
+    rel_diag_add<10>(s[8 * k + 6], d[k], d[k + 1]);
+    rel_diag_add<11>(s[8 * k + 7], d[k], d[k + 1]);
+  }
+}
+
 // As the forward, with the query on the lane: dS^T needs lse and delta of the lane alone, and dQ^T += K^T dS^T takes it from the
-// accumulators.  dtable: the 32 lanes of a half hold 32 consecutive distances in each register, so each wave half adds them to a vector
-// over the distances of its own (one address per lane: the order of the sums is fixed); tiles beyond max_distance add to two
-// registers.
+// accumulators.  dtable: rel_diagonals sums a near tile along its diagonals in registers, and each group of 16 lanes adds the sums to a
+// vector over the distances of its own (an address is one lane's: plain LDS reads and writes in a fixed order; LDS float atomics
+// took 175 cycles a wave instruction, which made this kernel 3.5 times slower).  Tiles beyond max_distance add to two registers.
 template <typename T, int D, int NQ>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, QB = 128 * NQ, EXT = 32 + 32 * NQ;
+  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, QB = 128 * NQ, EXT = 64 + 32 * NQ;
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int nbias = (2 * (a.far + EXT) + 1 + 3) & ~3;
-  float* diag = bias + nbias;   // [8][nbias]: per wave half
+  float* diag = bias + nbias;   // [16][nbias]: per group of 16 lanes
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
   const int nqb = (a.Lq + QB - 1) / QB, item = rel_item(blockIdx.x, gridDim.x);
@@ -583,8 +613,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
   const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + (h / a.G) * a.v_sh;
   rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
   if (a.dtab_part)
-    for (int x = tid; x < 8 * nbias; x += 256) diag[x] = 0.f;
-  float* my_diag = diag + (2 * wave + hf) * nbias;
+    for (int x = tid; x < 16 * nbias; x += 256) diag[x] = 0.f;
+  float* my_diag = diag + (tid >> 4) * nbias + 4 * hf - (lane & 31);
 
   s16x8 qf[NQ][D / 16], gf[NQ][D / 16];
   f32x16 dq[NQ][D / 32];
@@ -689,8 +719,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
             far_l += left ? t4 : 0.f;
             far_r += left ? 0.f : t4;
           } else {
+            float d[3];
+            rel_diagonals(s[qs], d);
+            float* at = my_diag + (a.far + EXT + jt - (i_wave + 32 * qs + off));   // (lane & 31 = 16 R + c)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) __hip_atomic_fetch_add(my_diag + at0 + acc_row(e), s[qs][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int k = 0; k < 3; ++k) d[k] += at[16 * k];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) at[16 * k] = d[k];
           }
         }
         df[qs][0] = rel_operand<T>(s[qs], 0);
@@ -712,14 +747,14 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
     if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, dq[qs], a.scale, hf);
   }
   if (!a.dtab_part) return;
-  // ---- this workgroup's sums by bucket: the far sums join their wave's vectors at its ends, the eight vectors are added in order, and
+  // ---- this workgroup's sums by bucket: the far sums join their wave's vectors at its ends, the sixteen vectors are added in order, and
   // a thread per (bucket, slice) collects its distances
   far_l = wave_sum(far_l);
   far_r = wave_sum(far_r);
   __syncthreads();
   if (lane == 0) {
-    diag[2 * wave * nbias] += far_l;
-    diag[2 * wave * nbias + 2 * (a.far + EXT)] += far_r;
+    diag[4 * wave * nbias] += far_l;
+    diag[4 * wave * nbias + 2 * (a.far + EXT)] += far_r;
   }
   __syncthreads();
   const int n = 2 * (a.far + EXT) + 1;
@@ -727,7 +762,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
   for (int x = tid; x < n; x += 256) {
     float t = 0.f;
 #pragma unroll
-    for (int v = 0; v < 8; ++v) t += diag[v * nbias + x];
+    for (int v = 0; v < 16; ++v) t += diag[v * nbias + x];
     diag[x] = t;
     which[x] = rel_bucket(a, min(max(x - a.far - EXT, -a.far), a.far));
   }
@@ -892,8 +927,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dkv_kernel(const Rel
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// Queries per wave, 32 NQ.
-static int rel_nq(const mmk_rel_attn* p) { return p->D == 64 ? 2 : 1; }
+// Queries per wave, 32 NQ.  Two blocks share every K / V fragment read from LDS, which is what bounds D = 64 otherwise; a sequence that one
+// workgroup of 128 rows covers would leave half the waves idle (256 x 12 heads x 77 rows: 58 us with two blocks, 36 with one); at
+// D = 128 two blocks do not fit the registers of two waves a SIMD.
+static int rel_nq(const mmk_rel_attn* p) { return p->D == 64 && p->Lq > 128 ? 2 : 1; }
 static int rel_dq_blocks(const mmk_rel_attn* p) { return (p->Lq + 128 * rel_nq(p) - 1) / (128 * rel_nq(p)); }
 
 constexpr int REL_LDS = 160 * 1024;
@@ -995,19 +1032,32 @@ static int rel_forward(const mmk_rel_attn* p, RelArgs& a, hipStream_t st) {
     const int64_t n = (int64_t)a.B * a.H * a.Lq * (D / 4);
     return rel_launch(rel_join_kernel<T, D>, MMK_K_REL_ATTN_FWD, (n + 255) / 256, 0, 0, a, st);
   }
-  constexpr int NQ = D == 64 ? 2 : 1, EXT = 64 + 32 * NQ, TILES = 2 * 2 * (D / 64) * 8192;
-  const int64_t grid = (int64_t)a.B * a.H * ((a.Lq + 128 * NQ - 1) / (128 * NQ));
-  return rel_launch(rel_fwd_kernel<T, D, NQ>, MMK_K_REL_ATTN_FWD, grid, TILES + rel_vec_bytes(a.far, EXT), TILES + rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
+  constexpr int TILES = 2 * 2 * (D / 64) * 8192;
+  auto go = [&](auto nq) {
+    constexpr int NQ = decltype(nq)::value, EXT = 64 + 32 * NQ;
+    const int64_t grid = (int64_t)a.B * a.H * ((a.Lq + 128 * NQ - 1) / (128 * NQ));
+    return rel_launch(rel_fwd_kernel<T, D, NQ>, MMK_K_REL_ATTN_FWD, grid, TILES + rel_vec_bytes(a.far, EXT), TILES + rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
+  };
+  if constexpr (D == 64) {
+    if (rel_nq(p) == 2) return go(std::integral_constant<int, 2>());
+  }
+  return go(std::integral_constant<int, 1>());
 }
 
 template <typename T, int D>
 static int rel_backward(const mmk_rel_attn* p, RelArgs& a, void* dtable, hipStream_t st) {
-  constexpr int NQ = D == 64 ? 2 : 1, EXT = 32 + 32 * NQ, TILES = 2 * 2 * (D / 64) * 8192;
+  constexpr int TILES = 2 * 2 * (D / 64) * 8192;
   const int nqb = rel_dq_blocks(p);
   if (a.Lq > 0) {
-    const int lds = TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 9 : 1);
-    if (int rc = rel_launch(rel_dq_kernel<T, D, NQ>, MMK_K_REL_ATTN_BWD, (int64_t)a.B * a.H * nqb, lds, TILES + 9 * rel_vec_bytes(REL_MAX_FAR, EXT), a, st))
-      return rc;
+    auto go = [&](auto nq) {
+      constexpr int NQ = decltype(nq)::value, EXT = 64 + 32 * NQ;
+      const int lds = TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 17 : 1);
+      return rel_launch(rel_dq_kernel<T, D, NQ>, MMK_K_REL_ATTN_BWD, (int64_t)a.B * a.H * nqb, lds, TILES + 17 * rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
+    };
+    int rc;
+    if constexpr (D == 64) rc = rel_nq(p) == 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
+    else rc = go(std::integral_constant<int, 1>());
+    if (rc) return rc;
   }
   if (a.Lk > 0) {
     const int64_t grid = (int64_t)a.B * a.Hk * ((a.Lk + 127) / 128);
