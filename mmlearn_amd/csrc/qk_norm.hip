@@ -261,21 +261,22 @@ __global__ __launch_bounds__(QKN_THREADS) void qk_norm_kernel(const QkArgs a) {
   }
 }
 
-// dw[d] = sum over the workgroups' partials, 32 columns per workgroup, eight row slices each joined in order
+// dw[d] = sum over the workgroups' partials: 8 columns and 32 row slices a workgroup, each slice in order, the slices joined in order
 template <typename W>
 __global__ __launch_bounds__(256) void qk_norm_dw_kernel(const QkArgs a) {
-  __shared__ float red[8][32];
+  __shared__ float red[32][8];
   const QkSide& s = a.s[blockIdx.y];
   if (s.part == nullptr) return;
-  const int col = threadIdx.x & 31, sl = threadIdx.x >> 5, d = blockIdx.x * 32 + col;
+  const int col = threadIdx.x & 7, sl = threadIdx.x >> 3, d = blockIdx.x * 8 + col;
   float t = 0.f;
-  if (d < a.D)
-    for (int r = sl; r < s.blocks; r += 8) t += s.part[(int64_t)r * a.D + d];
+  if (d < a.D) {
+#pragma unroll 8
+    for (int r = sl; r < s.blocks; r += 32) t += s.part[(int64_t)r * a.D + d];
+  }
   red[sl][col] = t;
   __syncthreads();
   if (sl == 0 && d < a.D) {
-#pragma unroll
-    for (int k = 1; k < 8; ++k) t += red[k][col];
+    for (int k = 1; k < 32; ++k) t += red[k][col];
     reinterpret_cast<W*>(s.dw)[d] = from_f32<W>(t);
   }
 }
@@ -307,7 +308,7 @@ static int qk_launch(const QkArgs& a, bool ilv, bool bwd, hipStream_t st) {
   else ilv ? go(qk_norm_kernel<T, W, V, CP, true, false>) : go(qk_norm_kernel<T, W, V, CP, false, false>);
   MMK_LAUNCH_CHECK();
   if (bwd && (a.s[0].part || a.s[1].part)) {
-    hipLaunchKernelGGL((qk_norm_dw_kernel<W>), dim3((a.D + 31) / 32, 2), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((qk_norm_dw_kernel<W>), dim3((a.D + 7) / 8, 2), dim3(256), 0, st, a);
     MMK_LAUNCH_CHECK();
   }
   return 0;
@@ -322,7 +323,7 @@ static int qk_run(QkArgs& a, bool ilv, bool bwd, hipStream_t st) {
   const int rpb = QKN_THREADS >> a.lpr_log2;
   for (QkSide& s : a.s) {
     const int64_t need = ((int64_t)a.B * a.L * s.H + rpb - 1) / rpb;
-    s.blocks = bwd ? (int)std::min<int64_t>(need, s.blocks) : (int)need;
+    s.blocks = (int)std::min<int64_t>(need, bwd ? s.blocks : QKN_MAX_BLOCKS);
   }
   if (V == 8) return qk_launch<T, W, 8, 1>(a, ilv, bwd, st);
   if (V == 4) return qk_launch<T, W, 4, 1>(a, ilv, bwd, st);
