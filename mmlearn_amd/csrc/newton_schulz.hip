@@ -27,7 +27,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_GROUP = 64;      // matrices of one launch (their addresses are kernel arguments)
-constexpr int NS_PARTS = 256;     // partial sums of squares per matrix
+constexpr int NS_PARTS = 1024;    // partial sums of squares per matrix: at one 64 x 64 tile each, enough workgroups to fill the chip
 constexpr int NS_TILE = 128;
 
 struct NsPtrs {
@@ -76,19 +76,27 @@ __global__ __launch_bounds__(256) void ns_reduce_kernel(const NsArgs a, const Ns
   double sum = 0.0;
   for (int t = blockIdx.x; t < tr * tc; t += NS_PARTS) {
     const int r0 = 64 * (t / tc), c0 = 64 * (t % tc);
-    for (int k = w; k < 64; k += 4) {
-      const int r = r0 + (by_col ? k : l), c = c0 + (by_col ? l : k);
-      if (r >= a.rows || c >= a.cols) continue;
-      float g = to_f32(src[(int64_t)r * a.rs + (int64_t)c * a.cs]);
+    float g[16], mv[16];   // all of a thread's values in flight at once
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int k = w + 4 * u, r = r0 + (by_col ? k : l), c = c0 + (by_col ? l : k);
+      const bool in = r < a.rows && c < a.cols;
+      g[u] = in ? to_f32(src[(int64_t)r * a.rs + (int64_t)c * a.cs]) : 0.f;
+      if (MOM) mv[u] = in ? mom[(int64_t)r * a.cols + c] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
       if (MOM) {
-        const int64_t at = (int64_t)r * a.cols + c;
-        const float mv = fmaf(a.mu, mom[at], g);
-        mom[at] = mv;
-        g = a.nesterov ? fmaf(a.mu, mv, g) : mv;
-        if (a.tall) tile[k][l] = g;
-        else x32[(int64_t)r * a.np + c] = g;
+        const int k = w + 4 * u, r = r0 + k, c = c0 + l;
+        mv[u] = fmaf(a.mu, mv[u], g[u]);
+        g[u] = a.nesterov ? fmaf(a.mu, mv[u], g[u]) : mv[u];
+        if (a.tall) tile[k][l] = g[u];
+        if (r < a.rows && c < a.cols) {
+          mom[(int64_t)r * a.cols + c] = mv[u];
+          if (!a.tall) x32[(int64_t)r * a.np + c] = g[u];
+        }
       }
-      sum += (double)g * (double)g;
+      sum += (double)g[u] * (double)g[u];
     }
     if (MOM && a.tall) {
       __syncthreads();
@@ -112,31 +120,35 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const NsArgs a, const N
   __shared__ double red[256];
   __shared__ float tile[64][65];
   const int mat = blockIdx.y, tid = threadIdx.x, l = tid & 63, w = tid >> 6;
-  red[tid] = a.parts[mat * NS_PARTS + tid];
+  const T* src = reinterpret_cast<const T*>(p.src[mat]);
+  const int tn = a.np / 64, i0 = 64 * (blockIdx.x / tn), j0 = 64 * (blockIdx.x % tn);
+  float* x32 = a.x32 + (int64_t)mat * a.mp * a.np;
+  // read along the axis that is contiguous in memory: j of X, or i
+  const bool by_j = MOM || (a.tall ? a.rs <= a.cs : a.cs <= a.rs);
+  float v[16];
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int k = w + 4 * u, i = i0 + (by_j ? k : l), j = j0 + (by_j ? l : k);
+    v[u] = i < a.m && j < a.n ? (MOM ? x32[(int64_t)i * a.np + j] : to_f32(src[ns_src_at(a, i, j)])) : 0.f;
+  }
+  double sq = 0.0;
+  for (int k = tid; k < NS_PARTS; k += 256) sq += a.parts[mat * NS_PARTS + k];
+  red[tid] = sq;
   __syncthreads();
   for (int o = 128; o > 0; o >>= 1) {
     if (tid < o) red[tid] += red[tid + o];
     __syncthreads();
   }
   const float inv = (float)(1.0 / (sqrt(red[0]) + (double)a.eps));
-  const T* src = reinterpret_cast<const T*>(p.src[mat]);
-  const int tn = a.np / 64, i0 = 64 * (blockIdx.x / tn), j0 = 64 * (blockIdx.x % tn);
-  float* x32 = a.x32 + (int64_t)mat * a.mp * a.np;
-  // read along the axis that is contiguous in memory: j of X, or i
-  const bool by_j = MOM || (a.tall ? a.rs <= a.cs : a.cs <= a.rs);
-  for (int k = w; k < 64; k += 4) {
-    const int ii = by_j ? k : l, jj = by_j ? l : k, i = i0 + ii, j = j0 + jj;
-    float v = 0.f;
-    if (i < a.m && j < a.n) v = (MOM ? x32[(int64_t)i * a.np + j] : to_f32(src[ns_src_at(a, i, j)])) * inv;
-    tile[ii][jj] = v;
-  }
+#pragma unroll
+  for (int u = 0; u < 16; ++u) tile[by_j ? w + 4 * u : l][by_j ? l : w + 4 * u] = v[u] * inv;
   __syncthreads();
   f16_t* x16 = a.x16 + (int64_t)mat * a.mp * a.np;
   f16_t* xt = a.xt[0] + (int64_t)mat * a.mp * a.np;
   for (int k = w; k < 64; k += 4) {
-    const float v = tile[k][l];
-    x32[(int64_t)(i0 + k) * a.np + j0 + l] = v;
-    x16[(int64_t)(i0 + k) * a.np + j0 + l] = (f16_t)(v * a.S);
+    const float x = tile[k][l];
+    x32[(int64_t)(i0 + k) * a.np + j0 + l] = x;
+    x16[(int64_t)(i0 + k) * a.np + j0 + l] = (f16_t)(x * a.S);
     xt[(int64_t)(j0 + k) * a.mp + i0 + l] = (f16_t)(tile[l][k] * a.S);
   }
 }
