@@ -52,6 +52,8 @@ struct RelArgs {
   const void* o;
   void *dq, *dk, *dv;        // contiguous [B, L, heads, D]
   float *delta, *dtab_part;  // [B, H, Lq]; [workgroups of the dQ kernel][buckets] or null
+  float* dkv_part;           // [splits][dK, dV][B, Lk, Hk, D]
+  int dkv_splits;
   // split forward
   float* part;               // partial results of the key splits
   int splits, row_blocks;
@@ -68,9 +70,29 @@ template <>
 __device__ __forceinline__ f32x16 rel_mfma<f16_t>(s16x8 a, s16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ s16x8 rel_row_frag(const char* p) { return *reinterpret_cast<const s16x8*>(p); }
-__device__ __forceinline__ s16x8 rel_tr_frag(const char* img, const ImgLane& il, int off, int ct) {
-  return __builtin_bit_cast(s16x8, lds_tr_frag(img, il, off, ct));
+// Per-lane offsets into an image (attn_image.h: ImgLane) held as two registers: the chunk index is XORed into bits 4 .. 6, so the offset of
+// another k step, half or column block is one XOR away.
+struct RelLane {
+  int row0, tr0;
+  __device__ __forceinline__ explicit RelLane(int lane) {
+    const ImgLane il = img_lane(lane);
+    row0 = il.row[0];
+    tr0 = il.tr[0][0];
+  }
+  // the same offsets, formed anew where they are used: hoisted out of the loop they would pin a register each
+  __device__ __forceinline__ RelLane fresh() const {
+    RelLane o = *this;
+    asm volatile("" : "+v"(o.row0), "+v"(o.tr0));
+    return o;
+  }
+};
+__device__ __forceinline__ s16x8 rel_row_frag(const char* img, const RelLane& il, int kk) {   // k step kk (16 columns) of the lane's row
+  return *reinterpret_cast<const s16x8*>(img + (il.row0 ^ (kk << 5)));
+}
+__device__ __forceinline__ s16x8 rel_tr_frag(const char* img, const RelLane& il, int off, int ct) {   // transposed: rows from off / 128, column block ct
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(img + off + (il.tr0 ^ (ct << 6))));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(img + off + 1024 + (il.tr0 ^ (ct << 6) ^ 16)));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 // eight accumulator registers (one k step) as a B operand
 template <typename T>
@@ -146,22 +168,19 @@ __device__ __forceinline__ int rel_item(int id, int total) {
   return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
 }
 
-// One wave's share of a 64-row tile in LDS: CB column blocks of 64 of X, then of Y, 8 pieces of 8 rows each
-template <typename T, int CB, int NW>
+// One wave's share of a 64-row tile in LDS: CB column blocks of 64 of X, then of Y; of each image's 8 pieces of 8 rows, pieces `wave` and
+// `wave` + 4 (32 rows further, where the swizzle is the same: one per-lane offset serves both)
+template <typename T, int CB>
 struct RelLoader {
-  uint32_t vx[2], vy[2];
+  uint32_t vx, vy;
   __device__ __forceinline__ RelLoader(int64_t x_sl, int64_t y_sl, int wave, int lane) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = 8 * ((wave + NW * u) & 7) + (lane >> 3), ch = (lane & 7) ^ img_swz(row & 15);
-      vx[u] = (uint32_t)(row * (int)x_sl + ch * 8) * 2u;
-      vy[u] = (uint32_t)(row * (int)y_sl + ch * 8) * 2u;
-    }
+    const int row = 8 * wave + (lane >> 3), ch = (lane & 7) ^ img_swz(row & 15);
+    vx = (uint32_t)(row * (int)x_sl + ch * 8) * 2u;
+    vy = (uint32_t)(row * (int)y_sl + ch * 8) * 2u;
   }
   // rows row0 .. row0 + 63 of X and Y (rows past `rows - 1` repeat that row), to the stage at `lds`
   __device__ __forceinline__ void issue(const T* x, const T* y, int64_t x_sl, int64_t y_sl, int row0, int rows, uint32_t lds, int wave,
                                         int lane) const {
-    static_assert(NW == 4, "two pieces of an image per wave");
     const bool whole = row0 + 64 <= rows;
 #pragma unroll
     for (int im = 0; im < 2 * CB; ++im) {
@@ -169,13 +188,13 @@ struct RelLoader {
       const T* base = (im < CB ? x : y) + (int64_t)row0 * sl + 64 * (im % CB);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int piece = wave + NW * u;
-        uint32_t vo = im < CB ? vx[u] : vy[u];
-        if (!whole) {
-          const int row = 8 * piece + (lane >> 3), ch = (lane & 7) ^ img_swz(row & 15);
-          vo = (uint32_t)(min(row, rows - 1 - row0) * (int)sl + ch * 8) * 2u;
+        const uint32_t at = lds + (uint32_t)(im * 8192 + (wave + 4 * u) * 1024);
+        if (whole) {
+          lds_dma16(base + 32 * u * sl, im < CB ? vx : vy, at);
+        } else {
+          const int row = 8 * (wave + 4 * u) + (lane >> 3), ch = (lane & 7) ^ img_swz(row & 15);
+          lds_dma16(base, (uint32_t)(min(row, rows - 1 - row0) * (int)sl + ch * 8) * 2u, at);
         }
-        lds_dma16(base, vo, lds + (uint32_t)(im * 8192 + piece * 1024));
       }
     }
   }
@@ -248,8 +267,8 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
     m[s] = -INFINITY;
     l[s] = 0.f;
   }
-  const ImgLane il = img_lane(lane);
-  const RelLoader<T, CB, 4> ld(a.k_sl, a.v_sl, wave, lane);
+  const RelLane il(lane);
+  const RelLoader<T, CB> ld(a.k_sl, a.v_sl, wave, lane);
   const uint32_t lds0 = lds_addr_of(smem);
   int keep = 1;
   if (nkt > 0) {
@@ -280,7 +299,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
     for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const s16x8 kf = rel_row_frag(K + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]);
+        const s16x8 kf = rel_row_frag(K + (kk >> 2) * 8192 + t * 4096, il, kk & 3);
 #pragma unroll
         for (int qs = 0; qs < NQ; ++qs) s[qs][t] = rel_mfma<T>(kf, qf[qs][kk], s[qs][t]);
       }
@@ -401,7 +420,7 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
     for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_zero();
   }
   float m = -INFINITY, l = 0.f;
-  const ImgLane il = img_lane(lane);
+  const RelLane il(lane);
   const uint32_t lds0 = lds_addr_of(mine);
   auto issue = [&](int t, int stage) {
 #pragma unroll
@@ -443,7 +462,7 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
     }
     f32x16 s = rel_zero();
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) s = rel_mfma<T>(rel_row_frag(K + (kk >> 2) * IMG + il.row[kk & 3]), qf[kk], s);
+    for (int kk = 0; kk < D / 16; ++kk) s = rel_mfma<T>(rel_row_frag(K + (kk >> 2) * IMG, il, kk & 3), qf[kk], s);
     const uint32_t w = word >> (4 * hf);
     const int rel0 = j0 + 4 * hf - ip, jmax = a.causal ? -rel0 : INT_MAX;
     float mt = -INFINITY;
@@ -587,16 +606,19 @@ __device__ __forceinline__ void rel_diagonals(const f32x16& s, float (&d)[3]) {
 }
 
 // As the forward, with the query on the lane: dS^T needs lse and delta of the lane alone, and dQ^T += K^T dS^T takes it from the
-// accumulators.  dtable: rel_diagonals sums a near tile along its diagonals in registers, and each group of 16 lanes adds the sums to a
+// accumulators.  dtable: rel_diagonals sums a near tile along its diagonals in registers, and each group of lanes adds the sums to a
 // vector over the distances of its own (an address is one lane's: plain LDS reads and writes in a fixed order; LDS float atomics
 // took 175 cycles a wave instruction, which made this kernel 3.5 times slower).  Tiles beyond max_distance add to two registers.
+constexpr int rel_diag_vectors(int D) { return D == 64 ? 16 : 8; }
 template <typename T, int D, int NQ>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelArgs a) {
+__global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int CB = D / 64, STAGE = 2 * CB * 8192, QB = 128 * NQ, EXT = 64 + 32 * NQ;
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int nbias = (2 * (a.far + EXT) + 1 + 3) & ~3;
-  float* diag = bias + nbias;   // [16][nbias]: per group of 16 lanes
+  // [VECS][nbias]: per group of 16 lanes, at D = 128 per wave half (two workgroups then fit a CU's LDS)
+  constexpr int VECS = rel_diag_vectors(D);
+  float* diag = bias + nbias;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
   const int nqb = (a.Lq + QB - 1) / QB, item = rel_item(blockIdx.x, gridDim.x);
@@ -613,8 +635,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
   const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + (h / a.G) * a.v_sh;
   rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
   if (a.dtab_part)
-    for (int x = tid; x < 16 * nbias; x += 256) diag[x] = 0.f;
-  float* my_diag = diag + (tid >> 4) * nbias + 4 * hf - (lane & 31);
+    for (int x = tid; x < VECS * nbias; x += 256) diag[x] = 0.f;
+  float* my_diag = diag + (VECS == 16 ? tid >> 4 : tid >> 5) * nbias + 4 * hf - (lane & 31);
 
   s16x8 qf[NQ][D / 16], gf[NQ][D / 16];
   f32x16 dq[NQ][D / 32];
@@ -644,8 +666,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) dq[s][dt] = rel_zero();
   }
-  const ImgLane il = img_lane(lane);
-  const RelLoader<T, CB, 4> ld(a.k_sl, a.v_sl, wave, lane);
+  const RelLane il(lane);
+  const RelLoader<T, CB> ld(a.k_sl, a.v_sl, wave, lane);
   const uint32_t lds0 = lds_addr_of(smem);
   int keep = 1;
   if (nkt > 0) {
@@ -676,8 +698,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
       for (int qs = 0; qs < NQ; ++qs) s[qs] = dp[qs] = rel_zero();
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const s16x8 kf = rel_row_frag(K + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]);
-        const s16x8 vf = rel_row_frag(V + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]);
+        const s16x8 kf = rel_row_frag(K + (kk >> 2) * 8192 + t * 4096, il, kk & 3);
+        const s16x8 vf = rel_row_frag(V + (kk >> 2) * 8192 + t * 4096, il, kk & 3);
 #pragma unroll
         for (int qs = 0; qs < NQ; ++qs) {
           s[qs] = rel_mfma<T>(kf, qf[qs][kk], s[qs]);
@@ -722,10 +744,18 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
             float d[3];
             rel_diagonals(s[qs], d);
             float* at = my_diag + (a.far + EXT + jt - (i_wave + 32 * qs + off));   // (lane & 31 = 16 R + c)
+            if (VECS == 16) {
 #pragma unroll
-            for (int k = 0; k < 3; ++k) d[k] += at[16 * k];
+              for (int k = 0; k < 3; ++k) d[k] += at[16 * k];
 #pragma unroll
-            for (int k = 0; k < 3; ++k) at[16 * k] = d[k];
+              for (int k = 0; k < 3; ++k) at[16 * k] = d[k];
+            } else {   // the upper 16 lanes of a half stand where the lower ones were one k before: one after the other (LDS keeps a wave's order)
+#pragma unroll
+              for (int k = 0; k < 3; ++k) {
+                at[16 * k] += d[k];
+                asm volatile("" ::: "memory");
+              }
+            }
           }
         }
         df[qs][0] = rel_operand<T>(s[qs], 0);
@@ -747,14 +777,14 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
     if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, dq[qs], a.scale, hf);
   }
   if (!a.dtab_part) return;
-  // ---- this workgroup's sums by bucket: the far sums join their wave's vectors at its ends, the sixteen vectors are added in order, and
+  // ---- this workgroup's sums by bucket: the far sums join their wave's vectors at its ends, the vectors are added in order, and
   // a thread per (bucket, slice) collects its distances
   far_l = wave_sum(far_l);
   far_r = wave_sum(far_r);
   __syncthreads();
   if (lane == 0) {
-    diag[4 * wave * nbias] += far_l;
-    diag[4 * wave * nbias + 2 * (a.far + EXT)] += far_r;
+    diag[VECS / 4 * wave * nbias] += far_l;
+    diag[VECS / 4 * wave * nbias + 2 * (a.far + EXT)] += far_r;
   }
   __syncthreads();
   const int n = 2 * (a.far + EXT) + 1;
@@ -762,7 +792,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dq_kernel(const RelA
   for (int x = tid; x < n; x += 256) {
     float t = 0.f;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) t += diag[v * nbias + x];
+    for (int v = 0; v < VECS; ++v) t += diag[v * nbias + x];
     diag[x] = t;
     which[x] = rel_bucket(a, min(max(x - a.far - EXT, -a.far), a.far));
   }
@@ -805,16 +835,18 @@ __global__ __launch_bounds__(256) void rel_dtable_kernel(const float* part, W* d
 
 // ------------------------------------------------------------------------------------------------ backward: dK, dV
 // The key on the lane: a wave keeps K and V of its 32 keys as operands, walks the query tiles of all heads of the group, and sums dK^T
-// and dV^T of the group in its accumulators.
+// and dV^T of the group in its accumulators.  With few key blocks (few key heads) or unequal ones (causal: the first keys see all rows, the
+// last few) the walk is divided among `dkv_splits` workgroups, whose f32 sums rel_dkv_join_kernel adds in order.
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dkv_kernel(const RelArgs a) {
+__global__ __launch_bounds__(256, 2) void rel_dkv_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int CB = D / 64, STAGE = 2 * CB * 8192 + 512, KB = 128, EXT = 96;
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
-  const int nkb = (a.Lk + KB - 1) / KB, item = rel_item(blockIdx.x, gridDim.x);
-  const int bk = item / nkb, kb = item - bk * nkb, b = bk / a.Hk, hk = bk - b * a.Hk;
+  const int nkb = (a.Lk + KB - 1) / KB, item = rel_item(blockIdx.x, gridDim.x), S = a.dkv_splits;
+  const int unit = item / S, split = item - unit * S;
+  const int bk = unit / nkb, kb = unit - bk * nkb, b = bk / a.Hk, hk = bk - b * a.Hk;
   const int off = rel_offset(a, b), klen = rel_key_len(a, b);
   const int j_wg = kb * KB, j_wave = j_wg + 32 * wave, j = j_wave + r;
   const bool kept = j < klen && rel_mask_at(a, b, j);
@@ -832,22 +864,23 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dkv_kernel(const Rel
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = rel_zero();
   }
-  const bool wave_keeps = __any(kept);
-  const bool wg_keeps = __syncthreads_or(kept);
+  const bool wave_keeps = __any(kept), wave_whole = __all(kept);
+  const bool wg_keeps = __builtin_amdgcn_readfirstlane(__syncthreads_or(kept));
   // query tiles: causal rows end before i + off = j
   const int nqt = (a.Lq + 63) / 64;
   const int first = a.causal ? max(0, j_wg - off) / 64 : 0;
-  const int per = max(nqt - first, 0), total = wg_keeps ? per * a.G : 0;
-  const ImgLane il = img_lane(lane);
+  const int per = max(nqt - first, 0), all = wg_keeps ? per * a.G : 0;
+  const int begin = (int)((int64_t)all * split / S), end = (int)((int64_t)all * (split + 1) / S);
+  const RelLane il_(lane);
   const int64_t g_sl = (int64_t)a.H * D;
-  const RelLoader<T, CB, 4> ld(a.q_sl, g_sl, wave, lane);
+  const RelLoader<T, CB> ld(a.q_sl, g_sl, wave, lane);
   const uint32_t lds0 = lds_addr_of(smem);
   float rowv = 0.f;   // lanes of waves 0, 1: lse, delta of the next tile's rows
   auto issue = [&](int x) {
     const int h = hk * a.G + x / per, i0 = 64 * (first + x % per);
     const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh;
     const T* gp = reinterpret_cast<const T*>(a.dout) + ((int64_t)b * a.Lq * a.H + h) * D;
-    ld.issue(qp, gp, a.q_sl, g_sl, i0, a.Lq, lds0 + (x & 1) * STAGE, wave, lane);
+    ld.issue(qp, gp, a.q_sl, g_sl, i0, a.Lq, lds0 + ((x - begin) & 1) * STAGE, wave, lane);
     if (wave < 2) {
       const int i = i0 + lane;
       const float* src = wave ? a.delta : a.lse;
@@ -856,10 +889,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dkv_kernel(const Rel
     }
   };
   int head = -1;
-  if (total > 0) issue(0);
-  for (int x = 0; x < total; ++x) {
+  if (begin < end) issue(begin);
+  for (int x = begin; x < end; ++x) {
     const int hg = x / per, i0 = 64 * (first + x % per);
-    char* Q = smem + (x & 1) * STAGE;
+    char* Q = smem + ((x - begin) & 1) * STAGE;
     char* Gr = Q + CB * 8192;
     float* rows = reinterpret_cast<float*>(Q + 2 * CB * 8192);   // [lse 64][delta 64]
     __builtin_amdgcn_s_waitcnt(0x0F70);
@@ -870,48 +903,72 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dkv_kernel(const Rel
       head = hg;
     }
     __syncthreads();
-    if (x + 1 < total) issue(x + 1);
+    if (x + 1 < end) issue(x + 1);
     if (!wave_keeps || (a.causal && i0 + 63 + off < j_wave)) continue;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int it = i0 + 32 * t;
       if (it >= a.Lq || (a.causal && it + 31 + off < j_wave)) continue;
-      f32x16 s = rel_zero(), dp = rel_zero();
+      // phase by phase, P's product before dP is formed: with everything in flight at once D = 128 would not fit 256 registers
+      const RelLane il = il_.fresh();
+      f32x16 s = rel_zero();
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        s = rel_mfma<T>(rel_row_frag(Q + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]), kf[kk], s);
-        dp = rel_mfma<T>(rel_row_frag(Gr + (kk >> 2) * 8192 + t * 4096 + il.row[kk & 3]), vf[kk], dp);
-      }
+      for (int kk = 0; kk < D / 16; ++kk) s = rel_mfma<T>(rel_row_frag(Q + (kk >> 2) * 8192 + t * 4096, il, kk & 3), kf[kk], s);
       const int rel_hi = j_wave + 31 - (it + off), rel_lo = j_wave - (it + 31 + off);
       const bool left = rel_hi <= -a.far, right = rel_lo >= a.far;
-      const float* lr = rows + 32 * t + 4 * hf;
-      const float* bp = bias + (a.far + EXT + j - (it + off) - 4 * hf);   // minus the row (only used where the tile is near)
-      const float c = bias[left ? 0 : 2 * (a.far + EXT)];
+      const bool masked = !wave_whole || (a.causal && rel_hi > 0);
       const int imin = a.causal ? j - off - it - 4 * hf : INT_MIN;
-      f32x16 p;
+      const float* lr = rows + 32 * t + 4 * hf;
+      if (left || right) {
+        const float c = bias[left ? 0 : 2 * (a.far + EXT)];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], a.sl2, c);
+      } else {
+        const float* bp = bias + (a.far + EXT + j - (it + off) - 4 * hf);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], a.sl2, bp[-acc_row(e)]);
+      }
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const float4 ls = *reinterpret_cast<const float4*>(lr + 8 * q4);
-        const float4 de = *reinterpret_cast<const float4*>(lr + 64 + 8 * q4);
-        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv4[4] = {de.x, de.y, de.z, de.w};
+        const float lv[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 4 * q4 + e;
-          const float bias2 = left || right ? c : bp[-(8 * q4 + e)];
-          const float pv = att_exp2(fmaf(s[k], a.sl2, bias2) - lv[e]);
-          const bool ok = kept && 8 * q4 + e >= imin;
-          p[k] = ok ? pv : 0.f;
-          s[k] = ok ? pv * (dp[k] - dv4[e]) : 0.f;
-        }
+        for (int e = 0; e < 4; ++e) s[4 * q4 + e] = att_exp2(s[4 * q4 + e] - lv[e]);
       }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = kept && acc_row(e) >= imin ? s[e] : 0.f;
+      }
+      if (D == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        const s16x8 pf = rel_operand<T>(p, st), df = rel_operand<T>(s, st);
+        const s16x8 pf = rel_operand<T>(s, st);
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) {
+        for (int dt = 0; dt < D / 32; ++dt)
           dv[dt] = rel_mfma<T>(rel_tr_frag(Gr + (dt >> 1) * 8192, il, t * 4096 + st * 2048, dt & 1), pf, dv[dt]);
+      }
+      if (D == 128) __builtin_amdgcn_sched_barrier(0);
+      f32x16 dp = rel_zero();
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) dp = rel_mfma<T>(rel_row_frag(Gr + (kk >> 2) * 8192 + t * 4096, il, kk & 3), vf[kk], dp);
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 de = *reinterpret_cast<const float4*>(lr + 64 + 8 * q4);
+        const float dl[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = s[4 * q4 + e] * (dp[4 * q4 + e] - dl[e]);
+      }
+      if (masked) {   // (what a masked value holds reached dP)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] = kept && acc_row(e) >= imin ? dp[e] : 0.f;
+      }
+      if (D == 128) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const s16x8 df = rel_operand<T>(dp, st);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
           dk[dt] = rel_mfma<T>(rel_tr_frag(Q + (dt >> 1) * 8192, il, t * 4096 + st * 2048, dt & 1), df, dk[dt]);
-        }
       }
     }
   }
@@ -921,9 +978,30 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void rel_dkv_kernel(const Rel
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = rel_zero();
     }
-    rel_store_row<T, D>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, hf);
-    rel_store_row<T, D>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, hf);
+    if (S == 1) {
+      rel_store_row<T, D>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, hf);
+      rel_store_row<T, D>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, hf);
+    } else {
+      const int64_t n = (int64_t)a.B * a.Lk * a.Hk * D;
+      rel_store_row<float, D>(a.dkv_part + 2 * split * n + at, dk, 1.f, hf);
+      rel_store_row<float, D>(a.dkv_part + (2 * split + 1) * n + at, dv, 1.f, hf);
+    }
   }
+}
+
+// dK, dV of the splits' sums, in order; four values a thread
+template <typename T>
+__global__ __launch_bounds__(256) void rel_dkv_join_kernel(const RelArgs a, int64_t n) {
+  const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (x >= n) return;
+  float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+  for (int s = 0; s < a.dkv_splits; ++s) {
+    const float4 ks = *reinterpret_cast<const float4*>(a.dkv_part + 2 * s * n + x), vs = *reinterpret_cast<const float4*>(a.dkv_part + (2 * s + 1) * n + x);
+    k.x += ks.x; k.y += ks.y; k.z += ks.z; k.w += ks.w;
+    v.x += vs.x; v.y += vs.y; v.z += vs.z; v.w += vs.w;
+  }
+  Vec4<T>::store(reinterpret_cast<T*>(a.dk) + x, make_float4(k.x * a.scale, k.y * a.scale, k.z * a.scale, k.w * a.scale));
+  Vec4<T>::store(reinterpret_cast<T*>(a.dv) + x, v);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -945,6 +1023,17 @@ static int rel_splits(const mmk_rel_attn* p) {
   const int64_t want = (512 + groups - 1) / groups, most = std::max<int64_t>(1, ((int64_t)p->Lk + 255) / 256);
   return (int)std::min<int64_t>(std::min(want, most), 64);
 }
+// Workgroups that share one key block's walk: two a CU are wanted, four where causal leaves them unequal, each with 8 query tiles at least
+static int rel_dkv_splits(const mmk_rel_attn* p) {
+  const int64_t blocks = std::max<int64_t>(1, (int64_t)p->B * p->Hk * ((p->Lk + 127) / 128)), want = p->causal ? 1024 : 512;
+  const int64_t tiles = (int64_t)(p->H / p->Hk) * ((p->Lq + 63) / 64);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(want + blocks - 1) / blocks, tiles / 8, 16}));
+}
+static int64_t rel_dkv_floats(const mmk_rel_attn* p) {
+  const int s = rel_dkv_splits(p);
+  return s == 1 ? 0 : 2 * (int64_t)s * p->B * p->Lk * p->Hk * p->D;
+}
+
 static int rel_check(const mmk_rel_attn* p) {
   MMK_REQUIRE(p != nullptr, "no geometry");
   MMK_REQUIRE(p->dtype == MMK_BF16 || p->dtype == MMK_F16, "operands are bf16 or f16");
@@ -952,7 +1041,7 @@ static int rel_check(const mmk_rel_attn* p) {
   MMK_REQUIRE(p->D == 64 || p->D == 128, "head dim must be 64 or 128");
   MMK_REQUIRE(p->B >= 0 && p->H >= 1 && p->Hk >= 1 && p->H % p->Hk == 0 && p->Lq >= 0 && p->Lk >= 0, "bad sizes");
   MMK_REQUIRE(p->Lq <= (1 << 28) && p->Lk <= (1 << 28), "sequence too long");
-  MMK_REQUIRE((int64_t)p->B * p->H * (((int64_t)std::max(p->Lq, p->Lk) + 127) / 128) < (1 << 30), "too many workgroups");
+  MMK_REQUIRE((int64_t)p->B * p->H * (((int64_t)std::max(p->Lq, p->Lk) + 127) / 128) < (1 << 26), "too many workgroups");
   MMK_REQUIRE(p->buckets >= 1 && p->buckets <= REL_MAX_BUCKETS && p->n_borders >= 0 && p->n_borders <= REL_MAX_BORDERS, "too many buckets");
   MMK_REQUIRE(p->near_buckets >= 1 && p->max_distance >= 1 && p->max_distance <= REL_MAX_FAR, "max_distance must be 1 .. 512");
   MMK_REQUIRE((p->bidirectional ? 2 : 1) * (p->near_buckets + p->n_borders + 1) == p->buckets, "near and logarithmic buckets do not add up");
@@ -1051,8 +1140,8 @@ static int rel_backward(const mmk_rel_attn* p, RelArgs& a, void* dtable, hipStre
   if (a.Lq > 0) {
     auto go = [&](auto nq) {
       constexpr int NQ = decltype(nq)::value, EXT = 64 + 32 * NQ;
-      const int lds = TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 17 : 1);
-      return rel_launch(rel_dq_kernel<T, D, NQ>, MMK_K_REL_ATTN_BWD, (int64_t)a.B * a.H * nqb, lds, TILES + 17 * rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
+      const int lds = TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 1 + rel_diag_vectors(D) : 1);
+      return rel_launch(rel_dq_kernel<T, D, NQ>, MMK_K_REL_ATTN_BWD, (int64_t)a.B * a.H * nqb, lds, TILES + (1 + rel_diag_vectors(D)) * rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
     };
     int rc;
     if constexpr (D == 64) rc = rel_nq(p) == 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
@@ -1060,10 +1149,15 @@ static int rel_backward(const mmk_rel_attn* p, RelArgs& a, void* dtable, hipStre
     if (rc) return rc;
   }
   if (a.Lk > 0) {
-    const int64_t grid = (int64_t)a.B * a.Hk * ((a.Lk + 127) / 128);
+    const int64_t grid = (int64_t)a.B * a.Hk * ((a.Lk + 127) / 128) * a.dkv_splits;
     if (int rc = rel_launch(rel_dkv_kernel<T, D>, MMK_K_REL_ATTN_BWD, grid, TILES + 1024 + rel_vec_bytes(a.far, 96),
                             TILES + 1024 + rel_vec_bytes(REL_MAX_FAR, 96), a, st))
       return rc;
+    if (a.dkv_splits > 1) {
+      const int64_t n = (int64_t)a.B * a.Lk * a.Hk * D;
+      hipLaunchKernelGGL(rel_dkv_join_kernel<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, a, n);
+      MMK_LAUNCH_CHECK();
+    }
   }
   if (a.dtab_part) {
     const int n = a.Lq > 0 ? nqb : 0;
@@ -1109,7 +1203,7 @@ int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, float* lse, float* ws, vo
 
 int64_t mmk_rel_attn_bwd_ws_floats(const mmk_rel_attn* p, int want_dtable) {
   if (rel_check(p)) return -1;
-  return (int64_t)p->B * p->H * p->Lq + (want_dtable ? (int64_t)p->B * p->H * rel_dq_blocks(p) * p->buckets : 0);
+  return rel_dkv_floats(p) + (int64_t)p->B * p->H * p->Lq + (want_dtable ? (int64_t)p->B * p->H * rel_dq_blocks(p) * p->buckets : 0);
 }
 
 int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dtable,
@@ -1128,8 +1222,10 @@ int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const float* lse, c
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
-  a.delta = ws;
-  a.dtab_part = dtable ? ws + (int64_t)p->B * p->H * p->Lq : nullptr;
+  a.dkv_part = ws;   // (first: its rows are read four floats at a time)
+  a.dkv_splits = rel_dkv_splits(p);
+  a.delta = ws + rel_dkv_floats(p);
+  a.dtab_part = dtable ? a.delta + (int64_t)p->B * p->H * p->Lq : nullptr;
   return rel_dispatch(p, [&](auto t, auto d) { return rel_backward<decltype(t), decltype(d)::value>(p, a, dtable, (hipStream_t)stream); });
 }
 
