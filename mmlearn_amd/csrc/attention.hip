@@ -318,11 +318,6 @@ __device__ __forceinline__ void attn_load_q(const AttnArgs& a, int bh, int t, in
   for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(qrow + 16 * kk);
 }
 
-// s_waitcnt vmcnt(0) as the BUILTIN (expcnt / lgkmcnt fields left at their maxima): unlike an asm statement the
-// compiler's wait-count bookkeeping sees it, so it knows every earlier load has landed and inserts no vmcnt of its own
-// in the compute phase -- vmcnt is in-order, and any such wait would also wait for the prefetch issued after it.
-__device__ __forceinline__ void wait_vmem_all() { __builtin_amdgcn_s_waitcnt(0x0F70); }
-
 // Persistent workgroups: NT <= NW, wave w owns query tile w of every (batch, head) item the workgroup walks.  The K / V
 // images are double-buffered: the LDS-DMA of item n+1 and its Q fragments are in flight while item n is computed, so
 // the HBM stream never stops behind a compute phase (one barrier per item).

@@ -40,6 +40,11 @@ __device__ __forceinline__ uint32_t lds_addr_of(const char* p) {
   return (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) char*)p);
 }
 
+// s_waitcnt vmcnt(0) as the BUILTIN (expcnt / lgkmcnt fields left at their maxima): unlike an asm statement the
+// compiler's wait-count bookkeeping sees it, so it knows every earlier load has landed and inserts no vmcnt of its own
+// in the compute phase -- vmcnt is in-order, and any such wait would also wait for the prefetch issued after it.
+__device__ __forceinline__ void wait_vmem_all() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // MFMA operands out of an image.  k along the 64 COLUMNS: lane (r, h) takes row `row`, elements 16kk + 8h .. +7, one
 // ds_read_b128 at  row * 128 + (((2 kk + h) ^ img_swz(row)) << 4).  k along the ROWS (transposed use of the same image):
 // for the 32x32x16 A operand X^T[c][k] with c = 32 ct + (lane & 31) and the accumulator-as-operand k order, the lane

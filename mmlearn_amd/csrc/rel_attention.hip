@@ -167,6 +167,12 @@ __device__ __forceinline__ int rel_item(int id, int total) {
   const int per = total >> 3;
   return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
 }
+// which head the items of place `p` belong to: the heads of one sample are dealt to the eight XCDs in turn, because samples of unequal length
+// would otherwise load them unequally (16 x 12 x 512 x 64 with lengths from a third up: dK/dV 60 us by whole samples, 58 dealt)
+__device__ __forceinline__ int rel_head(int p, int n) {
+  const int per = n >> 3;
+  return p < per * 8 ? (p % per) * 8 + p / per : p;
+}
 
 // One wave's share of a 64-row tile in LDS: CB column blocks of 64 of X, then of Y; of each image's 8 pieces of 8 rows, pieces `wave` and
 // `wave` + 4 (32 rows further, where the swizzle is the same: one per-lane offset serves both)
@@ -181,22 +187,22 @@ struct RelLoader {
   // rows row0 .. row0 + 63 of X and Y (rows past `rows - 1` repeat that row), to the stage at `lds`
   __device__ __forceinline__ void issue(const T* x, const T* y, int64_t x_sl, int64_t y_sl, int row0, int rows, uint32_t lds, int wave,
                                         int lane) const {
-    const bool whole = row0 + 64 <= rows;
+    auto each = [&](auto voff) {
 #pragma unroll
-    for (int im = 0; im < 2 * CB; ++im) {
-      const int64_t sl = im < CB ? x_sl : y_sl;
-      const T* base = (im < CB ? x : y) + (int64_t)row0 * sl + 64 * (im % CB);
+      for (int im = 0; im < 2 * CB; ++im) {
+        const int64_t sl = im < CB ? x_sl : y_sl;
+        const T* base = (im < CB ? x : y) + (int64_t)row0 * sl + 64 * (im % CB);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t at = lds + (uint32_t)(im * 8192 + (wave + 4 * u) * 1024);
-        if (whole) {
-          lds_dma16(base + 32 * u * sl, im < CB ? vx : vy, at);
-        } else {
-          const int row = 8 * (wave + 4 * u) + (lane >> 3), ch = (lane & 7) ^ img_swz(row & 15);
-          lds_dma16(base, (uint32_t)(min(row, rows - 1 - row0) * (int)sl + ch * 8) * 2u, at);
-        }
+        for (int u = 0; u < 2; ++u) voff(base, sl, im < CB, u, lds + (uint32_t)(im * 8192 + (wave + 4 * u) * 1024));
       }
-    }
+    };
+    if (row0 + 64 <= rows)
+      each([&](const T* base, int64_t sl, bool is_x, int u, uint32_t at) { lds_dma16(base + 32 * u * sl, is_x ? vx : vy, at); });
+    else
+      each([&](const T* base, int64_t sl, bool, int u, uint32_t at) {
+        const int row = 8 * (wave + 4 * u) + (lane >> 3), ch = (lane & 7) ^ img_swz(row & 15);
+        lds_dma16(base, (uint32_t)(min(row, rows - 1 - row0) * (int)sl + ch * 8) * 2u, at);
+      });
   }
 };
 
@@ -231,43 +237,28 @@ __device__ __forceinline__ void rel_store_row(T* row, const f32x16 (&o)[D / 32],
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// Workgroup: 4 waves x NQ x 32 queries of one (sample, head); tiles of 64 keys.
-template <typename T, int D, int NQ>
+// Workgroup: 4 waves x 32 queries of one (sample, head); tiles of 64 keys.  (64 queries a wave would halve the LDS reads, but the vector
+// unit -- exponential, bias, maximum, sum: twice the cycles of the products at D = 64 -- bounds it and finer workgroups fill the chip better:
+// 4 x 12 x 512 x 64 20 us with 32 and 23 with 64, 2 x 12 x 8192 x 64 503 and 498.)
+template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, QB = 128 * NQ, EXT = 64 + 32 * NQ;
+  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, EXT = 96;
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
-  const int nqb = (a.Lq + QB - 1) / QB, item = rel_item(blockIdx.x, gridDim.x);
-  const int bh = item / nqb, b = bh / a.H, h = bh - b * a.H;
-  const int qb = a.causal ? nqb - 1 - (item - bh * nqb) : item - bh * nqb;   // causal: the longest rows first
+  const int nqb = (a.Lq + 127) / 128, item = rel_item(blockIdx.x, gridDim.x);
+  const int place = item / nqb, bh = rel_head(place, a.B * a.H), b = bh / a.H, h = bh - b * a.H;
+  const int qb = a.causal ? nqb - 1 - (item - place * nqb) : item - place * nqb;   // causal: the longest rows first
   const int off = rel_offset(a, b), klen = rel_key_len(a, b);
-  const int i_wg = qb * QB, i_wave = i_wg + 32 * NQ * wave;
+  const int i_wg = qb * 128, i_wave = i_wg + 32 * wave, i = i_wave + r;
   int nkt = (klen + 63) / 64;
   if (a.causal) {
-    const int last = min(klen - 1, min(i_wg + QB, a.Lq) - 1 + off);
+    const int last = min(klen - 1, min(i_wg + 128, a.Lq) - 1 + off);
     nkt = last < 0 ? 0 : last / 64 + 1;
   }
   const T* kp = reinterpret_cast<const T*>(a.k) + b * a.k_sb + (h / a.G) * a.k_sh;
   const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + (h / a.G) * a.v_sh;
-  rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
-
-  s16x8 qf[NQ][D / 16];
-  f32x16 o[NQ][D / 32];
-  float m[NQ], l[NQ];
-#pragma unroll
-  for (int s = 0; s < NQ; ++s) {
-    const int i = min(i_wave + 32 * s + r, a.Lq - 1);
-    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + i * a.q_sl + 8 * hf;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) qf[s][kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) o[s][dt] = rel_zero();
-    m[s] = -INFINITY;
-    l[s] = 0.f;
-  }
-  const RelLane il(lane);
   const RelLoader<T, CB> ld(a.k_sl, a.v_sl, wave, lane);
   const uint32_t lds0 = lds_addr_of(smem);
   int keep = 1;
@@ -275,110 +266,104 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
     ld.issue(kp, vp, a.k_sl, a.v_sl, 0, a.Lk, lds0, wave, lane);
     keep = rel_mask_at(a, b, lane);
   }
+
+  s16x8 qf[D / 16];
+  f32x16 o[D / 32];
+  float m = -INFINITY, l = 0.f;
+  {
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + min(i, a.Lq - 1) * a.q_sl + 8 * hf;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) qf[kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_zero();
+  }
+  rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
+  const RelLane il(lane);
+  const int ip = i + off;   // this lane's query position
   for (int kt = 0; kt < nkt; ++kt) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this tile and its mask are here
-    __syncthreads();
+    wait_vmem_all();   // this tile and its mask are here
+    __syncthreads();   // and nobody reads the one before it any more
     const int j0 = 64 * kt;
     const uint64_t word = __ballot(j0 + lane < klen && keep);
     if (kt + 1 < nkt) {
       ld.issue(kp, vp, a.k_sl, a.v_sl, j0 + 64, a.Lk, lds0 + ((kt + 1) & 1) * STAGE, wave, lane);
       keep = rel_mask_at(a, b, j0 + 64 + lane);
     }
-    if (word == 0) continue;
     char* K = smem + (kt & 1) * STAGE;
     char* V = K + CB * 8192;
+    if (word == 0) continue;
     if (~word) {
       rel_zero_rows<CB>(V, word, wave, lane);
       __syncthreads();
     }
-    if (i_wave >= a.Lq || (a.causal && j0 > i_wave + 32 * NQ - 1 + off)) continue;   // no row, or no key of the tile, for this wave
-    f32x16 s[NQ][2];
-#pragma unroll
-    for (int qs = 0; qs < NQ; ++qs) s[qs][0] = s[qs][1] = rel_zero();
+    if (i_wave >= a.Lq || (a.causal && j0 > i_wave + 31 + off)) continue;   // no row, or no key of the tile, for this wave
+    f32x16 s[2];
+    s[0] = s[1] = rel_zero();
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const s16x8 kf = rel_row_frag(K + (kk >> 2) * 8192 + t * 4096, il, kk & 3);
-#pragma unroll
-        for (int qs = 0; qs < NQ; ++qs) s[qs][t] = rel_mfma<T>(kf, qf[qs][kk], s[qs][t]);
-      }
-    const int rel_hi = j0 + 63 - (i_wave + off), rel_lo = j0 - (i_wave + 32 * NQ - 1 + off);
-    const bool masked = ~word || (a.causal && rel_hi > 0);
-    s16x8 pf[NQ][4];
-#pragma unroll
-    for (int qs = 0; qs < NQ; ++qs) {
-      const int ip = i_wave + 32 * qs + r + off;   // this lane's query position
-      if (rel_hi <= -a.far || rel_lo >= a.far) {
-        const float c = bias[rel_hi <= -a.far ? 0 : 2 * (a.far + EXT)];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[qs][t][e] = fmaf(s[qs][t][e], a.sl2, c);
-      } else {
-        const float* bp = bias + (a.far + EXT + j0 + 4 * hf - ip);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[qs][t][e] = fmaf(s[qs][t][e], a.sl2, bp[32 * t + acc_row(e)]);
-      }
-      if (masked) {
-        const int jmax = a.causal ? ip - j0 - 4 * hf : INT_MAX;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t w = (uint32_t)(word >> (32 * t)) >> (4 * hf);
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (!((w >> acc_row(e)) & 1) || 32 * t + acc_row(e) > jmax) s[qs][t][e] = -INFINITY;
-        }
-      }
-      float mt = s[qs][0][0];
+      for (int t = 0; t < 2; ++t) s[t] = rel_mfma<T>(rel_row_frag(K + (kk >> 2) * 8192 + t * 4096, il, kk & 3), qf[kk], s[t]);
+    const int rel_hi = j0 + 63 - (i_wave + off), rel_lo = j0 - (i_wave + 31 + off);
+    if (rel_hi <= -a.far || rel_lo >= a.far) {
+      const float c = bias[rel_hi <= -a.far ? 0 : 2 * (a.far + EXT)];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[qs][t][e]);
-      mt = fmaxf(mt, rel_other_half(mt));
-      // the running maximum moves only when it grows by more than 2^8: until then the sums stay exact enough in f32 and the
-      // rescale of O is skipped for the whole wave
-      if (__any(mt > m[qs] + 8.f)) {
-        const float mn = fmaxf(m[qs], mt);
-        const float alpha = mn == m[qs] ? 1.f : att_exp2(m[qs] - mn);
-        m[qs] = mn;
-        l[qs] *= alpha;
+        for (int e = 0; e < 16; ++e) s[t][e] = fmaf(s[t][e], a.sl2, c);
+    } else {
+      const float* bp = bias + (a.far + EXT + j0 + 4 * hf - ip);
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[qs][dt][e] *= alpha;
-      }
-      const float nm = m[qs] == -INFINITY ? 0.f : -m[qs];
+        for (int e = 0; e < 16; ++e) s[t][e] = fmaf(s[t][e], a.sl2, bp[32 * t + acc_row(e)]);
+    }
+    if (~word || (a.causal && rel_hi > 0)) {
+      const int jmax = a.causal ? ip - j0 - 4 * hf : INT_MAX;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
+        const uint32_t w = (uint32_t)(word >> (32 * t)) >> (4 * hf);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[qs][t][e] = att_exp2(s[qs][t][e] + nm);
-          l[qs] += s[qs][t][e];
-        }
-        pf[qs][2 * t] = rel_operand<T>(s[qs][t], 0);
-        pf[qs][2 * t + 1] = rel_operand<T>(s[qs][t], 1);
+        for (int e = 0; e < 16; ++e)
+          if (!((w >> acc_row(e)) & 1) || 32 * t + acc_row(e) > jmax) s[t][e] = -INFINITY;
       }
     }
+    float mt = s[0][0];
 #pragma unroll
-    for (int st = 0; st < 4; ++st)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        const s16x8 vf = rel_tr_frag(V + (dt >> 1) * 8192, il, st * 2048, dt & 1);
+      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t][e]);
+    mt = fmaxf(mt, rel_other_half(mt));
+    // the running maximum moves only when it grows by more than 2^8: until then the sums stay exact enough in f32 and the
+    // rescale of O is skipped for the whole wave
+    if (__any(mt > m + 8.f)) {
+      const float mn = fmaxf(m, mt);
+      const float alpha = mn == m ? 1.f : att_exp2(m - mn);
+      m = mn;
+      l *= alpha;
 #pragma unroll
-        for (int qs = 0; qs < NQ; ++qs) o[qs][dt] = rel_mfma<T>(vf, pf[qs][st], o[qs][dt]);
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+    }
+    const float nm = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[t][e] = att_exp2(s[t][e] + nm);
+        l += s[t][e];
       }
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      const s16x8 pf = rel_operand<T>(s[st >> 1], st & 1);
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_mfma<T>(rel_tr_frag(V + (dt >> 1) * 8192, il, st * 2048, dt & 1), pf, o[dt]);
+    }
   }
-#pragma unroll
-  for (int qs = 0; qs < NQ; ++qs) {
-    const int i = i_wave + 32 * qs + r;
-    const float sum = l[qs] + rel_other_half(l[qs]);
-    if (i < a.Lq) {
-      rel_store_row<T, D>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + h) * D, o[qs], sum > 0.f ? 1.f / sum : sum, hf);
-      if (a.lse && hf == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : m[qs] + log2f(sum);
-    }
+  const float sum = l + rel_other_half(l);
+  if (i < a.Lq) {
+    rel_store_row<T, D>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + h) * D, o, sum > 0.f ? 1.f / sum : sum, hf);
+    if (a.lse && hf == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : m + log2f(sum);
   }
 }
 
@@ -442,7 +427,7 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
   }
   int stage = 0;
   for (int t = t0; t < t1; t += 4, stage ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);
+    wait_vmem_all();
     asm volatile("" ::: "memory");
     const int j0 = 32 * t;
     const uint32_t word = (uint32_t)__ballot(j0 + r < klen && keep);
@@ -610,63 +595,27 @@ __device__ __forceinline__ void rel_diagonals(const f32x16& s, float (&d)[3]) {
 // vector over the distances of its own (an address is one lane's: plain LDS reads and writes in a fixed order; LDS float atomics
 // took 175 cycles a wave instruction, which made this kernel 3.5 times slower).  Tiles beyond max_distance add to two registers.
 constexpr int rel_diag_vectors(int D) { return D == 64 ? 16 : 8; }
-template <typename T, int D, int NQ>
+template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, QB = 128 * NQ, EXT = 64 + 32 * NQ;
+  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, EXT = 96, VECS = rel_diag_vectors(D);
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int nbias = (2 * (a.far + EXT) + 1 + 3) & ~3;
-  // [VECS][nbias]: per group of 16 lanes, at D = 128 per wave half (two workgroups then fit a CU's LDS)
-  constexpr int VECS = rel_diag_vectors(D);
-  float* diag = bias + nbias;
+  float* diag = bias + nbias;   // [VECS][nbias]: per group of 16 lanes, at D = 128 per wave half (two workgroups then fit a CU's LDS)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
-  const int nqb = (a.Lq + QB - 1) / QB, item = rel_item(blockIdx.x, gridDim.x);
-  const int bh = item / nqb, b = bh / a.H, h = bh - b * a.H;
-  const int qb = a.causal ? nqb - 1 - (item - bh * nqb) : item - bh * nqb;
+  const int nqb = (a.Lq + 127) / 128, item = rel_item(blockIdx.x, gridDim.x);
+  const int place = item / nqb, bh = rel_head(place, a.B * a.H), b = bh / a.H, h = bh - b * a.H;
+  const int qb = a.causal ? nqb - 1 - (item - place * nqb) : item - place * nqb;
   const int off = rel_offset(a, b), klen = rel_key_len(a, b);
-  const int i_wg = qb * QB, i_wave = i_wg + 32 * NQ * wave;
+  const int i_wg = qb * 128, i_wave = i_wg + 32 * wave, i = i_wave + r;
   int nkt = (klen + 63) / 64;
   if (a.causal) {
-    const int last = min(klen - 1, min(i_wg + QB, a.Lq) - 1 + off);
+    const int last = min(klen - 1, min(i_wg + 128, a.Lq) - 1 + off);
     nkt = last < 0 ? 0 : last / 64 + 1;
   }
   const T* kp = reinterpret_cast<const T*>(a.k) + b * a.k_sb + (h / a.G) * a.k_sh;
   const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + (h / a.G) * a.v_sh;
-  rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
-  if (a.dtab_part)
-    for (int x = tid; x < VECS * nbias; x += 256) diag[x] = 0.f;
-  float* my_diag = diag + (VECS == 16 ? tid >> 4 : tid >> 5) * nbias + 4 * hf - (lane & 31);
-
-  s16x8 qf[NQ][D / 16], gf[NQ][D / 16];
-  f32x16 dq[NQ][D / 32];
-  float lse[NQ], delta[NQ], far_l = 0.f, far_r = 0.f;
-#pragma unroll
-  for (int s = 0; s < NQ; ++s) {
-    const int i = i_wave + 32 * s + r, ic = min(i, a.Lq - 1);
-    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + ic * a.q_sl + 8 * hf;
-    const int64_t orow = (((int64_t)b * a.Lq + ic) * a.H + h) * D + 8 * hf;
-    const T* gp = reinterpret_cast<const T*>(a.dout) + orow;
-    const T* op = reinterpret_cast<const T*>(a.o) + orow;
-    float dl = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      typedef T t8 __attribute__((ext_vector_type(8)));
-      qf[s][kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
-      gf[s][kk] = *reinterpret_cast<const s16x8*>(gp + 16 * kk);
-      const t8 g8 = __builtin_bit_cast(t8, gf[s][kk]), o8 = *reinterpret_cast<const t8*>(op + 16 * kk);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dl = fmaf(to_f32(g8[e]), to_f32(o8[e]), dl);
-    }
-    dl += rel_other_half(dl);
-    const int64_t at = ((int64_t)b * a.H + h) * a.Lq + ic;
-    lse[s] = i < a.Lq ? a.lse[at] : INFINITY;
-    delta[s] = dl;
-    if (i < a.Lq && hf == 0) a.delta[at] = dl;
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) dq[s][dt] = rel_zero();
-  }
-  const RelLane il(lane);
   const RelLoader<T, CB> ld(a.k_sl, a.v_sl, wave, lane);
   const uint32_t lds0 = lds_addr_of(smem);
   int keep = 1;
@@ -674,108 +623,119 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelArgs a) {
     ld.issue(kp, vp, a.k_sl, a.v_sl, 0, a.Lk, lds0, wave, lane);
     keep = rel_mask_at(a, b, lane);
   }
+
+  s16x8 qf[D / 16], gf[D / 16];
+  f32x16 dq[D / 32];
+  float lse, delta = 0.f, far_l = 0.f, far_r = 0.f;
+  {
+    const int ic = min(i, a.Lq - 1);
+    const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + ic * a.q_sl + 8 * hf;
+    const int64_t orow = (((int64_t)b * a.Lq + ic) * a.H + h) * D + 8 * hf;
+    const T* gp = reinterpret_cast<const T*>(a.dout) + orow;
+    const T* op = reinterpret_cast<const T*>(a.o) + orow;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      qf[kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
+      gf[kk] = *reinterpret_cast<const s16x8*>(gp + 16 * kk);
+      const t8 g8 = __builtin_bit_cast(t8, gf[kk]), o8 = *reinterpret_cast<const t8*>(op + 16 * kk);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf(to_f32(g8[e]), to_f32(o8[e]), delta);
+    }
+    delta += rel_other_half(delta);
+    const int64_t at = ((int64_t)b * a.H + h) * a.Lq + ic;
+    lse = i < a.Lq ? a.lse[at] : INFINITY;
+    if (i < a.Lq && hf == 0) a.delta[at] = delta;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) dq[dt] = rel_zero();
+  }
+  rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
+  if (a.dtab_part)
+    for (int x = tid; x < VECS * nbias; x += 256) diag[x] = 0.f;
+  float* my_diag = diag + (VECS == 16 ? tid >> 4 : tid >> 5) * nbias + 4 * hf - r;
+  const RelLane il(lane);
+  const int ip = i + off;
   for (int kt = 0; kt < nkt; ++kt) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
+    wait_vmem_all();   // this tile and its mask are here
+    __syncthreads();   // and nobody reads the one before it any more
     const int j0 = 64 * kt;
     const uint64_t word = __ballot(j0 + lane < klen && keep);
     if (kt + 1 < nkt) {
       ld.issue(kp, vp, a.k_sl, a.v_sl, j0 + 64, a.Lk, lds0 + ((kt + 1) & 1) * STAGE, wave, lane);
       keep = rel_mask_at(a, b, j0 + 64 + lane);
     }
-    if (word == 0) continue;
     char* K = smem + (kt & 1) * STAGE;
     char* V = K + CB * 8192;
+    if (word == 0) continue;
     if (~word) {
       rel_zero_rows<CB>(K, word, wave, lane);
       __syncthreads();
     }
-    if (i_wave >= a.Lq || (a.causal && j0 > i_wave + 32 * NQ - 1 + off)) continue;
+    if (i_wave >= a.Lq || (a.causal && j0 > i_wave + 31 + off)) continue;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      f32x16 s[NQ], dp[NQ];
-#pragma unroll
-      for (int qs = 0; qs < NQ; ++qs) s[qs] = dp[qs] = rel_zero();
+      f32x16 s = rel_zero(), dp = rel_zero();
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const s16x8 kf = rel_row_frag(K + (kk >> 2) * 8192 + t * 4096, il, kk & 3);
-        const s16x8 vf = rel_row_frag(V + (kk >> 2) * 8192 + t * 4096, il, kk & 3);
-#pragma unroll
-        for (int qs = 0; qs < NQ; ++qs) {
-          s[qs] = rel_mfma<T>(kf, qf[qs][kk], s[qs]);
-          dp[qs] = rel_mfma<T>(vf, gf[qs][kk], dp[qs]);
-        }
+        s = rel_mfma<T>(rel_row_frag(K + (kk >> 2) * 8192 + t * 4096, il, kk & 3), qf[kk], s);
+        dp = rel_mfma<T>(rel_row_frag(V + (kk >> 2) * 8192 + t * 4096, il, kk & 3), gf[kk], dp);
       }
       const int jt = j0 + 32 * t;
-      const int rel_hi = jt + 31 - (i_wave + off), rel_lo = jt - (i_wave + 32 * NQ - 1 + off);
+      const int rel_hi = jt + 31 - (i_wave + off), rel_lo = jt - (i_wave + 31 + off);
       const bool left = rel_hi <= -a.far, right = rel_lo >= a.far;
       const uint32_t wt = (uint32_t)(word >> (32 * t));
-      const bool masked = ~wt || (a.causal && rel_hi > 0);
-      const uint32_t w = wt >> (4 * hf);
-      s16x8 df[NQ][2];
+      if (left || right) {
+        const float c = bias[left ? 0 : 2 * (a.far + EXT)] - lse;
 #pragma unroll
-      for (int qs = 0; qs < NQ; ++qs) {
-        const int ip = i_wave + 32 * qs + r + off;
-        const int at0 = a.far + EXT + jt + 4 * hf - ip;   // (only used where the tile is near: within the vector)
+        for (int e = 0; e < 16; ++e) s[e] = att_exp2(fmaf(s[e], a.sl2, c));
+      } else {
+        const float* bp = bias + (a.far + EXT + jt + 4 * hf - ip);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = att_exp2(fmaf(s[e], a.sl2, bp[acc_row(e)]) - lse);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] *= dp[e] - delta;
+      if (~wt || (a.causal && rel_hi > 0)) {
+        const int jmax = a.causal ? ip - jt - 4 * hf : INT_MAX;
+        const uint32_t w = wt >> (4 * hf);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((w >> acc_row(e)) & 1) || acc_row(e) > jmax) s[e] = 0.f;
+      }
+      if (a.dtab_part) {
         if (left || right) {
-          const float c = bias[left ? 0 : 2 * (a.far + EXT)] - lse[qs];
+          float t4 = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[qs][e] = att_exp2(fmaf(s[qs][e], a.sl2, c));
+          for (int e = 0; e < 16; ++e) t4 += s[e];
+          far_l += left ? t4 : 0.f;
+          far_r += left ? 0.f : t4;
         } else {
+          float d[3];
+          rel_diagonals(s, d);
+          float* at = my_diag + (a.far + EXT + jt - (i_wave + off));   // (r = 16 R + c)
+          if (VECS == 16) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[qs][e] = att_exp2(fmaf(s[qs][e], a.sl2, bias[at0 + acc_row(e)]) - lse[qs]);
-        }
+            for (int k = 0; k < 3; ++k) d[k] += at[16 * k];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[qs][e] *= dp[qs][e] - delta[qs];
-        if (masked) {
-          const int jmax = a.causal ? ip - jt - 4 * hf : INT_MAX;
+            for (int k = 0; k < 3; ++k) at[16 * k] = d[k];
+          } else {   // the upper 16 lanes of a half stand where the lower ones were one k before: one after the other (LDS keeps a wave's order)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (!((w >> acc_row(e)) & 1) || acc_row(e) > jmax) s[qs][e] = 0.f;
-        }
-        if (a.dtab_part) {
-          if (left || right) {
-            float t4 = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) t4 += s[qs][e];
-            far_l += left ? t4 : 0.f;
-            far_r += left ? 0.f : t4;
-          } else {
-            float d[3];
-            rel_diagonals(s[qs], d);
-            float* at = my_diag + (a.far + EXT + jt - (i_wave + 32 * qs + off));   // (lane & 31 = 16 R + c)
-            if (VECS == 16) {
-#pragma unroll
-              for (int k = 0; k < 3; ++k) d[k] += at[16 * k];
-#pragma unroll
-              for (int k = 0; k < 3; ++k) at[16 * k] = d[k];
-            } else {   // the upper 16 lanes of a half stand where the lower ones were one k before: one after the other (LDS keeps a wave's order)
-#pragma unroll
-              for (int k = 0; k < 3; ++k) {
-                at[16 * k] += d[k];
-                asm volatile("" ::: "memory");
-              }
+            for (int k = 0; k < 3; ++k) {
+              at[16 * k] += d[k];
+              asm volatile("" ::: "memory");
             }
           }
         }
-        df[qs][0] = rel_operand<T>(s[qs], 0);
-        df[qs][1] = rel_operand<T>(s[qs], 1);
       }
 #pragma unroll
-      for (int st = 0; st < 2; ++st)
+      for (int st = 0; st < 2; ++st) {
+        const s16x8 df = rel_operand<T>(s, st);
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) {
-          const s16x8 kf = rel_tr_frag(K + (dt >> 1) * 8192, il, t * 4096 + st * 2048, dt & 1);
-#pragma unroll
-          for (int qs = 0; qs < NQ; ++qs) dq[qs][dt] = rel_mfma<T>(kf, df[qs][st], dq[qs][dt]);
-        }
+        for (int dt = 0; dt < D / 32; ++dt) dq[dt] = rel_mfma<T>(rel_tr_frag(K + (dt >> 1) * 8192, il, t * 4096 + st * 2048, dt & 1), df, dq[dt]);
+      }
     }
   }
-#pragma unroll
-  for (int qs = 0; qs < NQ; ++qs) {
-    const int i = i_wave + 32 * qs + r;
-    if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, dq[qs], a.scale, hf);
-  }
+  if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, dq, a.scale, hf);
   if (!a.dtab_part) return;
   // ---- this workgroup's sums by bucket: the far sums join their wave's vectors at its ends, the vectors are added in order, and
   // a thread per (bucket, slice) collects its distances
@@ -809,7 +769,7 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelArgs a) {
   if (tid < a.buckets) {
     t = 0.f;
     for (int s = 0; s < slices; ++s) t += red[s * a.buckets + tid];
-    a.dtab_part[(int64_t)item * a.buckets + tid] = t;
+    a.dtab_part[((int64_t)bh * nqb + qb) * a.buckets + tid] = t;
   }
 }
 
@@ -846,7 +806,7 @@ __global__ __launch_bounds__(256, 2) void rel_dkv_kernel(const RelArgs a) {
   const int r = lane & 31, hf = lane >> 5;
   const int nkb = (a.Lk + KB - 1) / KB, item = rel_item(blockIdx.x, gridDim.x), S = a.dkv_splits;
   const int unit = item / S, split = item - unit * S;
-  const int bk = unit / nkb, kb = unit - bk * nkb, b = bk / a.Hk, hk = bk - b * a.Hk;
+  const int place = unit / nkb, kb = unit - place * nkb, bk = rel_head(place, a.B * a.Hk), b = bk / a.Hk, hk = bk - b * a.Hk;
   const int off = rel_offset(a, b), klen = rel_key_len(a, b);
   const int j_wg = kb * KB, j_wave = j_wg + 32 * wave, j = j_wave + r;
   const bool kept = j < klen && rel_mask_at(a, b, j);
@@ -895,7 +855,7 @@ __global__ __launch_bounds__(256, 2) void rel_dkv_kernel(const RelArgs a) {
     char* Q = smem + ((x - begin) & 1) * STAGE;
     char* Gr = Q + CB * 8192;
     float* rows = reinterpret_cast<float*>(Q + 2 * CB * 8192);   // [lse 64][delta 64]
-    __builtin_amdgcn_s_waitcnt(0x0F70);
+    wait_vmem_all();
     if (wave < 2) rows[64 * wave + lane] = rowv;
     if (hg != head) {   // (nobody reads the old bias any more once all are past this barrier)
       __syncthreads();
@@ -1005,11 +965,7 @@ __global__ __launch_bounds__(256) void rel_dkv_join_kernel(const RelArgs a, int6
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// Queries per wave, 32 NQ.  Two blocks share every K / V fragment read from LDS, which is what bounds D = 64 otherwise; a sequence that one
-// workgroup of 128 rows covers would leave half the waves idle (256 x 12 heads x 77 rows: 58 us with two blocks, 36 with one); at
-// D = 128 two blocks do not fit the registers of two waves a SIMD.
-static int rel_nq(const mmk_rel_attn* p) { return p->D == 64 && p->Lq > 128 ? 2 : 1; }
-static int rel_dq_blocks(const mmk_rel_attn* p) { return (p->Lq + 128 * rel_nq(p) - 1) / (128 * rel_nq(p)); }
+static int rel_dq_blocks(const mmk_rel_attn* p) { return (p->Lq + 127) / 128; }
 
 constexpr int REL_LDS = 160 * 1024;
 static int64_t rel_split_lds(const mmk_rel_attn* p) {   // four waves' double-buffered tiles and the bias vector of every head of the group
@@ -1121,16 +1077,9 @@ static int rel_forward(const mmk_rel_attn* p, RelArgs& a, hipStream_t st) {
     const int64_t n = (int64_t)a.B * a.H * a.Lq * (D / 4);
     return rel_launch(rel_join_kernel<T, D>, MMK_K_REL_ATTN_FWD, (n + 255) / 256, 0, 0, a, st);
   }
-  constexpr int TILES = 2 * 2 * (D / 64) * 8192;
-  auto go = [&](auto nq) {
-    constexpr int NQ = decltype(nq)::value, EXT = 64 + 32 * NQ;
-    const int64_t grid = (int64_t)a.B * a.H * ((a.Lq + 128 * NQ - 1) / (128 * NQ));
-    return rel_launch(rel_fwd_kernel<T, D, NQ>, MMK_K_REL_ATTN_FWD, grid, TILES + rel_vec_bytes(a.far, EXT), TILES + rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
-  };
-  if constexpr (D == 64) {
-    if (rel_nq(p) == 2) return go(std::integral_constant<int, 2>());
-  }
-  return go(std::integral_constant<int, 1>());
+  constexpr int EXT = 96, TILES = 2 * 2 * (D / 64) * 8192;
+  const int64_t grid = (int64_t)a.B * a.H * ((a.Lq + 127) / 128);
+  return rel_launch(rel_fwd_kernel<T, D>, MMK_K_REL_ATTN_FWD, grid, TILES + rel_vec_bytes(a.far, EXT), TILES + rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
 }
 
 template <typename T, int D>
@@ -1138,15 +1087,11 @@ static int rel_backward(const mmk_rel_attn* p, RelArgs& a, void* dtable, hipStre
   constexpr int TILES = 2 * 2 * (D / 64) * 8192;
   const int nqb = rel_dq_blocks(p);
   if (a.Lq > 0) {
-    auto go = [&](auto nq) {
-      constexpr int NQ = decltype(nq)::value, EXT = 64 + 32 * NQ;
-      const int lds = TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 1 + rel_diag_vectors(D) : 1);
-      return rel_launch(rel_dq_kernel<T, D, NQ>, MMK_K_REL_ATTN_BWD, (int64_t)a.B * a.H * nqb, lds, TILES + (1 + rel_diag_vectors(D)) * rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
-    };
-    int rc;
-    if constexpr (D == 64) rc = rel_nq(p) == 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
-    else rc = go(std::integral_constant<int, 1>());
-    if (rc) return rc;
+    constexpr int EXT = 96;
+    if (int rc = rel_launch(rel_dq_kernel<T, D>, MMK_K_REL_ATTN_BWD, (int64_t)a.B * a.H * nqb,
+                            TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 1 + rel_diag_vectors(D) : 1),
+                            TILES + (1 + rel_diag_vectors(D)) * rel_vec_bytes(REL_MAX_FAR, EXT), a, st))
+      return rc;
   }
   if (a.Lk > 0) {
     const int64_t grid = (int64_t)a.B * a.Hk * ((a.Lk + 127) / 128) * a.dkv_splits;
