@@ -142,16 +142,17 @@ __device__ __forceinline__ void rel_bias_fill(const RelArgs& a, float* bias, int
   }
 }
 
+// (both are the same for the whole workgroup; read back into scalars, which keeps the branches on them scalar)
 __device__ __forceinline__ int rel_offset(const RelArgs& a, int b) {
   const int o = a.off_ptr ? a.off_ptr[b] : a.off;
-  return min(max(o, -(1 << 29)), 1 << 29);   // (distances stay within 32 bits; far beyond every bucket border)
+  return __builtin_amdgcn_readfirstlane(min(max(o, -(1 << 29)), 1 << 29));   // (distances stay within 32 bits; far beyond every bucket border)
 }
 // how many leading keys of the sample can be kept at all
 __device__ __forceinline__ int rel_key_len(const RelArgs& a, int b) {
   int64_t n = a.Lk;
   if (a.mask_kind == MMK_REL_MASK_LEN32) n = reinterpret_cast<const int32_t*>(a.mask)[b];
   if (a.mask_kind == MMK_REL_MASK_LEN64) n = reinterpret_cast<const int64_t*>(a.mask)[b];
-  return (int)(n < 0 ? 0 : n < a.Lk ? n : a.Lk);
+  return __builtin_amdgcn_readfirstlane((int)(n < 0 ? 0 : n < a.Lk ? n : a.Lk));
 }
 // whether the mask keeps key j (1 where there is no per-key mask); j may lie past the end
 __device__ __forceinline__ int rel_mask_at(const RelArgs& a, int b, int j) {
