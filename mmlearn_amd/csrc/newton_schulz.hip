@@ -11,8 +11,9 @@
 // large ones drown in the large ones' rounding, amplified 3.4 times a step (measured: 2e-2 instead of 6e-4).  The f16 copies carry a
 // power of two S ~ sqrt(max side), exact, which lifts the entries of large matrices (about 1 / S) out of f16's subnormals.
 //
-// Layout: rows and columns padded to 128 with zeros, which the iteration keeps.  All products have both operands contracted along their
-// rows: A = X X^T reads X; A^2 reads A (symmetric); B X reads B and the transposed copy of X that the previous step's epilogue stored.
+// Layout: sides padded with zeros, which the iteration keeps.  X is stored transposed, [n][m], as two f16 arrays: the operand S X rounded, and
+// the rest S X - that (together 22 bits, kept between steps).  A step moves 8 bytes an element: the transposed copy serves both products
+// -- B X takes its rows, X X^T contracts along its columns with transposed LDS reads -- and its epilogue is in place.
 #include <hip/hip_ext.h>
 
 #include <algorithm>
@@ -22,13 +23,10 @@
 
 namespace mmk {
 
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_GROUP = 64;      // matrices of one launch (their addresses are kernel arguments)
 constexpr int NS_PARTS = 1024;    // partial sums of squares per matrix: at one 64 x 64 tile each, enough workgroups to fill the chip
-constexpr int NS_TILE = 128;
 
 struct NsPtrs {
   const void* src[NS_GROUP];
@@ -39,14 +37,15 @@ struct NsPtrs {
 struct NsArgs {
   int rows, cols, m, n, mp, np;   // m <= n: short and long side, padded
   int tall;                       // rows > cols: X = G^T
+  int dst_vec;                    // rows of the results are whole, aligned vectors of eight
   int64_t rs, cs;                 // element strides of src
   float eps, S, inv_S;
   float ca, cb, cc;
   // workspace, all per matrix
   double* parts;   // [NS_PARTS]
-  float* x32;      // [mp][np]
-  f16_t* x16;      // [mp][np], times S
-  f16_t* xt[2];    // [np][mp], times S: read and written by alternate steps
+  float* u32;      // momentum: the update before it is normalised, [np][mp] (X^T); shares its memory with xt[1] and a16
+  f16_t* xt[2];    // X^T [np][mp], times S, rounded: read and written by alternate steps
+  f16_t* xl;       // what the rounding left
   f16_t* a16;      // [mp][mp], times S
   f16_t* b16;      // [mp][mp], times S
   // momentum
@@ -62,7 +61,7 @@ __device__ __forceinline__ int64_t ns_src_at(const NsArgs& a, int i, int j) {   
 }
 
 // Sum of squares of each matrix as NS_PARTS partials in f64 (no overflow for any f32 entries); with MOM the momentum is moved on first --
-// M <- mu M + G, U = G + mu M (nesterov) or M -- and U goes to x32, not normalised yet (through LDS where X is G^T).
+// M <- mu M + G, U = G + mu M (nesterov) or M -- and U^T goes to u32 in X^T's layout, not normalised yet (through LDS where that is U^T).
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void ns_reduce_kernel(const NsArgs a, const NsPtrs p) {
   __shared__ float tile[MOM ? 64 : 1][65];
@@ -70,7 +69,7 @@ __global__ __launch_bounds__(256) void ns_reduce_kernel(const NsArgs a, const Ns
   const int mat = blockIdx.y, l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const T* src = reinterpret_cast<const T*>(p.src[mat]);
   float* mom = MOM ? reinterpret_cast<float*>(p.mom[mat]) : nullptr;
-  float* x32 = a.x32 + (int64_t)mat * a.mp * a.np;
+  float* u32 = MOM ? a.u32 + (int64_t)mat * a.mp * a.np : nullptr;
   const int tr = (a.rows + 63) / 64, tc = (a.cols + 63) / 64;
   const bool by_col = MOM || a.cs <= a.rs;   // a wave reads along the axis that is contiguous in memory
   double sum = 0.0;
@@ -90,18 +89,18 @@ __global__ __launch_bounds__(256) void ns_reduce_kernel(const NsArgs a, const Ns
         const int k = w + 4 * u, r = r0 + k, c = c0 + l;
         mv[u] = fmaf(a.mu, mv[u], g[u]);
         g[u] = a.nesterov ? fmaf(a.mu, mv[u], g[u]) : mv[u];
-        if (a.tall) tile[k][l] = g[u];
+        if (!a.tall) tile[k][l] = g[u];
         if (r < a.rows && c < a.cols) {
           mom[(int64_t)r * a.cols + c] = mv[u];
-          if (!a.tall) x32[(int64_t)r * a.np + c] = g[u];
+          if (a.tall) u32[(int64_t)r * a.mp + c] = g[u];
         }
       }
       sum += (double)g[u] * (double)g[u];
     }
-    if (MOM && a.tall) {
+    if (MOM && !a.tall) {
       __syncthreads();
       for (int k = w; k < 64; k += 4)
-        if (c0 + k < a.cols && r0 + l < a.rows) x32[(int64_t)(c0 + k) * a.np + r0 + l] = tile[l][k];
+        if (c0 + k < a.cols && r0 + l < a.rows) u32[(int64_t)(c0 + k) * a.mp + r0 + l] = tile[l][k];
       __syncthreads();
     }
   }
@@ -114,22 +113,22 @@ __global__ __launch_bounds__(256) void ns_reduce_kernel(const NsArgs a, const Ns
   if (threadIdx.x == 0) a.parts[mat * NS_PARTS + blockIdx.x] = red[0];
 }
 
-// X = G / (|G| + eps) into x32, x16 and xt[0], zero beyond the matrix.  64 x 64 tiles through LDS for the transposed copy.
+// X^T = G^T / (|G| + eps) as xt[0] and xl, zero beyond the matrix.  64 x 64 tiles, through LDS where G is read along the other axis.
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void ns_prepare_kernel(const NsArgs a, const NsPtrs p) {
   __shared__ double red[256];
-  __shared__ float tile[64][65];
+  __shared__ float tile[64][65];   // [j][i]
   const int mat = blockIdx.y, tid = threadIdx.x, l = tid & 63, w = tid >> 6;
   const T* src = reinterpret_cast<const T*>(p.src[mat]);
-  const int tn = a.np / 64, i0 = 64 * (blockIdx.x / tn), j0 = 64 * (blockIdx.x % tn);
-  float* x32 = a.x32 + (int64_t)mat * a.mp * a.np;
-  // read along the axis that is contiguous in memory: j of X, or i
-  const bool by_j = MOM || (a.tall ? a.rs <= a.cs : a.cs <= a.rs);
+  const int64_t mn = (int64_t)a.mp * a.np;
+  const int tm = a.mp / 64, j0 = 64 * (blockIdx.x / tm), i0 = 64 * (blockIdx.x % tm);
+  // read along the axis that is contiguous in memory: i (the short side) or j
+  const bool by_i = MOM || (a.tall ? a.cs <= a.rs : a.rs <= a.cs);
   float v[16];
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
-    const int k = w + 4 * u, i = i0 + (by_j ? k : l), j = j0 + (by_j ? l : k);
-    v[u] = i < a.m && j < a.n ? (MOM ? x32[(int64_t)i * a.np + j] : to_f32(src[ns_src_at(a, i, j)])) : 0.f;
+    const int k = w + 4 * u, i = i0 + (by_i ? l : k), j = j0 + (by_i ? k : l);
+    v[u] = i < a.m && j < a.n ? (MOM ? a.u32[mat * mn + (int64_t)j * a.mp + i] : to_f32(src[ns_src_at(a, i, j)])) : 0.f;
   }
   double sq = 0.0;
   for (int k = tid; k < NS_PARTS; k += 256) sq += a.parts[mat * NS_PARTS + k];
@@ -141,178 +140,296 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const NsArgs a, const N
   }
   const float inv = (float)(1.0 / (sqrt(red[0]) + (double)a.eps));
 #pragma unroll
-  for (int u = 0; u < 16; ++u) tile[by_j ? w + 4 * u : l][by_j ? l : w + 4 * u] = v[u] * inv;
+  for (int u = 0; u < 16; ++u) tile[by_i ? w + 4 * u : l][by_i ? l : w + 4 * u] = v[u] * inv * a.S;
   __syncthreads();
-  f16_t* x16 = a.x16 + (int64_t)mat * a.mp * a.np;
-  f16_t* xt = a.xt[0] + (int64_t)mat * a.mp * a.np;
   for (int k = w; k < 64; k += 4) {
+    const int64_t at = mat * mn + (int64_t)(j0 + k) * a.mp + i0 + l;
     const float x = tile[k][l];
-    x32[(int64_t)(i0 + k) * a.np + j0 + l] = x;
-    x16[(int64_t)(i0 + k) * a.np + j0 + l] = (f16_t)(x * a.S);
-    xt[(int64_t)(j0 + k) * a.mp + i0 + l] = (f16_t)(tile[l][k] * a.S);
+    const f16_t hi = (f16_t)x;
+    a.xt[0][at] = hi;
+    a.xl[at] = (f16_t)(x - (float)hi);
   }
 }
 
-enum { NS_XXT = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3 };
+enum { NS_XXT = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3, NS_WEIGHTS = 4 };
 
-// One 128 x 128 tile of P Q^T (contraction along rows of K values), and what the step does with it:
-//   NS_XXT   A = P Q^T                      P = Q = X      NS_POLY  B = b A + c P Q^T               P = Q = A      (upper tiles + mirror)
-//   NS_STEP  X = a X + P Q^T, f32 and both f16 copies      P = B, Q = X^T
-//   NS_LAST  the same, rounded to bf16 into dst, or as the step of the f32 weights
-// W: the weights' step instead of the bf16 result
-template <int MODE, bool W>
-__global__ __launch_bounds__(256, 2) void ns_gemm_kernel(const NsArgs a, const NsPtrs p, int xt_in) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];   // 2 stages of P and Q tiles, 16 KiB each
-  constexpr int STAGE = 2 * 16384;
+// s_waitcnt vmcnt(N) as a builtin; the loop below holds no other load than the LDS-DMA it counts
+template <int N>
+__device__ __forceinline__ void ns_wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+// eight values of X at (row, col ..) of the result
+template <int MODE>
+__device__ __forceinline__ void ns_result(const NsArgs& a, void* dst, int row, int col, const float (&v)[8]) {
+  if (row >= a.rows) return;
+  const int64_t at = (int64_t)row * a.cols + col;
+  if (MODE == NS_WEIGHTS) {
+    const float lr = a.lr_dev ? *a.lr_dev : a.lr, keep = 1.f - lr * a.weight_decay, move = -lr * a.adjust;
+    float* w = reinterpret_cast<float*>(dst) + at;
+    if (a.dst_vec) {   // (rows are whole vectors)
+      if (col >= a.cols) return;
+      float4 lo = *reinterpret_cast<float4*>(w), hi = *reinterpret_cast<float4*>(w + 4);
+      lo = make_float4(fmaf(move, v[0], lo.x * keep), fmaf(move, v[1], lo.y * keep), fmaf(move, v[2], lo.z * keep), fmaf(move, v[3], lo.w * keep));
+      hi = make_float4(fmaf(move, v[4], hi.x * keep), fmaf(move, v[5], hi.y * keep), fmaf(move, v[6], hi.z * keep), fmaf(move, v[7], hi.w * keep));
+      *reinterpret_cast<float4*>(w) = lo;
+      *reinterpret_cast<float4*>(w + 4) = hi;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < a.cols) w[e] = fmaf(move, v[e], w[e] * keep);
+    }
+  } else {
+    bf16_t* o = reinterpret_cast<bf16_t*>(dst) + at;
+    if (a.dst_vec) {
+      if (col < a.cols) Vec8<bf16_t>::store(o, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < a.cols) o[e] = (bf16_t)v[e];
+    }
+  }
+}
+
+// One TM x TN tile of a product, and what the step does with it:
+//   NS_XXT      A = X X^T                 operands: columns of X^T             tiles with a block on or above the diagonal, and the mirror image
+//   NS_POLY     B = b A + c A A^T         operands: rows of A                  the same
+//   NS_STEP     X = a X + B X             rows of B, rows of X^T               X^T in place (the operand copy into the other buffer)
+//   NS_LAST     the same, rounded to bf16 into dst;  NS_WEIGHTS  the same as the step of the f32 weights
+// 2 x WN waves of 32 MB x 64 (MB x 2 accumulators of v_mfma_f32_32x32x16_f16): 128 x 128 tiles of four waves (MB = 2, WN = 2), or 256 x 256 of
+// eight (4, 4).  K steps of 64 through a ring of NST LDS stages filled by LDS-DMA, 128-byte rows: what bounds these products is the L2
+// side (rows of 64 bytes, twice the requests, made the step product of 4096 x 4096 161 us instead of 144), not latency (deeper
+// rings and fragments read a step ahead changed nothing).  Consecutive tiles run on one XCD, so that a matrix is fetched into one L2 or two
+// instead of eight.
+// The accumulators leave through LDS as f32, 64 columns at a time, so that all global accesses of the epilogue are whole rows of 16 bytes a lane.
+template <int MODE, int MB, int WN, int NST>
+__global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, const NsPtrs p, int xt_in, int tiles) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int NW = 2 * WN, NT = 64 * NW, TM = 64 * MB, TN = 64 * WN, PB = TM * 128, STAGE = PB + TN * 128, PIECES = (TM + TN) / 8 / NW;
+  constexpr bool SYM = MODE == NS_XXT || MODE == NS_POLY;
+  static_assert(TM / 8 % NW == 0 && TN / 8 % NW == 0 && (!SYM || TM == TN), "pieces divide evenly; symmetric products use square tiles");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 31, hf = lane >> 5, wm = wave >> 1, wn = wave & 1;
-  const int mat = blockIdx.y;
+  const int r = lane & 31, hf = lane >> 5, wm = wave / WN, wn = wave % WN;
+  // blockIdx -> tile: consecutive tiles on one XCD
+  const int per = gridDim.x >> 3, item = (int)blockIdx.x < per * 8 ? (blockIdx.x & 7) * per + (blockIdx.x >> 3) : blockIdx.x;
+  const int mat = item / tiles, tile = item - mat * tiles;
   const int64_t mn = (int64_t)a.mp * a.np, mm = (int64_t)a.mp * a.mp;
   int ti, tj;
-  if (MODE == NS_XXT || MODE == NS_POLY) {   // tile number -> (ti <= tj)
-    tj = (int)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
-    while ((tj + 1) * (tj + 2) / 2 <= (int)blockIdx.x) ++tj;
-    while (tj * (tj + 1) / 2 > (int)blockIdx.x) --tj;
-    ti = blockIdx.x - tj * (tj + 1) / 2;
-  } else {
-    const int tiles_m = a.mp / NS_TILE;
-    ti = blockIdx.x % tiles_m;
-    tj = blockIdx.x / tiles_m;
+  if (SYM) {   // ti <= tj
+    tj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+    while ((tj + 1) * (tj + 2) / 2 <= tile) ++tj;
+    while (tj * (tj + 1) / 2 > tile) --tj;
+    ti = tile - tj * (tj + 1) / 2;
+  } else {     // groups of eight tile rows, columns inside: the tiles in flight on an XCD share both operands
+    const int tiles_m = a.mp / TM, tiles_n = a.np / TN;
+    const int g = tile / (8 * tiles_n), rows = min(8, tiles_m - 8 * g), in = tile - g * 8 * tiles_n;
+    ti = 8 * g + in % rows;
+    tj = in / rows;
   }
   const f16_t *P, *Q;
   int K;
+  int64_t step;   // elements between K steps
   if (MODE == NS_XXT) {
-    P = Q = a.x16 + mat * mn;
+    P = a.xt[xt_in] + mat * mn + ti * TM;
+    Q = a.xt[xt_in] + mat * mn + tj * TN;
     K = a.np;
-  } else if (MODE == NS_POLY) {
-    P = Q = a.a16 + mat * mm;
-    K = a.mp;
+    step = (int64_t)64 * a.mp;
   } else {
-    P = a.b16 + mat * mm;
-    Q = a.xt[xt_in] + mat * mn;
+    P = (MODE == NS_POLY ? a.a16 : a.b16) + mat * mm + (int64_t)ti * TM * a.mp;
+    Q = (MODE == NS_POLY ? a.a16 + mat * mm : a.xt[xt_in] + mat * mn) + (int64_t)tj * TN * a.mp;
     K = a.mp;
+    step = 64;
   }
-  P += (int64_t)ti * NS_TILE * K;
-  Q += (int64_t)tj * NS_TILE * K;
-
-  uint32_t voff[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int row = 8 * (wave + 4 * u) + (lane >> 3);
-    voff[u] = (uint32_t)(row * K + ((lane & 7) ^ img_swz(row & 15)) * 8) * 2u;
-  }
+  // ---- LDS stages: attn_image.h images, rows of 64 values.  Rows of an operand: one image of TM (TN) rows.  Columns of X^T: images of
+  // 64 rows x 64 columns, 8 KiB.  A DMA piece is 8 rows; the swizzle repeats every 16 rows, so pieces of one parity share their offsets.
   const uint32_t lds0 = lds_addr_of(smem);
-  auto issue = [&](int kt) {
-    const uint32_t at = lds0 + (uint32_t)((kt & 1) * STAGE);
+  const int prow = 8 * (wave & 1) + (lane >> 3);   // (NW is even: all pieces of a wave have its parity)
+  const uint32_t voff = (uint32_t)((lane >> 3) * a.mp + ((lane & 7) ^ img_swz(prow)) * 8) * 2u;
+  auto issue = [&](int k, int stage) {
+    const uint32_t at = lds0 + (uint32_t)(stage * STAGE);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      lds_dma16(P + 64 * kt, voff[u], at + (uint32_t)((wave + 4 * u) * 1024));
-      lds_dma16(Q + 64 * kt, voff[u], at + 16384u + (uint32_t)((wave + 4 * u) * 1024));
+    for (int u = 0; u < PIECES; ++u) {
+      const bool is_p = u < TM / 8 / NW;
+      const int pc = wave + NW * (is_p ? u : u - TM / 8 / NW);
+      const f16_t* base = (is_p ? P : Q) + k * step;
+      if (MODE == NS_XXT) base += (int64_t)(8 * (pc & 7)) * a.mp + 64 * (pc >> 3);
+      else base += (int64_t)(8 * pc) * a.mp;
+      lds_dma16(base, voff, at + (uint32_t)((is_p ? 0 : PB) + pc * 1024));
     }
   };
-  f32x16 acc[2][2];
+  const ImgLane il = img_lane(lane);
+  // fragment of 32 rows (or columns) `blk` of an operand part, k quarter kk of 16
+  auto frag = [&](const char* part, int blk, int kk) -> f16x8 {
+    if (MODE == NS_XXT) return __builtin_bit_cast(f16x8, lds_tr_frag(part + (blk >> 1) * 8192, il, kk * 2048, blk & 1));
+    return *reinterpret_cast<const f16x8*>(part + blk * 4096 + il.row[kk]);
+  };
+
+  f32x16 acc[MB][2];
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < MB; ++x)
 #pragma unroll
     for (int y = 0; y < 2; ++y)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
-  const ImgLane il = img_lane(lane);
   const int nk = K / 64;
-  issue(0);
-  for (int kt = 0; kt < nk; ++kt) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    if (kt + 1 < nk) issue(kt + 1);
-    const char* sp = smem + (kt & 1) * STAGE + wm * 8192;
-    const char* sq = smem + (kt & 1) * STAGE + 16384 + wn * 8192;
+  for (int k = 0; k < min(NST - 1, nk); ++k) issue(k, k);
+  int stage = 0;
+  for (int k = 0; k < nk; ++k) {
+    if (k + NST - 2 < nk) ns_wait_loads<(NST - 2) * PIECES>();
+    else ns_wait_loads<0>();   // (nothing more is requested: the last stages arrive together)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the stage is here, and no wave still reads the one before it
+    if (k + NST - 1 < nk) issue(k + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+    const char* sp = smem + stage * STAGE;
+    const char* sq = sp + PB;
+    stage = stage == NST - 1 ? 0 : stage + 1;
+    // the fragments of a quarter are read while the products of the one before run
+    f16x8 fp[2][MB], fq[2][2];
+    auto read = [&](int kk) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) fq[kk & 1][y] = frag(sq, 2 * wn + y, kk);
+#pragma unroll
+      for (int x = 0; x < MB; ++x) fp[kk & 1][x] = frag(sp, MB * wm + x, kk);
+    };
+    read(0);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      f16x8 fp[2], fq[2];
+      if (kk < 3) read(kk + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        fp[x] = *reinterpret_cast<const f16x8*>(sp + x * 4096 + il.row[kk]);
-        fq[x] = *reinterpret_cast<const f16x8*>(sq + x * 4096 + il.row[kk]);
-      }
+      for (int x = 0; x < MB; ++x)
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x], fq[y], acc[x][y], 0, 0, 0);
+        for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk & 1][x], fq[kk & 1][y], acc[x][y], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-  // acc[x][y]: row i = 64 wm + 32 x + 8 (e >> 2) + 4 hf + (e & 3), column j = 64 wn + 32 y + r of the tile
+  // ---- epilogue: pass `pass` brings the 64 columns j of wave column wn = pass to LDS, each with the tile's TM rows i along it
+  constexpr int PITCH = TM + 4;
+  float* T = reinterpret_cast<float*>(smem);   // [64 j][PITCH]
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int pass = 0; pass < WN; ++pass) {
+    __syncthreads();
+    if (wn == pass) {
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+      for (int x = 0; x < MB; ++x)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int i = ti * NS_TILE + 64 * wm + 32 * x + 8 * g + 4 * hf, j = tj * NS_TILE + 64 * wn + 32 * y + r;
-        float v[4];
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * g + e];
-        if (MODE == NS_XXT || MODE == NS_POLY) {
-          f16_t* out = (MODE == NS_XXT ? a.a16 : a.b16) + mat * mm;
-          const f16_t* in = a.a16 + mat * mm;
-          f16x4 o;
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4*>(T + (32 * y + r) * PITCH + 32 * MB * wm + 32 * x + 8 * g + 4 * hf) =
+                make_float4(acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2], acc[x][y][4 * g + 3]);
+    }
+    __syncthreads();
+    const int j0 = tj * TN + 64 * pass, i0 = ti * TM;
+#pragma unroll 2
+    for (int c = tid; c < 8 * TM; c += NT) {
+      const int row = c / (TM / 8), col = 8 * (c % (TM / 8)), j = j0 + row, i = i0 + col;
+      float* t = T + row * PITCH + col;
+      float v[8];
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(t);
+      *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(t + 4);
+      if (SYM) {
+        const int64_t at = mat * mm + (int64_t)j * a.mp + i;
+        f16x8 o;
+        if (MODE == NS_XXT) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float t = MODE == NS_XXT ? v[e] * a.inv_S : fmaf(a.cb, (float)in[(int64_t)(i + e) * a.mp + j], v[e] * (a.cc * a.inv_S));
-            o[e] = (f16_t)t;
-            if (ti != tj) out[(int64_t)(i + e) * a.mp + j] = o[e];
-          }
-          *reinterpret_cast<f16x4*>(out + (int64_t)j * a.mp + i) = o;   // the mirror image (on the diagonal: the tile itself)
+          for (int e = 0; e < 8; ++e) o[e] = (f16_t)(v[e] * a.inv_S);
+          *reinterpret_cast<f16x8*>(a.a16 + at) = o;
         } else {
-          float* x32 = a.x32 + mat * mn;
-          const float k2 = a.inv_S * a.inv_S;
+          const f16x8 a8 = *reinterpret_cast<const f16x8*>(a.a16 + at);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(a.ca, x32[(int64_t)(i + e) * a.np + j], v[e] * k2);
-          if (MODE == NS_STEP) {
-            f16x4 o;
+          for (int e = 0; e < 8; ++e) o[e] = (f16_t)fmaf(a.cb, (float)a8[e], v[e] * (a.cc * a.inv_S));
+          *reinterpret_cast<f16x8*>(a.b16 + at) = o;
+        }
+        *reinterpret_cast<f16x8*>(t) = o;   // (this thread's own place: for the mirror image below)
+      } else {
+        // S X' = a S X + (S B) (S X) / S
+        const int64_t at = mat * mn + (int64_t)j * a.mp + i;
+        const f16x8 h8 = *reinterpret_cast<const f16x8*>(a.xt[xt_in] + at), l8 = *reinterpret_cast<const f16x8*>(a.xl + at);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              o[e] = (f16_t)(v[e] * a.S);
-              x32[(int64_t)(i + e) * a.np + j] = v[e];
-              a.x16[mat * mn + (int64_t)(i + e) * a.np + j] = o[e];
-            }
-            *reinterpret_cast<f16x4*>(a.xt[1 - xt_in] + mat * mn + (int64_t)j * a.mp + i) = o;
-          } else if (j < a.n) {
-            const float lr = W && a.lr_dev ? *a.lr_dev : a.lr;
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(a.ca, (float)h8[e] + (float)l8[e], v[e] * a.inv_S);
+        if (MODE == NS_STEP) {
+          f16x8 hi, lo;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (i + e < a.m) {
-                const int64_t at = a.tall ? (int64_t)j * a.cols + i + e : (int64_t)(i + e) * a.cols + j;
-                if (W) {
-                  float* wt = reinterpret_cast<float*>(p.dst[mat]);
-                  wt[at] = fmaf(-lr * a.adjust, v[e], wt[at] * (1.f - lr * a.weight_decay));
-                } else {
-                  reinterpret_cast<bf16_t*>(p.dst[mat])[at] = (bf16_t)v[e];
-                }
-              }
+          for (int e = 0; e < 8; ++e) {
+            hi[e] = (f16_t)v[e];
+            lo[e] = (f16_t)(v[e] - (float)hi[e]);
+          }
+          *reinterpret_cast<f16x8*>(a.xt[1 - xt_in] + at) = hi;
+          *reinterpret_cast<f16x8*>(a.xl + at) = lo;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= a.inv_S;
+          if (a.tall) {
+            ns_result<MODE>(a, p.dst[mat], j, i, v);
+          } else {
+            *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(v);
+            *reinterpret_cast<float4*>(t + 4) = *reinterpret_cast<const float4*>(v + 4);
           }
         }
       }
+    }
+    if (MODE == NS_STEP) continue;
+    if (!SYM && a.tall) continue;
+    __syncthreads();
+    if (SYM) {   // the mirror image (a tile on the diagonal is its own): 8 x 8 blocks turned in registers; eight lanes store 64 columns j of a row i
+      f16_t* out = (MODE == NS_XXT ? a.a16 : a.b16) + mat * mm;
+      for (int c = tid; c < (ti == tj ? 0 : TM); c += NT) {
+        const int j8 = 8 * (c & 7), i8 = 8 * (c >> 3);
+        f16x8 in[8], o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) in[e] = *reinterpret_cast<const f16x8*>(T + (j8 + e) * PITCH + i8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int f = 0; f < 8; ++f) o[e][f] = in[f][e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) *reinterpret_cast<f16x8*>(out + (int64_t)(i0 + i8 + e) * a.mp + j0 + j8) = o[e];
+      }
+    } else {     // rows of the result are rows i
+      for (int c = tid; c < 8 * TM; c += NT) {
+        const int j8 = 8 * (c & 7), row = c >> 3;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = T[(j8 + e) * PITCH + row];
+        ns_result<MODE>(a, p.dst[mat], i0 + row, j0 + j8, v);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
-static int64_t ns_up(int64_t v) { return (v + NS_TILE - 1) / NS_TILE * NS_TILE; }
-// bytes of one matrix in the workspace
-static int64_t ns_bytes(int rows, int cols) {
-  const int64_t mp = ns_up(std::min(rows, cols)), np = ns_up(std::max(rows, cols));
-  return NS_PARTS * 8 + mp * np * (4 + 2 + 2 * 2) + mp * mp * (2 + 2);
+static int64_t ns_up(int64_t v, int to) { return (v + to - 1) / to * to; }
+// Tiles of 256 x 256 for the step product (and the padding they need) where they fill whole rounds of the CUs to three quarters: 1 x 4096 x
+// 4096 (256 tiles) 148 us a product against 160 with tiles of 128, 12 x 768 x 2304 (324 tiles, the second round almost empty) 75 and 61
+static bool ns_wide(int count, int rows, int cols) {
+  const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+  const int64_t tiles = count * (ns_up(m, 256) / 256) * (ns_up(n, 256) / 256);
+  return tiles * 4 >= (tiles + 255) / 256 * 256 * 3;
+}
+struct NsSize {
+  int64_t mp, np, bytes;
+};
+// padded sides and bytes of one matrix in the workspace
+static NsSize ns_size(int rows, int cols, bool wide) {
+  NsSize s;
+  s.mp = ns_up(std::min(rows, cols), wide ? 256 : 128);
+  s.np = ns_up(std::max(rows, cols), wide ? 256 : 128);
+  s.bytes = NS_PARTS * 8 + s.mp * s.np * (2 * 2 + 2) + std::max(s.mp, s.np) * s.mp * 2 + s.mp * s.mp * 2;
+  return s;
 }
 // matrices of one pass: as many as 1 GiB of workspace holds, at least one
-static int ns_group(int count, int rows, int cols) {
-  const int64_t fit = (int64_t(1) << 30) / ns_bytes(rows, cols);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)count, (int64_t)NS_GROUP, fit}));
+static int ns_group(int count, int64_t bytes) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)count, (int64_t)NS_GROUP, (int64_t(1) << 30) / bytes}));
 }
 
-template <typename K>
-static int ns_launch(K kern, dim3 grid, int lds, hipStream_t st, const NsArgs& a, const NsPtrs& p, int xt_in) {
+template <int MODE, int MB, int WN, int NST>
+static int ns_gemm(const NsArgs& a, const NsPtrs& p, int count, int tiles, int xt_in, hipStream_t st) {
+  constexpr int TM = 64 * MB, TN = 64 * WN, LDS = std::max(NST * (TM + TN) * 128, 64 * (TM + 4) * 4);
+  auto kern = ns_gemm_kernel<MODE, MB, WN, NST>;
   KernelSetup ks;
-  if (int rc = kernel_setup(reinterpret_cast<const void*>(kern), 256, lds, &ks)) return rc;
+  if (int rc = kernel_setup(reinterpret_cast<const void*>(kern), 128 * WN, LDS, &ks)) return rc;
   ProfEvents pe(MMK_K_NEWTON_SCHULZ);
-  hipExtLaunchKernelGGL(kern, grid, dim3(256), lds, st, pe.start, pe.stop, 0, a, p, xt_in);
+  hipExtLaunchKernelGGL(kern, dim3(tiles * count), dim3(128 * WN), LDS, st, pe.start, pe.stop, 0, a, p, xt_in, tiles);
   MMK_LAUNCH_CHECK();
   return 0;
 }
@@ -333,21 +450,34 @@ static int ns_begin(const NsArgs& a, const NsPtrs& p, int count, bool mom, hipSt
   return 0;
 }
 
-static int ns_run(const mmk_newton_schulz_args* q, NsArgs a, const NsPtrs& p, int count, hipStream_t st) {
-  const bool mom = q->momenta != nullptr;
-  const int rc0 = MMK_DISPATCH_DTYPE(q->dtype, T, [&]() -> int { return ns_begin<T>(a, p, count, mom, st); });
-  if (rc0) return rc0;
-  const int tm = a.mp / NS_TILE, tn = a.np / NS_TILE, lds = 2 * 2 * 16384;
-  const dim3 sym(tm * (tm + 1) / 2, count), full(tm * tn, count);
+template <int MODE>
+static int ns_product(const NsArgs& a, const NsPtrs& p, int count, bool wide, int xt_in, hipStream_t st) {
+  if constexpr (MODE == NS_XXT || MODE == NS_POLY) {
+    const int tm = a.mp / 128;
+    return ns_gemm<MODE, 2, 2, 2>(a, p, count, tm * (tm + 1) / 2, xt_in, st);
+  } else {
+    if (wide) return ns_gemm<MODE, 4, 4, 2>(a, p, count, (a.mp / 256) * (a.np / 256), xt_in, st);
+    return ns_gemm<MODE, 2, 2, 2>(a, p, count, (a.mp / 128) * (a.np / 128), xt_in, st);
+  }
+}
+
+static int ns_steps(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, bool wide, hipStream_t st) {
   for (int s = 0; s < q->steps; ++s) {
-    if (int rc = ns_launch(ns_gemm_kernel<NS_XXT, false>, sym, lds, st, a, p, s & 1)) return rc;
-    if (int rc = ns_launch(ns_gemm_kernel<NS_POLY, false>, sym, lds, st, a, p, s & 1)) return rc;
-    const int rc = s + 1 < q->steps ? ns_launch(ns_gemm_kernel<NS_STEP, false>, full, lds, st, a, p, s & 1)
-                   : q->weights     ? ns_launch(ns_gemm_kernel<NS_LAST, true>, full, lds, st, a, p, s & 1)
-                                    : ns_launch(ns_gemm_kernel<NS_LAST, false>, full, lds, st, a, p, s & 1);
+    if (int rc = ns_product<NS_XXT>(a, p, count, wide, s & 1, st)) return rc;
+    if (int rc = ns_product<NS_POLY>(a, p, count, wide, s & 1, st)) return rc;
+    const int rc = s + 1 < q->steps ? ns_product<NS_STEP>(a, p, count, wide, s & 1, st)
+                   : q->weights     ? ns_product<NS_WEIGHTS>(a, p, count, wide, s & 1, st)
+                                    : ns_product<NS_LAST>(a, p, count, wide, s & 1, st);
     if (rc) return rc;
   }
   return 0;
+}
+
+static int ns_run(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, bool wide, hipStream_t st) {
+  const bool mom = q->momenta != nullptr;
+  const int rc = MMK_DISPATCH_DTYPE(q->dtype, T, [&]() -> int { return ns_begin<T>(a, p, count, mom, st); });
+  if (rc) return rc;
+  return ns_steps(q, a, p, count, wide, st);
 }
 
 static int ns_check(int count, int rows, int cols) {
@@ -364,7 +494,9 @@ extern "C" {
 
 int64_t mmk_newton_schulz_ws_bytes(int count, int rows, int cols) {
   if (ns_check(count, rows, cols)) return -1;
-  return count == 0 ? 0 : ns_bytes(rows, cols) * ns_group(count, rows, cols);
+  if (count == 0) return 0;
+  const NsSize s = ns_size(rows, cols, ns_wide(count, rows, cols));
+  return s.bytes * ns_group(count, s.bytes);
 }
 
 int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
@@ -380,8 +512,10 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
   a.tall = q->rows > q->cols;
   a.m = std::min(q->rows, q->cols);
   a.n = std::max(q->rows, q->cols);
-  a.mp = (int)ns_up(a.m);
-  a.np = (int)ns_up(a.n);
+  const bool wide = ns_wide(q->count, q->rows, q->cols);
+  const NsSize size = ns_size(q->rows, q->cols, wide);
+  a.mp = (int)size.mp;
+  a.np = (int)size.np;
   a.rs = q->row_stride;
   a.cs = q->col_stride;
   a.eps = q->eps;
@@ -397,30 +531,33 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
   a.lr = q->lr;
   a.adjust = q->adjust;
   a.weight_decay = q->weight_decay;
-  const int group = ns_group(q->count, q->rows, q->cols);
-  const int64_t mn = (int64_t)a.mp * a.np, mm = (int64_t)a.mp * a.mp;
+  const int group = ns_group(q->count, size.bytes);
+  const int64_t mn = size.mp * size.np, mm = size.mp * size.mp;
   char* w = reinterpret_cast<char*>(ws);
   auto take = [&](int64_t bytes) {
     char* at = w;
     w += bytes * group;
     return at;
   };
-  a.x32 = (float*)take(mn * 4);
-  a.x16 = (f16_t*)take(mn * 2);
-  a.xt[0] = (f16_t*)take(mn * 2);
-  a.xt[1] = (f16_t*)take(mn * 2);
-  a.a16 = (f16_t*)take(mm * 2);
-  a.b16 = (f16_t*)take(mm * 2);
   a.parts = (double*)take(NS_PARTS * 8);
+  a.xt[0] = (f16_t*)take(mn * 2);
+  a.xl = (f16_t*)take(mn * 2);
+  // xt[1] and, behind it, a16: the un-normalised update of the momentum (4 bytes an element) is read before either is written
+  a.u32 = (float*)w;
+  a.xt[1] = (f16_t*)take(mn * 2);
+  a.a16 = (f16_t*)take(std::max(mm, mn) * 2);
+  a.b16 = (f16_t*)take(mm * 2);
   for (int at = 0; at < q->count; at += group) {
     const int n = std::min(group, q->count - at);
     NsPtrs p = {};
+    a.dst_vec = q->cols % 8 == 0;
     for (int i = 0; i < n; ++i) {
       p.src[i] = q->src[at + i];
       p.mom[i] = q->momenta ? q->momenta[at + i] : nullptr;
       p.dst[i] = q->dst[at + i];
+      a.dst_vec &= reinterpret_cast<uintptr_t>(p.dst[i]) % 16 == 0;
     }
-    if (int rc = ns_run(q, a, p, n, (hipStream_t)stream)) return rc;
+    if (int rc = ns_run(q, a, p, n, wide, (hipStream_t)stream)) return rc;
   }
   return 0;
 }
