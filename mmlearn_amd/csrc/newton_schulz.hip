@@ -197,7 +197,7 @@ __device__ __forceinline__ void ns_result(const NsArgs& a, void* dst, int row, i
 //   NS_STEP     X = a X + B X             rows of B, rows of X^T               X^T in place (the operand copy into the other buffer)
 //   NS_LAST     the same, rounded to bf16 into dst;  NS_WEIGHTS  the same as the step of the f32 weights
 // 2 x WN waves of 32 MB x 64 (MB x 2 accumulators of v_mfma_f32_32x32x16_f16): 128 x 128 tiles of four waves (MB = 2, WN = 2), or 256 x 256 of
-// eight (4, 4).  K steps of 64 through a ring of NST LDS stages filled by LDS-DMA, 128-byte rows: what bounds these products is the L2
+// eight (4, 4).  K steps of 64 through NST LDS stages (one: no overlap within a workgroup) filled by LDS-DMA, 128-byte rows: what bounds these products is the L2
 // side (rows of 64 bytes, twice the requests, made the step product of 4096 x 4096 161 us instead of 144), not latency (deeper
 // rings and fragments read a step ahead changed nothing).  Consecutive tiles run on one XCD, so that a matrix is fetched into one L2 or two
 // instead of eight.
@@ -272,13 +272,13 @@ __global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, co
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
   const int nk = K / 64;
-  for (int k = 0; k < min(NST - 1, nk); ++k) issue(k, k);
+  for (int k = 0; k < min(max(NST - 1, 1), nk); ++k) issue(k, k);
   int stage = 0;
   for (int k = 0; k < nk; ++k) {
-    if (k + NST - 2 < nk) ns_wait_loads<(NST - 2) * PIECES>();
+    if (NST > 1 && k + NST - 2 < nk) ns_wait_loads<(NST > 1 ? NST - 2 : 0) * PIECES>();
     else ns_wait_loads<0>();   // (nothing more is requested: the last stages arrive together)
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the stage is here, and no wave still reads the one before it
-    if (k + NST - 1 < nk) issue(k + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+    if (NST > 1 && k + NST - 1 < nk) issue(k + NST - 1, stage == 0 ? NST - 1 : stage - 1);
     const char* sp = smem + stage * STAGE;
     const char* sq = sp + PB;
     stage = stage == NST - 1 ? 0 : stage + 1;
@@ -300,6 +300,10 @@ __global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, co
 #pragma unroll
         for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk & 1][x], fq[kk & 1][y], acc[x][y], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if (NST == 1 && k + 1 < nk) {   // the one stage is free once all waves have read it
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      issue(k + 1, 0);
     }
   }
   // ---- epilogue: pass `pass` brings the 64 columns j of wave column wn = pass to LDS, each with the tile's TM rows i along it
@@ -450,15 +454,16 @@ static int ns_begin(const NsArgs& a, const NsPtrs& p, int count, bool mom, hipSt
   return 0;
 }
 
+// Stages of the ring: with more than two workgroups for every CU one stage each (four share a CU, and the loads of one run under the products
+// of the others: 12 x 768 x 2304, 1296 tiles, 57 us a step product against 61 with two stages; 4096 x 4096, 528 tiles, 101 us for X X^T
+// against 114), else two (252 tiles: 34 us against 45)
 template <int MODE>
 static int ns_product(const NsArgs& a, const NsPtrs& p, int count, bool wide, int xt_in, hipStream_t st) {
-  if constexpr (MODE == NS_XXT || MODE == NS_POLY) {
-    const int tm = a.mp / 128;
-    return ns_gemm<MODE, 2, 2, 2>(a, p, count, tm * (tm + 1) / 2, xt_in, st);
-  } else {
-    if (wide) return ns_gemm<MODE, 4, 4, 2>(a, p, count, (a.mp / 256) * (a.np / 256), xt_in, st);
-    return ns_gemm<MODE, 2, 2, 2>(a, p, count, (a.mp / 128) * (a.np / 128), xt_in, st);
-  }
+  const int tm = a.mp / 128;
+  int tiles = tm * (a.np / 128);
+  if constexpr (MODE == NS_XXT || MODE == NS_POLY) tiles = tm * (tm + 1) / 2;
+  else if (wide) return ns_gemm<MODE, 4, 4, 2>(a, p, count, (a.mp / 256) * (a.np / 256), xt_in, st);
+  return (int64_t)tiles * count > 512 ? ns_gemm<MODE, 2, 2, 1>(a, p, count, tiles, xt_in, st) : ns_gemm<MODE, 2, 2, 2>(a, p, count, tiles, xt_in, st);
 }
 
 static int ns_steps(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, bool wide, hipStream_t st) {
