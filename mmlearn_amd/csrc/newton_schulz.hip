@@ -24,6 +24,7 @@
 namespace mmk {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_GROUP = 64;      // matrices of one launch (their addresses are kernel arguments)
 constexpr int NS_PARTS = 1024;    // partial sums of squares per matrix: at one 64 x 64 tile each, enough workgroups to fill the chip
@@ -56,6 +57,16 @@ struct NsArgs {
   float lr, adjust, weight_decay;
 };
 
+// moves the momentum on and returns the update
+__device__ __forceinline__ float ns_momentum(const NsArgs& a, float& m, float g) {
+  m = fmaf(a.mu, m, g);
+  return a.nesterov ? fmaf(a.mu, m, g) : m;
+}
+// one weight's step; `lr` in f32 as it stands in the device word
+__device__ __forceinline__ float ns_weight(const NsArgs& a, float lr, float w, float x) {
+  return fmaf(-lr * a.adjust, x, w * (1.f - lr * a.weight_decay));
+}
+
 __device__ __forceinline__ int64_t ns_src_at(const NsArgs& a, int i, int j) {   // element (i, j) of X in G
   return a.tall ? (int64_t)j * a.rs + (int64_t)i * a.cs : (int64_t)i * a.rs + (int64_t)j * a.cs;
 }
@@ -87,8 +98,7 @@ __global__ __launch_bounds__(256) void ns_reduce_kernel(const NsArgs a, const Ns
     for (int u = 0; u < 16; ++u) {
       if (MOM) {
         const int k = w + 4 * u, r = r0 + k, c = c0 + l;
-        mv[u] = fmaf(a.mu, mv[u], g[u]);
-        g[u] = a.nesterov ? fmaf(a.mu, mv[u], g[u]) : mv[u];
+        g[u] = ns_momentum(a, mv[u], g[u]);
         if (!a.tall) tile[k][l] = g[u];
         if (r < a.rows && c < a.cols) {
           mom[(int64_t)r * a.cols + c] = mv[u];
@@ -165,19 +175,17 @@ __device__ __forceinline__ void ns_result(const NsArgs& a, void* dst, int row, i
   if (row >= a.rows) return;
   const int64_t at = (int64_t)row * a.cols + col;
   if (MODE == NS_WEIGHTS) {
-    const float lr = a.lr_dev ? *a.lr_dev : a.lr, keep = 1.f - lr * a.weight_decay, move = -lr * a.adjust;
+    const float lr = a.lr_dev ? *a.lr_dev : a.lr;
     float* w = reinterpret_cast<float*>(dst) + at;
     if (a.dst_vec) {   // (rows are whole vectors)
       if (col >= a.cols) return;
-      float4 lo = *reinterpret_cast<float4*>(w), hi = *reinterpret_cast<float4*>(w + 4);
-      lo = make_float4(fmaf(move, v[0], lo.x * keep), fmaf(move, v[1], lo.y * keep), fmaf(move, v[2], lo.z * keep), fmaf(move, v[3], lo.w * keep));
-      hi = make_float4(fmaf(move, v[4], hi.x * keep), fmaf(move, v[5], hi.y * keep), fmaf(move, v[6], hi.z * keep), fmaf(move, v[7], hi.w * keep));
-      *reinterpret_cast<float4*>(w) = lo;
-      *reinterpret_cast<float4*>(w + 4) = hi;
+      const float4 lo = *reinterpret_cast<float4*>(w), hi = *reinterpret_cast<float4*>(w + 4);
+      *reinterpret_cast<float4*>(w) = make_float4(ns_weight(a, lr, lo.x, v[0]), ns_weight(a, lr, lo.y, v[1]), ns_weight(a, lr, lo.z, v[2]), ns_weight(a, lr, lo.w, v[3]));
+      *reinterpret_cast<float4*>(w + 4) = make_float4(ns_weight(a, lr, hi.x, v[4]), ns_weight(a, lr, hi.y, v[5]), ns_weight(a, lr, hi.z, v[6]), ns_weight(a, lr, hi.w, v[7]));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (col + e < a.cols) w[e] = fmaf(move, v[e], w[e] * keep);
+        if (col + e < a.cols) w[e] = ns_weight(a, lr, w[e], v[e]);
     }
   } else {
     bf16_t* o = reinterpret_cast<bf16_t*>(dst) + at;
@@ -401,6 +409,182 @@ __global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, co
   }
 }
 
+// ------------------------------------------------------------------------------------------------ small matrices
+// A matrix of at most 128 x 256 never leaves its CU: one workgroup of eight waves does the whole iteration (the launches alone cost 108 us
+// for 201 x 65, this 39).  X^T is held twice: in f32 in the accumulator layout of the step product (wave w: rows 32 w .. of X^T on the
+// lanes, 128 columns in 4 x 16 registers), which takes a X without any rounding, and rounded to f16 in LDS (two images of 256 rows x 64
+// columns), whose rows serve B X and whose columns, read transposed, X X^T.  A and then B stand in a third place (two images of 128 x 64).
+constexpr int NS_SMALL_M = 128, NS_SMALL_N = 256, NS_SMALL_PITCH = 129;
+constexpr int NS_SMALL_X = 2 * 256 * 128, NS_SMALL_LDS = NS_SMALL_X + 128 * NS_SMALL_PITCH * 4;
+
+// byte offset of column c (of 128) in row `row` of the images at distance `image` of each other
+__device__ __forceinline__ int ns_img_at(int row, int c, int image) {
+  return (c >> 6) * image + row * 128 + ((((c & 63) >> 3) ^ img_swz(row)) << 4) + (c & 7) * 2;
+}
+
+template <typename T, bool MOM, bool W>
+__global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const NsPtrs p, int steps) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* X = smem;
+  char* A = smem + NS_SMALL_X;                          // 32 KiB, inside the staging area of the first and last phase
+  float* stage = reinterpret_cast<float*>(A);           // [128 j][129]
+  const int mat = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, hf = lane >> 5, fast = tid & 127, slow = tid >> 7;
+  const T* src = reinterpret_cast<const T*>(p.src[mat]);
+  float* mom = MOM ? reinterpret_cast<float*>(p.mom[mat]) : nullptr;
+  const int halves = a.n > 128 ? 2 : 1;
+  f32x16 x[4];
+  double sum = 0.0;
+  // ---- G in halves of 128 rows j of X^T, read along the axis that is contiguous in memory
+  const bool by_i = a.tall ? a.cs <= a.rs : a.rs <= a.cs;
+  for (int half = 0; half < 2; ++half) {
+    if (half < halves) {
+#pragma unroll 8
+      for (int k = slow; k < 128; k += 4) {
+        const int i = by_i ? fast : k, jl = by_i ? k : fast, j = 128 * half + jl;
+        float v = 0.f;
+        if (i < a.m && j < a.n) {
+          v = to_f32(src[ns_src_at(a, i, j)]);
+          if (MOM) {
+            float* at = mom + (a.tall ? (int64_t)j * a.cols + i : (int64_t)i * a.cols + j);
+            float m = *at;
+            v = ns_momentum(a, m, v);
+            *at = m;
+          }
+        }
+        sum += (double)v * (double)v;
+        stage[jl * NS_SMALL_PITCH + i] = v;
+      }
+    }
+    __syncthreads();
+    if (wave >> 2 == half) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          x[b][e] = half < halves ? stage[(32 * (wave & 3) + r) * NS_SMALL_PITCH + 32 * b + (e & 3) + 8 * (e >> 2) + 4 * hf] : 0.f;
+    }
+    __syncthreads();
+  }
+  double* red = reinterpret_cast<double*>(stage);
+  red[tid] = sum;
+  __syncthreads();
+  for (int o = 256; o > 0; o >>= 1) {
+    if (tid < o) red[tid] += red[tid + o];
+    __syncthreads();
+  }
+  const float scale = (float)(1.0 / (sqrt(red[0]) + (double)a.eps)) * a.S;   // (the product with S is exact)
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[b][e] *= scale;
+  auto store_x = [&]() {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f16x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (f16_t)x[b][4 * g + e];
+        *reinterpret_cast<f16x4*>(X + ns_img_at(32 * wave + r, 32 * b + 8 * g + 4 * hf, 32768)) = o;
+      }
+  };
+  store_x();
+  const ImgLane il = img_lane(lane);
+  const int bi = wave >> 1, bc = 2 * (wave & 1);   // this wave's blocks of A: rows 32 bi .., columns 32 bc .. + 63
+  const int k16 = (a.n + 15) / 16;
+  auto zero = [](f32x16& z) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  };
+  for (int s = 0; s < steps; ++s) {
+    __syncthreads();   // X is complete; nobody reads B any more
+    f32x16 acc[4];
+    zero(acc[0]);
+    zero(acc[1]);
+    for (int k = 0; k < k16; ++k) {
+      const f16x8 fp = __builtin_bit_cast(f16x8, lds_tr_frag(X + (bi >> 1) * 32768, il, k * 2048, bi & 1));
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp, __builtin_bit_cast(f16x8, lds_tr_frag(X + (bc >> 1) * 32768, il, k * 2048, y)), acc[y], 0, 0, 0);
+    }
+    // element (i, i') of the symmetric result stands in row i' (the lane) at columns i (four registers): its mirror image
+    f16x4 av[2][4];
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) av[y][g][e] = (f16_t)(acc[y][4 * g + e] * a.inv_S);
+        *reinterpret_cast<f16x4*>(A + ns_img_at(32 * (bc + y) + r, 32 * bi + 8 * g + 4 * hf, 16384)) = av[y][g];
+      }
+    __syncthreads();
+    zero(acc[0]);
+    zero(acc[1]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const f16x8 fp = *reinterpret_cast<const f16x8*>(A + (k >> 2) * 16384 + bi * 4096 + il.row[k & 3]);
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp, *reinterpret_cast<const f16x8*>(A + (k >> 2) * 16384 + (bc + y) * 4096 + il.row[k & 3]), acc[y], 0, 0, 0);
+    }
+    __syncthreads();   // all of A is read
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f16x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (f16_t)fmaf(a.cb, (float)av[y][g][e], acc[y][4 * g + e] * (a.cc * a.inv_S));
+        *reinterpret_cast<f16x4*>(A + ns_img_at(32 * (bc + y) + r, 32 * bi + 8 * g + 4 * hf, 16384)) = o;
+      }
+    __syncthreads();
+    if (32 * wave < a.n) {   // (rows past the matrix are zero and stay so)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) zero(acc[b]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const f16x8 fq = *reinterpret_cast<const f16x8*>(X + (k >> 2) * 32768 + wave * 4096 + il.row[k & 3]);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(A + (k >> 2) * 16384 + b * 4096 + il.row[k & 3]), fq, acc[b], 0, 0, 0);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[b][e] = fmaf(a.ca, x[b][e], acc[b][e] * a.inv_S);
+      if (s + 1 < steps) store_x();   // (a wave's rows are its own in this product)
+    }
+  }
+  // ---- result, half by half through LDS
+  const float lr = W && a.lr_dev ? *a.lr_dev : a.lr;
+  for (int half = 0; half < halves; ++half) {
+    __syncthreads();
+    if (wave >> 2 == half) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          stage[(32 * (wave & 3) + r) * NS_SMALL_PITCH + 32 * b + (e & 3) + 8 * (e >> 2) + 4 * hf] = x[b][e] * a.inv_S;
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int k = slow; k < 128; k += 4) {   // rows of the result run along i if it is tall, else along j
+      const int i = a.tall ? fast : k, jl = a.tall ? k : fast, j = 128 * half + jl;
+      if (i < a.m && j < a.n) {
+        const int64_t at = a.tall ? (int64_t)j * a.cols + i : (int64_t)i * a.cols + j;
+        const float v = stage[jl * NS_SMALL_PITCH + i];
+        if (W) {
+          float* w = reinterpret_cast<float*>(p.dst[mat]) + at;
+          *w = ns_weight(a, lr, *w, v);
+        } else {
+          reinterpret_cast<bf16_t*>(p.dst[mat])[at] = (bf16_t)v;
+        }
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ host
 static int64_t ns_up(int64_t v, int to) { return (v + to - 1) / to * to; }
 // Tiles of 256 x 256 for the step product (and the padding they need) where they fill whole rounds of the CUs to three quarters: 1 x 4096 x
@@ -485,6 +669,21 @@ static int ns_run(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs
   return ns_steps(q, a, p, count, wide, st);
 }
 
+static bool ns_small(int rows, int cols) { return std::min(rows, cols) <= NS_SMALL_M && std::max(rows, cols) <= NS_SMALL_N; }
+template <typename T>
+static int ns_small_run(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, hipStream_t st) {
+  auto go = [&](auto kern) {
+    KernelSetup ks;
+    if (int rc = kernel_setup(reinterpret_cast<const void*>(kern), 512, NS_SMALL_LDS, &ks)) return rc;
+    ProfEvents pe(MMK_K_NEWTON_SCHULZ);
+    hipExtLaunchKernelGGL(kern, dim3(count), dim3(512), NS_SMALL_LDS, st, pe.start, pe.stop, 0, a, p, (int)q->steps);
+    MMK_LAUNCH_CHECK();
+    return 0;
+  };
+  if (q->momenta) return q->weights ? go(ns_small_kernel<T, true, true>) : go(ns_small_kernel<T, true, false>);
+  return q->weights ? go(ns_small_kernel<T, false, true>) : go(ns_small_kernel<T, false, false>);
+}
+
 static int ns_check(int count, int rows, int cols) {
   MMK_REQUIRE(count >= 0 && rows >= 1 && cols >= 1, "bad sizes");
   MMK_REQUIRE(std::max(rows, cols) <= 32768, "sides up to 32768");   // a tile's rows are addressed by 32-bit byte offsets
@@ -499,7 +698,7 @@ extern "C" {
 
 int64_t mmk_newton_schulz_ws_bytes(int count, int rows, int cols) {
   if (ns_check(count, rows, cols)) return -1;
-  if (count == 0) return 0;
+  if (count == 0 || ns_small(rows, cols)) return 0;
   const NsSize s = ns_size(rows, cols, ns_wide(count, rows, cols));
   return s.bytes * ns_group(count, s.bytes);
 }
@@ -510,7 +709,8 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
   MMK_REQUIRE(q->steps >= 1 && q->steps <= 32, "1 to 32 steps");
   MMK_REQUIRE(!q->momenta || q->dtype == MMK_F32 || q->dtype == MMK_BF16 || q->dtype == MMK_F16, "unsupported dtype");
   if (q->count == 0) return 0;
-  MMK_REQUIRE(q->src && q->dst && ws, "missing operand");
+  const bool small = ns_small(q->rows, q->cols);
+  MMK_REQUIRE(q->src && q->dst && (ws || small), "missing operand");
   NsArgs a = {};
   a.rows = q->rows;
   a.cols = q->cols;
@@ -536,7 +736,7 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
   a.lr = q->lr;
   a.adjust = q->adjust;
   a.weight_decay = q->weight_decay;
-  const int group = ns_group(q->count, size.bytes);
+  const int group = small ? NS_GROUP : ns_group(q->count, size.bytes);
   const int64_t mn = size.mp * size.np, mm = size.mp * size.mp;
   char* w = reinterpret_cast<char*>(ws);
   auto take = [&](int64_t bytes) {
@@ -562,7 +762,9 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
       p.dst[i] = q->dst[at + i];
       a.dst_vec &= reinterpret_cast<uintptr_t>(p.dst[i]) % 16 == 0;
     }
-    if (int rc = ns_run(q, a, p, n, wide, (hipStream_t)stream)) return rc;
+    const int rc = small ? MMK_DISPATCH_DTYPE(q->dtype, T, [&]() -> int { return ns_small_run<T>(q, a, p, n, (hipStream_t)stream); })
+                         : ns_run(q, a, p, n, wide, (hipStream_t)stream);
+    if (rc) return rc;
   }
   return 0;
 }
