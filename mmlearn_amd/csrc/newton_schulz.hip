@@ -209,14 +209,17 @@ __device__ __forceinline__ void ns_result(const NsArgs& a, void* dst, int row, i
 // side (rows of 64 bytes, twice the requests, made the step product of 4096 x 4096 161 us instead of 144), not latency (deeper
 // rings and fragments read a step ahead changed nothing).  Consecutive tiles run on one XCD, so that a matrix is fetched into one L2 or two
 // instead of eight.
+// KG groups of waves take the K steps in turn, each with a ring of its own, and their accumulators are added in LDS on the way out (always in
+// the same order): a workgroup that is alone on its CU then has two waves on each SIMD, and half the barriers.
 // The accumulators leave through LDS as f32, 64 columns at a time, so that all global accesses of the epilogue are whole rows of 16 bytes a lane.
-template <int MODE, int MB, int WN, int NST>
-__global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, const NsPtrs p, int xt_in, int tiles) {
+template <int MODE, int MB, int WN, int NST, int KG>
+__global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs a, const NsPtrs p, int xt_in, int tiles) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int NW = 2 * WN, NT = 64 * NW, TM = 64 * MB, TN = 64 * WN, PB = TM * 128, STAGE = PB + TN * 128, PIECES = (TM + TN) / 8 / NW;
+  constexpr int NW = 2 * WN, NT = 64 * NW * KG, TM = 64 * MB, TN = 64 * WN, PB = TM * 128, STAGE = PB + TN * 128, PIECES = (TM + TN) / 8 / NW;
   constexpr bool SYM = MODE == NS_XXT || MODE == NS_POLY;
   static_assert(TM / 8 % NW == 0 && TN / 8 % NW == 0 && (!SYM || TM == TN), "pieces divide evenly; symmetric products use square tiles");
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, all_waves = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = all_waves / NW, wave = all_waves % NW;
   const int r = lane & 31, hf = lane >> 5, wm = wave / WN, wn = wave % WN;
   // blockIdx -> tile: consecutive tiles on one XCD
   const int per = gridDim.x >> 3, item = (int)blockIdx.x < per * 8 ? (blockIdx.x & 7) * per + (blockIdx.x >> 3) : blockIdx.x;
@@ -250,7 +253,8 @@ __global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, co
   }
   // ---- LDS stages: attn_image.h images, rows of 64 values.  Rows of an operand: one image of TM (TN) rows.  Columns of X^T: images of
   // 64 rows x 64 columns, 8 KiB.  A DMA piece is 8 rows; the swizzle repeats every 16 rows, so pieces of one parity share their offsets.
-  const uint32_t lds0 = lds_addr_of(smem);
+  char* const ring = smem + kg * NST * STAGE;
+  const uint32_t lds0 = lds_addr_of(ring);
   const int prow = 8 * (wave & 1) + (lane >> 3);   // (NW is even: all pieces of a wave have its parity)
   const uint32_t voff = (uint32_t)((lane >> 3) * a.mp + ((lane & 7) ^ img_swz(prow)) * 8) * 2u;
   auto issue = [&](int k, int stage) {
@@ -259,7 +263,7 @@ __global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, co
     for (int u = 0; u < PIECES; ++u) {
       const bool is_p = u < TM / 8 / NW;
       const int pc = wave + NW * (is_p ? u : u - TM / 8 / NW);
-      const f16_t* base = (is_p ? P : Q) + k * step;
+      const f16_t* base = (is_p ? P : Q) + (k * KG + kg) * step;
       if (MODE == NS_XXT) base += (int64_t)(8 * (pc & 7)) * a.mp + 64 * (pc >> 3);
       else base += (int64_t)(8 * pc) * a.mp;
       lds_dma16(base, voff, at + (uint32_t)((is_p ? 0 : PB) + pc * 1024));
@@ -279,15 +283,15 @@ __global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, co
     for (int y = 0; y < 2; ++y)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
-  const int nk = K / 64;
+  const int all_k = K / 64, nk = (all_k - kg + KG - 1) / KG, turns = (all_k + KG - 1) / KG;   // this group's steps kg, kg + KG ..; turns of the workgroup
   for (int k = 0; k < min(max(NST - 1, 1), nk); ++k) issue(k, k);
   int stage = 0;
-  for (int k = 0; k < nk; ++k) {
+  for (int k = 0; k < turns; ++k) {
     if (NST > 1 && k + NST - 2 < nk) ns_wait_loads<(NST > 1 ? NST - 2 : 0) * PIECES>();
     else ns_wait_loads<0>();   // (nothing more is requested: the last stages arrive together)
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the stage is here, and no wave still reads the one before it
     if (NST > 1 && k + NST - 1 < nk) issue(k + NST - 1, stage == 0 ? NST - 1 : stage - 1);
-    const char* sp = smem + stage * STAGE;
+    const char* sp = ring + stage * STAGE;
     const char* sq = sp + PB;
     stage = stage == NST - 1 ? 0 : stage + 1;
     // the fragments of a quarter are read while the products of the one before run
@@ -298,20 +302,22 @@ __global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, co
 #pragma unroll
       for (int x = 0; x < MB; ++x) fp[kk & 1][x] = frag(sp, MB * wm + x, kk);
     };
-    read(0);
+    if (KG == 1 || k < nk) {   // (the last turn may have no step for the second group)
+      read(0);
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      if (kk < 3) read(kk + 1);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int kk = 0; kk < 4; ++kk) {
+        if (kk < 3) read(kk + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < MB; ++x)
+        for (int x = 0; x < MB; ++x)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk & 1][x], fq[kk & 1][y], acc[x][y], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
+          for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk & 1][x], fq[kk & 1][y], acc[x][y], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    if (NST == 1 && k + 1 < nk) {   // the one stage is free once all waves have read it
+    if (NST == 1 && k + 1 < turns) {   // the one stage is free once all waves have read it
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      issue(k + 1, 0);
+      if (k + 1 < nk) issue(k + 1, 0);
     }
   }
   // ---- epilogue: pass `pass` brings the 64 columns j of wave column wn = pass to LDS, each with the tile's TM rows i along it
@@ -320,17 +326,26 @@ __global__ __launch_bounds__(128 * WN, 2) void ns_gemm_kernel(const NsArgs a, co
 #pragma unroll
   for (int pass = 0; pass < WN; ++pass) {
     __syncthreads();
-    if (wn == pass) {
 #pragma unroll
-      for (int x = 0; x < MB; ++x)
+    for (int from = 0; from < KG; ++from) {
+      if (wn == pass && kg == from) {
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int x = 0; x < MB; ++x)
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4*>(T + (32 * y + r) * PITCH + 32 * MB * wm + 32 * x + 8 * g + 4 * hf) =
-                make_float4(acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2], acc[x][y][4 * g + 3]);
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              float4* at = reinterpret_cast<float4*>(T + (32 * y + r) * PITCH + 32 * MB * wm + 32 * x + 8 * g + 4 * hf);
+              float4 v = make_float4(acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2], acc[x][y][4 * g + 3]);
+              if (from > 0) {
+                const float4 o = *at;
+                v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+              }
+              *at = v;
+            }
+      }
+      __syncthreads();
     }
-    __syncthreads();
     const int j0 = tj * TN + 64 * pass, i0 = ti * TM;
 #pragma unroll 2
     for (int c = tid; c < 8 * TM; c += NT) {
@@ -610,14 +625,14 @@ static int ns_group(int count, int64_t bytes) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)count, (int64_t)NS_GROUP, (int64_t(1) << 30) / bytes}));
 }
 
-template <int MODE, int MB, int WN, int NST>
+template <int MODE, int MB, int WN, int NST, int KG>
 static int ns_gemm(const NsArgs& a, const NsPtrs& p, int count, int tiles, int xt_in, hipStream_t st) {
-  constexpr int TM = 64 * MB, TN = 64 * WN, LDS = std::max(NST * (TM + TN) * 128, 64 * (TM + 4) * 4);
-  auto kern = ns_gemm_kernel<MODE, MB, WN, NST>;
+  constexpr int TM = 64 * MB, TN = 64 * WN, LDS = std::max(KG * NST * (TM + TN) * 128, 64 * (TM + 4) * 4);
+  auto kern = ns_gemm_kernel<MODE, MB, WN, NST, KG>;
   KernelSetup ks;
-  if (int rc = kernel_setup(reinterpret_cast<const void*>(kern), 128 * WN, LDS, &ks)) return rc;
+  if (int rc = kernel_setup(reinterpret_cast<const void*>(kern), 128 * WN * KG, LDS, &ks)) return rc;
   ProfEvents pe(MMK_K_NEWTON_SCHULZ);
-  hipExtLaunchKernelGGL(kern, dim3(tiles * count), dim3(128 * WN), LDS, st, pe.start, pe.stop, 0, a, p, xt_in, tiles);
+  hipExtLaunchKernelGGL(kern, dim3(tiles * count), dim3(128 * WN * KG), LDS, st, pe.start, pe.stop, 0, a, p, xt_in, tiles);
   MMK_LAUNCH_CHECK();
   return 0;
 }
@@ -640,14 +655,18 @@ static int ns_begin(const NsArgs& a, const NsPtrs& p, int count, bool mom, hipSt
 
 // Stages of the ring: with more than two workgroups for every CU one stage each (four share a CU, and the loads of one run under the products
 // of the others: 12 x 768 x 2304, 1296 tiles, 57 us a step product against 61 with two stages; 4096 x 4096, 528 tiles, 101 us for X X^T
-// against 114), else two (252 tiles: 34 us against 45)
+// against 114), else two (252 tiles: 34 us against 45).  At most one workgroup a CU: two groups of waves along K (whole iterations of
+// 1024 x 4096: 355 us against 422, 128 x 4096: 243 against 279, 1536 x 1536: 302 against 353; four groups of one stage were slower, and
+// two groups of one stage for up to 512 tiles too)
 template <int MODE>
 static int ns_product(const NsArgs& a, const NsPtrs& p, int count, bool wide, int xt_in, hipStream_t st) {
   const int tm = a.mp / 128;
   int tiles = tm * (a.np / 128);
   if constexpr (MODE == NS_XXT || MODE == NS_POLY) tiles = tm * (tm + 1) / 2;
-  else if (wide) return ns_gemm<MODE, 4, 4, 2>(a, p, count, (a.mp / 256) * (a.np / 256), xt_in, st);
-  return (int64_t)tiles * count > 512 ? ns_gemm<MODE, 2, 2, 1>(a, p, count, tiles, xt_in, st) : ns_gemm<MODE, 2, 2, 2>(a, p, count, tiles, xt_in, st);
+  else if (wide) return ns_gemm<MODE, 4, 4, 2, 1>(a, p, count, (a.mp / 256) * (a.np / 256), xt_in, st);
+  const int64_t all = (int64_t)tiles * count;
+  if (all <= 256) return ns_gemm<MODE, 2, 2, 2, 2>(a, p, count, tiles, xt_in, st);
+  return all > 512 ? ns_gemm<MODE, 2, 2, 1, 1>(a, p, count, tiles, xt_in, st) : ns_gemm<MODE, 2, 2, 2, 1>(a, p, count, tiles, xt_in, st);
 }
 
 static int ns_steps(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, bool wide, hipStream_t st) {
