@@ -174,6 +174,11 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, device=None) -
     return torch.cat((angle.cos(), angle.sin()), 1).float().to(device)
 
 
+def _records(*operands: Optional[torch.Tensor]) -> bool:
+    """Whether autograd has to record the call (an autograd function costs a single token more than its kernel)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands)
+
+
 class _QKNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, table, positions, interleaved, eps):
@@ -233,6 +238,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
         raise ValueError(f"{name}: positions are int32 or int64 [L] or [B, L] with a contiguous last dim")
     if any(t is not None and t.device != q.device for t in (k, q_weight, k_weight, rotary, positions)):
         raise ValueError(f"{name}: all operands must be on one device")
+    if not _records(q, k, q_weight, k_weight):
+        return K.qk_norm_rotary_fwd(q, k, q_weight, k_weight, rotary, positions, interleaved, eps)
     return _QKNormRotary.apply(q, k, q_weight, k_weight, rotary, positions, bool(interleaved), float(eps))
 
 
@@ -287,7 +294,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     if not (k.shape == v.shape and k.shape[0] == B and k.shape[3] == D and D in (64, 128) and k.shape[1] >= 1 and H >= 1 and H % k.shape[1] == 0):
         raise ValueError(f"{name}: need q [B, H, Lq, D], k and v [B, Hk, Lk, D], D 64 or 128, H a multiple of Hk")
     for t in (q, k, v):
-        if t.stride(3) != 1 or any(s % 8 for s in K._strides_bhl(t)) or t.data_ptr() % 16 or K._strides_bhl(t)[2] > 1 << 23:
+        b, h, row = K._strides_bhl(t)
+        if t.stride(3) != 1 or (b | h | row) % 8 or t.data_ptr() % 16 or row > 1 << 23:
             raise ValueError(f"{name}: operands need a contiguous last dim, strides that are multiples of 8 (rows: at most 2^23) and 16-byte alignment")
     if max(q.shape[2], k.shape[2]) > 1 << 28:
         raise ValueError(f"{name}: at most 2^28 rows")
@@ -313,6 +321,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     if any(t is not None and t.device != q.device for t in (k, v, table, key_mask, offsets)):
         raise ValueError(f"{name}: all operands must be on one device")
     scale = D ** -0.5 if scale is None else float(scale)
+    if not _records(q, k, v, table):
+        return K.rel_attn_fwd(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset, False)[0]
     how = {"max_distance": max_distance, "bidirectional": bool(bidirectional), "scale": scale, "causal": bool(causal),
            "q_offset": 0 if offsets is not None else q_offset}
     return _RelativeAttention.apply(q, k, v, table, key_mask, offsets, how)

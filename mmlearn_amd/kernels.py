@@ -1309,7 +1309,7 @@ def attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tenso
 # ------------------------------------------------------------------ per-head norm of queries and keys with the position rotation
 def _strides_blh(t: torch.Tensor):
     """Element strides {batch, token, head} of a [B, L, H, D] view."""
-    return (C.c_int64 * 3)(t.stride(0), t.stride(1), t.stride(2))
+    return (C.c_int64 * 3)(*t.stride()[:3])
 
 
 def _qk_norm_operands(q, qw, kw, table, positions):
@@ -1377,15 +1377,16 @@ _REL_MASKS = {(1, torch.int32): 1, (1, torch.int64): 2, (2, torch.bool): 3, (2, 
 
 def _strides_bhl(t: torch.Tensor):
     """Element strides {batch, head, row}; a dim of one entry is never stepped over."""
-    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+    B, H, L, _ = t.shape
+    b, h, row, _ = t.stride()
+    return b if B > 1 else 0, h if H > 1 else 0, row if L > 1 else 0
 
 
 def _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset) -> _lib.RelAttn:
     p = _lib.RelAttn()
     B, H, Lq, D = q.shape
     p.q, p.k, p.v, p.table, p.mask = ptr(q), ptr(k), ptr(v), ptr(table), ptr(key_mask)
-    for n, t in (("q_strides", q), ("k_strides", k), ("v_strides", v)):
-        getattr(p, n)[:] = _strides_bhl(t)
+    p.q_strides[:], p.k_strides[:], p.v_strides[:] = _strides_bhl(q), _strides_bhl(k), _strides_bhl(v)
     p.B, p.H, p.Hk, p.Lq, p.Lk, p.D = B, H, k.shape[1], Lq, k.shape[2], D
     p.dtype, p.table_dtype = dtype_tag(q.dtype), dtype_tag(table.dtype)
     if key_mask is not None:
