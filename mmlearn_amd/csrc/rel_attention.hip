@@ -592,17 +592,19 @@ __device__ __forceinline__ void rel_diagonals(const f32x16& s, float (&d)[3]) {
 }
 
 // As the forward, with the query on the lane: dS^T needs lse and delta of the lane alone, and dQ^T += K^T dS^T takes it from the
-// accumulators.  dtable: rel_diagonals sums a near tile along its diagonals in registers, and each group of lanes adds the sums to a
-// vector over the distances of its own (an address is one lane's: plain LDS reads and writes in a fixed order; LDS float atomics
-// took 175 cycles a wave instruction, which made this kernel 3.5 times slower).  Tiles beyond max_distance add to two registers.
-constexpr int rel_diag_vectors(int D) { return D == 64 ? 16 : 8; }
+// accumulators.  dtable: rel_diagonals sums a near tile along its diagonals in registers, and each half wave adds the sums to a
+// vector over the distances of its own (plain LDS reads and writes in a fixed order; LDS float atomics took 175 cycles a wave
+// instruction, which made this kernel 3.5 times slower).  Tiles beyond max_distance add to two registers.
+// D = 64 leaves room for three workgroups a CU, in registers and in LDS (16 documents of 512 rows, 12 heads: 41 us instead of 57
+// with two, the dK / dV kernel below 45 instead of 61).
+constexpr int REL_DIAG = 8;   // vectors over the distances
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, EXT = 96, VECS = rel_diag_vectors(D);
+  constexpr int CB = D / 64, STAGE = 2 * CB * 8192, EXT = 96, VECS = REL_DIAG;
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int nbias = (2 * (a.far + EXT) + 1 + 3) & ~3;
-  float* diag = bias + nbias;   // [VECS][nbias]: per group of 16 lanes, at D = 128 per wave half (two workgroups then fit a CU's LDS)
+  float* diag = bias + nbias;   // [VECS][nbias], per half wave
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
   const int nqb = (a.Lq + 127) / 128, item = rel_item(blockIdx.x, gridDim.x);
@@ -653,7 +655,7 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelArgs a) {
   rel_bias_fill<T>(a, bias, EXT, h, tid, 256);
   if (a.dtab_part)
     for (int x = tid; x < VECS * nbias; x += 256) diag[x] = 0.f;
-  float* my_diag = diag + (VECS == 16 ? tid >> 4 : tid >> 5) * nbias + 4 * hf - r;
+  float* my_diag = diag + (tid >> 5) * nbias + 4 * hf - r;
   const RelLane il(lane);
   const int ip = i + off;
   for (int kt = 0; kt < nkt; ++kt) {
@@ -714,17 +716,11 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelArgs a) {
           float d[3];
           rel_diagonals(s, d);
           float* at = my_diag + (a.far + EXT + jt - (i_wave + off));   // (r = 16 R + c)
-          if (VECS == 16) {
+          // the upper 16 lanes of a half stand where the lower ones were one k before: one after the other (LDS keeps a wave's order)
 #pragma unroll
-            for (int k = 0; k < 3; ++k) d[k] += at[16 * k];
-#pragma unroll
-            for (int k = 0; k < 3; ++k) at[16 * k] = d[k];
-          } else {   // the upper 16 lanes of a half stand where the lower ones were one k before: one after the other (LDS keeps a wave's order)
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-              at[16 * k] += d[k];
-              asm volatile("" ::: "memory");
-            }
+          for (int k = 0; k < 3; ++k) {
+            at[16 * k] += d[k];
+            asm volatile("" ::: "memory");
           }
         }
       }
@@ -799,7 +795,7 @@ __global__ __launch_bounds__(256) void rel_dtable_kernel(const float* part, W* d
 // and dV^T of the group in its accumulators.  With few key blocks (few key heads) or unequal ones (causal: the first keys see all rows, the
 // last few) the walk is divided among `dkv_splits` workgroups, whose f32 sums rel_dkv_join_kernel adds in order.
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void rel_dkv_kernel(const RelArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int CB = D / 64, STAGE = 2 * CB * 8192 + 512, KB = 128, EXT = 96;
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
@@ -1090,8 +1086,8 @@ static int rel_backward(const mmk_rel_attn* p, RelArgs& a, void* dtable, hipStre
   if (a.Lq > 0) {
     constexpr int EXT = 96;
     if (int rc = rel_launch(rel_dq_kernel<T, D>, MMK_K_REL_ATTN_BWD, (int64_t)a.B * a.H * nqb,
-                            TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 1 + rel_diag_vectors(D) : 1),
-                            TILES + (1 + rel_diag_vectors(D)) * rel_vec_bytes(REL_MAX_FAR, EXT), a, st))
+                            TILES + rel_vec_bytes(a.far, EXT) * (a.dtab_part ? 1 + REL_DIAG : 1),
+                            TILES + (1 + REL_DIAG) * rel_vec_bytes(REL_MAX_FAR, EXT), a, st))
       return rc;
   }
   if (a.Lk > 0) {
