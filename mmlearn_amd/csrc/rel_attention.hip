@@ -163,16 +163,22 @@ __device__ __forceinline__ int rel_mask_at(const RelArgs& a, int b, int j) {
   return reinterpret_cast<const int64_t*>(a.mask)[at] != 0;
 }
 
-// blockIdx -> work item, so that neighbouring items (the query blocks of one head) run on one XCD and share its L2
-__device__ __forceinline__ int rel_item(int id, int total) {
-  const int per = total >> 3;
-  return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
-}
-// which head the items of place `p` belong to: the heads of one sample are dealt to the eight XCDs in turn, because samples of unequal length
-// would otherwise load them unequally (16 x 12 x 512 x 64 with lengths from a third up: dK/dV 60 us by whole samples, 58 dealt)
-__device__ __forceinline__ int rel_head(int p, int n) {
-  const int per = n >> 3;
-  return p < per * 8 ? (p % per) * 8 + p / per : p;
+// blockIdx -> head (of all samples) and rank among its `blocks` work items.  The heads are dealt to the eight XCDs in turn (samples of unequal
+// length would load them unequally otherwise), all items of a head run on one XCD and share its L2, and there the heads go in groups of
+// eight with the first rank of every head before the second: rank 0 is the longest item of a causal call, and a long one that started
+// last would run alone at the end (causal forward of 2 x 16 x 4097 x 128: 181 us, head by head 207; 4 x 12 x 2048 x 64 and back: 204 and
+// 253).  The last heads % 8 heads are spread over all XCDs, item by item.
+struct RelPlace {
+  int head, rank;
+};
+__device__ __forceinline__ RelPlace rel_place(int id, int blocks, int heads) {
+  const int per = heads >> 3, whole = per * 8 * blocks;
+  if (id >= whole) {
+    const int rest = heads & 7, x = id - whole;
+    return {per * 8 + x % rest, x / rest};
+  }
+  const int x = id >> 3, group = x / (8 * blocks), size = min(8, per - 8 * group), in = x - group * 8 * blocks;
+  return {(8 * group + in % size) * 8 + (id & 7), in / size};
 }
 
 // One wave's share of a 64-row tile in LDS: CB column blocks of 64 of X, then of Y; of each image's 8 pieces of 8 rows, pieces `wave` and
@@ -248,9 +254,10 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
-  const int nqb = (a.Lq + 127) / 128, item = rel_item(blockIdx.x, gridDim.x);
-  const int place = item / nqb, bh = rel_head(place, a.B * a.H), b = bh / a.H, h = bh - b * a.H;
-  const int qb = a.causal ? nqb - 1 - (item - place * nqb) : item - place * nqb;   // causal: the longest rows first
+  const int nqb = (a.Lq + 127) / 128;
+  const RelPlace pl = rel_place(blockIdx.x, nqb, a.B * a.H);
+  const int bh = pl.head, b = bh / a.H, h = bh - b * a.H;
+  const int qb = a.causal ? nqb - 1 - pl.rank : pl.rank;   // causal: the longest rows first
   const int off = rel_offset(a, b), klen = rel_key_len(a, b);
   const int i_wg = qb * 128, i_wave = i_wg + 32 * wave, i = i_wave + r;
   int nkt = (klen + 63) / 64;
@@ -607,9 +614,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelA
   float* diag = bias + nbias;   // [VECS][nbias], per half wave
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
-  const int nqb = (a.Lq + 127) / 128, item = rel_item(blockIdx.x, gridDim.x);
-  const int place = item / nqb, bh = rel_head(place, a.B * a.H), b = bh / a.H, h = bh - b * a.H;
-  const int qb = a.causal ? nqb - 1 - (item - place * nqb) : item - place * nqb;
+  const int nqb = (a.Lq + 127) / 128;
+  const RelPlace pl = rel_place(blockIdx.x, nqb, a.B * a.H);
+  const int bh = pl.head, b = bh / a.H, h = bh - b * a.H;
+  const int qb = a.causal ? nqb - 1 - pl.rank : pl.rank;
   const int off = rel_offset(a, b), klen = rel_key_len(a, b);
   const int i_wg = qb * 128, i_wave = i_wg + 32 * wave, i = i_wave + r;
   int nkt = (klen + 63) / 64;
@@ -801,9 +809,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const Rel
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
-  const int nkb = (a.Lk + KB - 1) / KB, item = rel_item(blockIdx.x, gridDim.x), S = a.dkv_splits;
-  const int unit = item / S, split = item - unit * S;
-  const int place = unit / nkb, kb = unit - place * nkb, bk = rel_head(place, a.B * a.Hk), b = bk / a.Hk, hk = bk - b * a.Hk;
+  const int nkb = (a.Lk + KB - 1) / KB, S = a.dkv_splits;
+  const RelPlace pl = rel_place(blockIdx.x, nkb * S, a.B * a.Hk);
+  const int kb = pl.rank / S, split = pl.rank - kb * S, b = pl.head / a.Hk, hk = pl.head - b * a.Hk;
   const int off = rel_offset(a, b), klen = rel_key_len(a, b);
   const int j_wg = kb * KB, j_wave = j_wg + 32 * wave, j = j_wave + r;
   const bool kept = j < klen && rel_mask_at(a, b, j);
