@@ -572,15 +572,15 @@ int mmk_qk_norm_rotary_bwd(const void* q, const void* k, const void* qw, const v
  * mmlearn/modules/encoders/text.py:20-178; those with relative_attention_bias materialise [1, H, Lq, Lk] for it):
  *   out = softmax(scale * q k^T + table[bucket(j - i - q_offset), h]) v  over the keys j that the mask (and with `causal`, j <= i + q_offset)
  * keeps; a row without keys gives zeros.  q [B, H, Lq, D], k / v [B, Hk, Lk, D] (H a multiple of Hk): bf16 / f16 views by element strides
- * {batch, head, row}, multiples of 8, 16-byte aligned; D 64 or 128.  out [B, Lq, H, D] contiguous; lse f32 [B, H, Lq] (base 2; NULL: not
- * wanted) feeds the backward.
+ * {batch, head, row}, multiples of 8, 16-byte aligned; D 64 or 128.  out [B, Lq, H, D] contiguous; out_lo (like out: what its rounding
+ * left) and lse f32 [B, H, Lq] (base 2) feed the backward; NULL both where there is none.
  * Buckets: with bidirectional, distances j - i > 0 use the second half of them; else positive distances count as 0.  Within a side the
  * first near_buckets hold one distance each, the next n_borders + 1 begin at near_buckets, borders[0], borders[1], .. (HOST memory,
  * ascending); all distances from max_distance (1 .. 512) on fall into one bucket.  table: [buckets][H], f32 or the operands' type.
  * mask: one of MMK_REL_MASK_* -- LEN: int [B] leading keys are kept; 8 / 32 / 64: [B, Lk] integers of that width with batch stride
  * mask_stride, nonzero = kept.  Masked keys and values may hold anything.  q_offsets (int32 [B], device) overrides q_offset.
  * ws: mmk_rel_attn_fwd_ws_floats() floats.
- * Backward: out / dout [B, Lq, H, D] contiguous; dq / dk / dv contiguous [B, L, heads, D]; dtable [buckets][H] in table_dtype, NULL: not
+ * Backward: out / out_lo / dout [B, Lq, H, D] contiguous; dq / dk / dv contiguous [B, L, heads, D]; dtable [buckets][H] in table_dtype, NULL: not
  * wanted; ws: mmk_rel_attn_bwd_ws_floats() floats.  All sums in a fixed order. */
 #define MMK_REL_MASK_NONE 0
 #define MMK_REL_MASK_LEN32 1
@@ -604,10 +604,10 @@ typedef struct {
   int32_t pad;
 } mmk_rel_attn;
 int64_t mmk_rel_attn_fwd_ws_floats(const mmk_rel_attn* p);
-int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, float* lse, float* ws, void* stream);
+int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, void* out_lo, float* lse, float* ws, void* stream);
 int64_t mmk_rel_attn_bwd_ws_floats(const mmk_rel_attn* p, int want_dtable);
-int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dtable,
-                     float* ws, void* stream);
+int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const void* out_lo, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                     void* dtable, float* ws, void* stream);
 
 /* Orthogonalised update of `count` matrices [rows, cols] of one shape by a quintic Newton-Schulz iteration (the step of a Muon-type
  * optimizer; beside mmk_adamw_update, which serves TrainingTask.configure_optimizers, mmlearn/tasks/base.py:72-155):

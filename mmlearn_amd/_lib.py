@@ -190,9 +190,9 @@ _SIGNATURES.update({
     "mmk_newton_schulz_ws_bytes": [_i, _i, _i],
     "mmk_newton_schulz": [_vp, _vp, _vp],
     "mmk_rel_attn_fwd_ws_floats": [_vp],
-    "mmk_rel_attn_fwd": [_vp] * 5,
+    "mmk_rel_attn_fwd": [_vp] * 6,
     "mmk_rel_attn_bwd_ws_floats": [_vp, _i],
-    "mmk_rel_attn_bwd": [_vp] * 10,
+    "mmk_rel_attn_bwd": [_vp] * 11,
     "mmk_qk_norm_rotary_bwd": [_vp] * 5 + [_i, _vp, _i, _i64] + [_vp] * 8 + [_i] * 7 + [_vp] * 4 + [_f, _i, _i, _vp],
 })
 _STR_FUNCS = {"mmk_last_error": [], "mmk_kernel_name": [_i]}

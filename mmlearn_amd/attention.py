@@ -248,22 +248,22 @@ class _RelativeAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, key_mask, offsets, how):
         q_offset = how["q_offset"] if offsets is None else offsets
-        out, lse = K.rel_attn_fwd(q, k, v, table, how["max_distance"], how["bidirectional"], how["scale"], how["causal"], key_mask, q_offset,
-                                  any(ctx.needs_input_grad[:4]))
-        ctx.save_for_backward(q, k, v, table, key_mask, offsets, out, lse)
+        out, out_lo, lse = K.rel_attn_fwd(q, k, v, table, how["max_distance"], how["bidirectional"], how["scale"], how["causal"], key_mask, q_offset,
+                                          any(ctx.needs_input_grad[:4]))
+        ctx.save_for_backward(q, k, v, table, key_mask, offsets, out, out_lo, lse)
         ctx.how = how
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, key_mask, offsets, out, lse = ctx.saved_tensors
+        q, k, v, table, key_mask, offsets, out, out_lo, lse = ctx.saved_tensors
         how = ctx.how
         dout = dout.to(q.dtype).contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()
         grads = K.rel_attn_bwd(q, k, v, table, how["max_distance"], how["bidirectional"], how["scale"], how["causal"], key_mask,
-                               how["q_offset"] if offsets is None else offsets, out, lse, dout, ctx.needs_input_grad[3])
+                               how["q_offset"] if offsets is None else offsets, out, out_lo, lse, dout, ctx.needs_input_grad[3])
         return (*grads, None, None, None)
 
 
@@ -284,8 +284,7 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     or an int32 tensor ``[B]`` (one token against a cache: the number of keys before it).  A row that nothing is left for gives zeros and
     passes no gradient.
 
-    The table's gradient is summed in f32 from scores whose softmax correction comes from the 16-bit output, so it is as exact as a
-    16-bit gradient also for an f32 table.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive."""
+    The table's gradient is exact to about 1e-5 of its size before it is rounded to the table's type.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive."""
     K.require_gpu(q, "query")
     name = "mmlearn_amd.relative_attention"
     if not (q.dim() == k.dim() == v.dim() == 4 and q.dtype in (torch.bfloat16, torch.float16) and q.dtype == k.dtype == v.dtype):

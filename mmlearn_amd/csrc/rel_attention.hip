@@ -12,8 +12,10 @@
 // lane, so the running maximum, the sum and the rescale of O^T are lane-local, and the exponentiated accumulators are the B operand
 // of O^T = V^T P^T as they stand (csrc/attention.hip uses the same forms for whole heads on chip; attn_image.h has the images).  K / V (or
 // Q / dO) tiles of 64 rows go to LDS by LDS-DMA, double-buffered, one barrier a tile.  P and dS are rounded to the operands' type for their
-// products -- the matrix unit takes 16-bit operands; statistics, sums, accumulators and the table's gradient stay in f32, and
-// delta is formed from the rounded o, as everything the backward knows of o.
+// products -- the matrix unit takes 16-bit operands; statistics, sums, accumulators and the table's gradient stay in f32.
+// delta decides how exact the table's gradient is: dS sums to zero along a row, and an error of delta is one of every dS of the row.  With
+// o rounded (or summed from rounded P) dtable is off by 4e-3 at 512 keys, an f32 one too.  So a forward that will be differentiated sums
+// o from P in two parts, rounded and the rest, and hands the backward what the rounding of o left: delta and dtable then hold to 1e-5.
 #include <hip/hip_ext.h>
 #include <limits.h>
 
@@ -37,6 +39,7 @@ struct RelArgs {
   const void *q, *k, *v;
   int64_t q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;   // element strides of [B, H, L, D] views
   void* out;       // [B, Lq, H, D] contiguous
+  void* out_lo;    // the same layout: what out's rounding left, for the backward; null: not wanted
   float* lse;      // [B, H, Lq], base 2 of the biased scores; +inf for a row without keys; may be null
   int B, H, Hk, G, Lq, Lk;   // G = H / Hk query heads share a key head
   float scale, sl2;          // sl2 = scale log2 e
@@ -49,7 +52,7 @@ struct RelArgs {
   int mask_kind;             // MMK_REL_MASK_*
   // backward
   const void* dout;          // [B, Lq, H, D] contiguous
-  const void* o;
+  const void *o, *o_lo;
   void *dq, *dk, *dv;        // contiguous [B, L, heads, D]
   float *delta, *dtab_part;  // [B, H, Lq]; [workgroups of the dQ kernel][buckets] or null
   float* dkv_part;           // [splits][dK, dV][B, Lk, Hk, D]
@@ -101,6 +104,16 @@ __device__ __forceinline__ s16x8 rel_operand(const f32x16& x, int s) {
   t8 o;
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = from_f32<T>(x[8 * s + e]);
+  return __builtin_bit_cast(s16x8, o);
+}
+// what rel_operand's rounding left
+template <typename T>
+__device__ __forceinline__ s16x8 rel_operand_rest(const f32x16& x, int s, s16x8 rounded) {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  const t8 hi = __builtin_bit_cast(t8, rounded);
+  t8 o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = from_f32<T>(x[8 * s + e] - to_f32(hi[e]));
   return __builtin_bit_cast(s16x8, o);
 }
 __device__ __forceinline__ f32x16 rel_zero() {
@@ -228,26 +241,69 @@ __device__ __forceinline__ void rel_zero_rows(char* img, uint64_t word, int wave
   }
 }
 
-// D^T accumulators (lane = row, registers = columns) -> row `row` of a contiguous-row tensor
+// a of the lower half's lanes and b of the upper half's stay; the other halves change places
+__device__ __forceinline__ void rel_swap_halves(uint32_t& a, uint32_t& b) {
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  const u2 r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+// D^T accumulators (lane = row, registers = columns) -> row `row` of a contiguous-row tensor, times mul; `rest`, if given, takes what the
+// rounding left.  A lane holds four of each eight columns; the halves trade, so that each lane stores 16 bytes.
 template <typename T, int D>
-__device__ __forceinline__ void rel_store_row(T* row, const f32x16 (&o)[D / 32], float mul, int h) {
+__device__ __forceinline__ void rel_store_row(T* row, T* rest, const f32x16 (&o)[D / 32], float mul, int h) {
   typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      t4 w;
+    for (int g = 0; g < 4; g += 2) {
+      t4 hi[2], lo[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(o[dt][4 * g + e] * mul);
-      *reinterpret_cast<t4*>(row + 32 * dt + 8 * g + 4 * h) = w;
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = o[dt][4 * (g + u) + e] * mul;
+          hi[u][e] = from_f32<T>(x);
+          lo[u][e] = from_f32<T>(x - to_f32(hi[u][e]));
+        }
+      auto put = [&](T* to, t4 x, t4 y) {
+        uint2 a = __builtin_bit_cast(uint2, x), b = __builtin_bit_cast(uint2, y);
+        rel_swap_halves(a.x, b.x);
+        rel_swap_halves(a.y, b.y);
+        *reinterpret_cast<uint4*>(to + 32 * dt + 8 * (g + h)) = make_uint4(a.x, a.y, b.x, b.y);
+      };
+      put(row, hi[0], hi[1]);
+      if (rest) put(rest, lo[0], lo[1]);
     }
+}
+template <int D>
+__device__ __forceinline__ void rel_store_row(float* row, const f32x16 (&o)[D / 32], int h) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(row + 32 * dt + 8 * g + 4 * h) = make_float4(o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]);
+}
+// four values of the output, and what their rounding left
+template <typename T>
+__device__ __forceinline__ void rel_store_out(const RelArgs& a, int64_t at, float4 v) {
+  const float x[4] = {v.x, v.y, v.z, v.w};
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = from_f32<T>(x[e]);
+    lo[e] = from_f32<T>(x[e] - to_f32(hi[e]));
+  }
+  *reinterpret_cast<t4*>(reinterpret_cast<T*>(a.out) + at) = hi;
+  if (a.out_lo) *reinterpret_cast<t4*>(reinterpret_cast<T*>(a.out_lo) + at) = lo;
 }
 
 // ------------------------------------------------------------------------------------------------ forward
 // Workgroup: 4 waves x 32 queries of one (sample, head); tiles of 64 keys.  (64 queries a wave would halve the LDS reads, but the vector
 // unit -- exponential, bias, maximum, sum: twice the cycles of the products at D = 64 -- bounds it and finer workgroups fill the chip better:
 // 4 x 12 x 512 x 64 20 us with 32 and 23 with 64, 2 x 12 x 8192 x 64 503 and 498.)
-template <typename T, int D>
+template <typename T, int D, bool LO>
 __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int CB = D / 64, STAGE = 2 * CB * 8192, EXT = 96;
@@ -364,13 +420,20 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
       const s16x8 pf = rel_operand<T>(s[st >> 1], st & 1);
+      s16x8 pl;
+      if (LO) pl = rel_operand_rest<T>(s[st >> 1], st & 1, pf);
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_mfma<T>(rel_tr_frag(V + (dt >> 1) * 8192, il, st * 2048, dt & 1), pf, o[dt]);
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const s16x8 vf = rel_tr_frag(V + (dt >> 1) * 8192, il, st * 2048, dt & 1);
+        o[dt] = rel_mfma<T>(vf, pf, o[dt]);
+        if (LO) o[dt] = rel_mfma<T>(vf, pl, o[dt]);
+      }
     }
   }
   const float sum = l + rel_other_half(l);
   if (i < a.Lq) {
-    rel_store_row<T, D>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + h) * D, o, sum > 0.f ? 1.f / sum : sum, hf);
+    const int64_t row = (((int64_t)b * a.Lq + i) * a.H + h) * D;
+    rel_store_row<T, D>(reinterpret_cast<T*>(a.out) + row, LO ? reinterpret_cast<T*>(a.out_lo) + row : nullptr, o, sum > 0.f ? 1.f / sum : sum, hf);
     if (a.lse && hf == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : m + log2f(sum);
   }
 }
@@ -487,6 +550,11 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
       const s16x8 pf = rel_operand<T>(s, st);
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_mfma<T>(rel_tr_frag(V + (dt >> 1) * IMG, il, st * 2048, dt & 1), pf, o[dt]);
+      if (a.out_lo) {
+        const s16x8 pl = rel_operand_rest<T>(s, st, pf);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_mfma<T>(rel_tr_frag(V + (dt >> 1) * IMG, il, st * 2048, dt & 1), pl, o[dt]);
+      }
     }
   }
   l += rel_other_half(l);
@@ -531,8 +599,7 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
     } else {
       const int ro = blk * 32 + rr, go = ro / a.Lq, io = ro - go * a.Lq, ho = hk * a.G + go;
       const float f = ll > 0.f ? 1.f / ll : ll;
-      Vec4<T>::store(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Lq + io) * a.H + ho) * D + d,
-                     make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+      rel_store_out<T>(a, (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
       if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm + log2f(ll);
     }
   }
@@ -563,7 +630,7 @@ __global__ __launch_bounds__(256) void rel_join_kernel(const RelArgs a) {
     acc.w += f * v4.w;
   }
   const float f = ll > 0.f ? 1.f / ll : ll;
-  Vec4<T>::store(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+  rel_store_out<T>(a, (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
   if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm + log2f(ll);
 }
 
@@ -644,14 +711,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelA
     const int64_t orow = (((int64_t)b * a.Lq + ic) * a.H + h) * D + 8 * hf;
     const T* gp = reinterpret_cast<const T*>(a.dout) + orow;
     const T* op = reinterpret_cast<const T*>(a.o) + orow;
+    const T* lp = reinterpret_cast<const T*>(a.o_lo) + orow;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       typedef T t8 __attribute__((ext_vector_type(8)));
       qf[kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
       gf[kk] = *reinterpret_cast<const s16x8*>(gp + 16 * kk);
-      const t8 g8 = __builtin_bit_cast(t8, gf[kk]), o8 = *reinterpret_cast<const t8*>(op + 16 * kk);
+      const t8 g8 = __builtin_bit_cast(t8, gf[kk]), o8 = *reinterpret_cast<const t8*>(op + 16 * kk), l8 = *reinterpret_cast<const t8*>(lp + 16 * kk);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf(to_f32(g8[e]), to_f32(o8[e]), delta);
+      for (int e = 0; e < 8; ++e) delta = fmaf(to_f32(g8[e]), to_f32(o8[e]) + to_f32(l8[e]), delta);
     }
     delta += rel_other_half(delta);
     const int64_t at = ((int64_t)b * a.H + h) * a.Lq + ic;
@@ -740,7 +808,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelA
       }
     }
   }
-  if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, dq, a.scale, hf);
+  if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, nullptr, dq, a.scale, hf);
   if (!a.dtab_part) return;
   // ---- this workgroup's sums by bucket: the far sums join their wave's vectors at its ends, the vectors are added in order, and
   // a thread per (bucket, slice) collects its distances
@@ -944,12 +1012,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const Rel
       for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = rel_zero();
     }
     if (S == 1) {
-      rel_store_row<T, D>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, hf);
-      rel_store_row<T, D>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, hf);
+      rel_store_row<T, D>(reinterpret_cast<T*>(a.dk) + at, nullptr, dk, a.scale, hf);
+      rel_store_row<T, D>(reinterpret_cast<T*>(a.dv) + at, nullptr, dv, 1.f, hf);
     } else {
       const int64_t n = (int64_t)a.B * a.Lk * a.Hk * D;
-      rel_store_row<float, D>(a.dkv_part + 2 * split * n + at, dk, 1.f, hf);
-      rel_store_row<float, D>(a.dkv_part + (2 * split + 1) * n + at, dv, 1.f, hf);
+      rel_store_row<D>(a.dkv_part + 2 * split * n + at, dk, hf);
+      rel_store_row<D>(a.dkv_part + (2 * split + 1) * n + at, dv, hf);
     }
   }
 }
@@ -1084,7 +1152,8 @@ static int rel_forward(const mmk_rel_attn* p, RelArgs& a, hipStream_t st) {
   }
   constexpr int EXT = 96, TILES = 2 * 2 * (D / 64) * 8192;
   const int64_t grid = (int64_t)a.B * a.H * ((a.Lq + 127) / 128);
-  return rel_launch(rel_fwd_kernel<T, D>, MMK_K_REL_ATTN_FWD, grid, TILES + rel_vec_bytes(a.far, EXT), TILES + rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
+  return rel_launch(a.out_lo ? rel_fwd_kernel<T, D, true> : rel_fwd_kernel<T, D, false>, MMK_K_REL_ATTN_FWD, grid, TILES + rel_vec_bytes(a.far, EXT),
+                    TILES + rel_vec_bytes(REL_MAX_FAR, EXT), a, st);
 }
 
 template <typename T, int D>
@@ -1139,13 +1208,14 @@ int64_t mmk_rel_attn_fwd_ws_floats(const mmk_rel_attn* p) {
   return s == 1 ? 0 : (int64_t)p->B * p->Hk * 32 * s * (p->D + 4);
 }
 
-int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, float* lse, float* ws, void* stream) {
+int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, void* out_lo, float* lse, float* ws, void* stream) {
   if (int rc = rel_check(p)) return rc;
   if ((int64_t)p->B * p->Lq == 0) return 0;
   MMK_REQUIRE(p->q && out && (p->Lk == 0 || (p->k && p->v)) && p->table, "missing operand");
   MMK_REQUIRE(mmk_rel_attn_fwd_ws_floats(p) == 0 || ws, "missing workspace");
   RelArgs a = rel_args(p);
   a.out = out;
+  a.out_lo = out_lo;
   a.lse = lse;
   a.part = ws;
   return rel_dispatch(p, [&](auto t, auto d) { return rel_forward<decltype(t), decltype(d)::value>(p, a, (hipStream_t)stream); });
@@ -1156,17 +1226,18 @@ int64_t mmk_rel_attn_bwd_ws_floats(const mmk_rel_attn* p, int want_dtable) {
   return rel_dkv_floats(p) + (int64_t)p->B * p->H * p->Lq + (want_dtable ? (int64_t)p->B * p->H * rel_dq_blocks(p) * p->buckets : 0);
 }
 
-int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dtable,
-                     float* ws, void* stream) {
+int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const void* out_lo, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                     void* dtable, float* ws, void* stream) {
   if (int rc = rel_check(p)) return rc;
   MMK_REQUIRE(p->Lk == 0 || (dk && dv), "missing operand");
-  MMK_REQUIRE(p->Lq == 0 || (p->q && out && lse && dout && dq && ws && p->table), "missing operand");
+  MMK_REQUIRE(p->Lq == 0 || (p->q && out && out_lo && lse && dout && dq && ws && p->table), "missing operand");
   if (p->B == 0) {
     if (!dtable) return 0;
     MMK_REQUIRE(false, "the table's gradient of no samples is the caller's zero");
   }
   RelArgs a = rel_args(p);
   a.o = out;
+  a.o_lo = out_lo;
   a.lse = const_cast<float*>(lse);
   a.dout = dout;
   a.dq = dq;

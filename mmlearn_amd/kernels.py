@@ -1405,23 +1405,25 @@ def _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_ma
 
 
 def rel_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int, bidirectional: bool, scale: float,
-                 causal: bool, key_mask: Optional[torch.Tensor], q_offset, want_lse: bool):
-    """q [B, H, Lq, D], k / v [B, Hk, Lk, D] views -> (out [B, Lq, H, D] contiguous, lse f32 [B, H, Lq] or None).  csrc/rel_attention.hip."""
+                 causal: bool, key_mask: Optional[torch.Tensor], q_offset, for_backward: bool):
+    """q [B, H, Lq, D], k / v [B, Hk, Lk, D] views -> out [B, Lq, H, D] contiguous and, for the backward, what its rounding left (the same
+    shape) and lse f32 [B, H, Lq], else None twice.  csrc/rel_attention.hip."""
     require_gpu(q)
     B, H, Lq, D = q.shape
     p = _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset)
     with on_device_of(q):
         out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-        lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if want_lse else None
+        out_lo = torch.empty_like(out) if for_backward else None
+        lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if for_backward else None
         n = _lib.lib().mmk_rel_attn_fwd_ws_floats(C.byref(p))
         ws = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
-        check(_lib.lib().mmk_rel_attn_fwd(C.byref(p), ptr(out), ptr(lse), ptr(ws), stream()))
-    return out, lse
+        check(_lib.lib().mmk_rel_attn_fwd(C.byref(p), ptr(out), ptr(out_lo), ptr(lse), ptr(ws), stream()))
+    return out, out_lo, lse
 
 
 def rel_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int, bidirectional: bool, scale: float,
-                 causal: bool, key_mask: Optional[torch.Tensor], q_offset, out: torch.Tensor, lse: torch.Tensor, dout: torch.Tensor,
-                 want_dtable: bool = True):
+                 causal: bool, key_mask: Optional[torch.Tensor], q_offset, out: torch.Tensor, out_lo: torch.Tensor, lse: torch.Tensor,
+                 dout: torch.Tensor, want_dtable: bool = True):
     """-> (dq, dk, dv as [B, heads, L, D] views of contiguous [B, L, heads, D] buffers, dtable or None)."""
     require_gpu(q)
     B, H, Lq, D = q.shape
@@ -1434,7 +1436,8 @@ def rel_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch
         dtable = None if not want_dtable else torch.empty_like(table) if B else torch.zeros_like(table)
         if B:
             ws = torch.empty(max(1, _lib.lib().mmk_rel_attn_bwd_ws_floats(C.byref(p), int(want_dtable))), dtype=torch.float32, device=q.device)
-            check(_lib.lib().mmk_rel_attn_bwd(C.byref(p), ptr(out), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws), stream()))
+            check(_lib.lib().mmk_rel_attn_bwd(C.byref(p), ptr(out), ptr(out_lo), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws),
+                                              stream()))
     return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dtable
 
 
