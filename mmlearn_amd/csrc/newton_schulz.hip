@@ -462,7 +462,7 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
 
 // ------------------------------------------------------------------------------------------------ small matrices
 // A matrix of at most 128 x 256 never leaves its CU: one workgroup of eight waves does the whole iteration (the launches alone cost 108 us
-// for 201 x 65, this 39).  X^T is held twice: in f32 in the accumulator layout of the step product (wave w: rows 32 w .. of X^T on the
+// for 201 x 65, this 34).  X^T is held twice: in f32 in the accumulator layout of the step product (wave w: rows 32 w .. of X^T on the
 // lanes, 128 columns in 4 x 16 registers), which takes a X without any rounding, and rounded to f16 in LDS (two images of 256 rows x 64
 // columns), whose rows serve B X and whose columns, read transposed, X X^T.  A and then B stand in a third place (two images of 128 x 64).
 constexpr int NS_SMALL_M = 128, NS_SMALL_N = 256, NS_SMALL_PITCH = 129;
@@ -473,7 +473,9 @@ __device__ __forceinline__ int ns_img_at(int row, int c, int image) {
   return (c >> 6) * image + row * 128 + ((((c & 63) >> 3) ^ img_swz(row)) << 4) + (c & 7) * 2;
 }
 
-template <typename T, bool MOM, bool W>
+// MB: blocks of 32 that hold anything of the short side (at least two): the rest is zero and not computed.  The k steps of a product are unrolled,
+// so that their fragments are in flight together (201 x 65 34 us, with four blocks 39; 64 x 256 29 and 40).
+template <typename T, bool MOM, bool W, int MB>
 __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const NsPtrs p, int steps) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* X = smem;
@@ -484,7 +486,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
   const T* src = reinterpret_cast<const T*>(p.src[mat]);
   float* mom = MOM ? reinterpret_cast<float*>(p.mom[mat]) : nullptr;
   const int halves = a.n > 128 ? 2 : 1;
-  f32x16 x[4];
+  f32x16 x[MB];
   double sum = 0.0;
   // ---- G in halves of 128 rows j of X^T, read along the axis that is contiguous in memory
   const bool by_i = a.tall ? a.cs <= a.rs : a.rs <= a.cs;
@@ -510,7 +512,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
     __syncthreads();
     if (wave >> 2 == half) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < MB; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           x[b][e] = half < halves ? stage[(32 * (wave & 3) + r) * NS_SMALL_PITCH + 32 * b + (e & 3) + 8 * (e >> 2) + 4 * hf] : 0.f;
@@ -526,12 +528,12 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
   }
   const float scale = (float)(1.0 / (sqrt(red[0]) + (double)a.eps)) * a.S;   // (the product with S is exact)
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
+  for (int b = 0; b < MB; ++b)
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[b][e] *= scale;
   auto store_x = [&]() {
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int b = 0; b < MB; ++b)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         f16x4 o;
@@ -544,64 +546,80 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
   const ImgLane il = img_lane(lane);
   const int bi = wave >> 1, bc = 2 * (wave & 1);   // this wave's blocks of A: rows 32 bi .., columns 32 bc .. + 63
   const int k16 = (a.n + 15) / 16;
+  const bool mine = bi < MB && bc < MB;   // (with three blocks a wave's second one may be the fourth: what it computes is not read)
   auto zero = [](f32x16& z) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) z[e] = 0.f;
   };
   for (int s = 0; s < steps; ++s) {
     __syncthreads();   // X is complete; nobody reads B any more
-    f32x16 acc[4];
+    f32x16 acc[MB];
     zero(acc[0]);
     zero(acc[1]);
-    for (int k = 0; k < k16; ++k) {
+    auto contract = [&](int k) {
       const f16x8 fp = __builtin_bit_cast(f16x8, lds_tr_frag(X + (bi >> 1) * 32768, il, k * 2048, bi & 1));
 #pragma unroll
       for (int y = 0; y < 2; ++y)
         acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp, __builtin_bit_cast(f16x8, lds_tr_frag(X + (bc >> 1) * 32768, il, k * 2048, y)), acc[y], 0, 0, 0);
+    };
+    if (mine) {
+      int k = 0;
+      for (; k + 4 <= k16; k += 4) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) contract(k + u);
+      }
+      for (; k < k16; ++k) contract(k);
     }
     // element (i, i') of the symmetric result stands in row i' (the lane) at columns i (four registers): its mirror image
     f16x4 av[2][4];
+    if (mine) {
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+        for (int g = 0; g < 4; ++g) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) av[y][g][e] = (f16_t)(acc[y][4 * g + e] * a.inv_S);
-        *reinterpret_cast<f16x4*>(A + ns_img_at(32 * (bc + y) + r, 32 * bi + 8 * g + 4 * hf, 16384)) = av[y][g];
-      }
+          for (int e = 0; e < 4; ++e) av[y][g][e] = (f16_t)(acc[y][4 * g + e] * a.inv_S);
+          *reinterpret_cast<f16x4*>(A + ns_img_at(32 * (bc + y) + r, 32 * bi + 8 * g + 4 * hf, 16384)) = av[y][g];
+        }
+    }
     __syncthreads();
     zero(acc[0]);
     zero(acc[1]);
+    if (mine) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const f16x8 fp = *reinterpret_cast<const f16x8*>(A + (k >> 2) * 16384 + bi * 4096 + il.row[k & 3]);
+      for (int k = 0; k < 2 * MB; ++k) {
+        const f16x8 fp = *reinterpret_cast<const f16x8*>(A + (k >> 2) * 16384 + bi * 4096 + il.row[k & 3]);
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
-        acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp, *reinterpret_cast<const f16x8*>(A + (k >> 2) * 16384 + (bc + y) * 4096 + il.row[k & 3]), acc[y], 0, 0, 0);
+        for (int y = 0; y < 2; ++y)
+          acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp, *reinterpret_cast<const f16x8*>(A + (k >> 2) * 16384 + (bc + y) * 4096 + il.row[k & 3]), acc[y],
+                                                          0, 0, 0);
+      }
     }
     __syncthreads();   // all of A is read
+    if (mine) {
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f16x4 o;
+        for (int g = 0; g < 4; ++g) {
+          f16x4 o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (f16_t)fmaf(a.cb, (float)av[y][g][e], acc[y][4 * g + e] * (a.cc * a.inv_S));
-        *reinterpret_cast<f16x4*>(A + ns_img_at(32 * (bc + y) + r, 32 * bi + 8 * g + 4 * hf, 16384)) = o;
-      }
+          for (int e = 0; e < 4; ++e) o[e] = (f16_t)fmaf(a.cb, (float)av[y][g][e], acc[y][4 * g + e] * (a.cc * a.inv_S));
+          *reinterpret_cast<f16x4*>(A + ns_img_at(32 * (bc + y) + r, 32 * bi + 8 * g + 4 * hf, 16384)) = o;
+        }
+    }
     __syncthreads();
     if (32 * wave < a.n) {   // (rows past the matrix are zero and stay so)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) zero(acc[b]);
+      for (int b = 0; b < MB; ++b) zero(acc[b]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 2 * MB; ++k) {
         const f16x8 fq = *reinterpret_cast<const f16x8*>(X + (k >> 2) * 32768 + wave * 4096 + il.row[k & 3]);
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < MB; ++b)
           acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(A + (k >> 2) * 16384 + b * 4096 + il.row[k & 3]), fq, acc[b], 0, 0, 0);
       }
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < MB; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[b][e] = fmaf(a.ca, x[b][e], acc[b][e] * a.inv_S);
       if (s + 1 < steps) store_x();   // (a wave's rows are its own in this product)
@@ -613,7 +631,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
     __syncthreads();
     if (wave >> 2 == half) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < MB; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           stage[(32 * (wave & 3) + r) * NS_SMALL_PITCH + 32 * b + (e & 3) + 8 * (e >> 2) + 4 * hf] = x[b][e] * a.inv_S;
@@ -725,8 +743,8 @@ static int ns_run(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs
 }
 
 static bool ns_small(int rows, int cols) { return std::min(rows, cols) <= NS_SMALL_M && std::max(rows, cols) <= NS_SMALL_N; }
-template <typename T>
-static int ns_small_run(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, hipStream_t st) {
+template <typename T, int MB>
+static int ns_small_go(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, hipStream_t st) {
   auto go = [&](auto kern) {
     KernelSetup ks;
     if (int rc = kernel_setup(reinterpret_cast<const void*>(kern), 512, NS_SMALL_LDS, &ks)) return rc;
@@ -735,8 +753,12 @@ static int ns_small_run(const mmk_newton_schulz_args* q, const NsArgs& a, const 
     MMK_LAUNCH_CHECK();
     return 0;
   };
-  if (q->momenta) return q->weights ? go(ns_small_kernel<T, true, true>) : go(ns_small_kernel<T, true, false>);
-  return q->weights ? go(ns_small_kernel<T, false, true>) : go(ns_small_kernel<T, false, false>);
+  if (q->momenta) return q->weights ? go(ns_small_kernel<T, true, true, MB>) : go(ns_small_kernel<T, true, false, MB>);
+  return q->weights ? go(ns_small_kernel<T, false, true, MB>) : go(ns_small_kernel<T, false, false, MB>);
+}
+template <typename T>
+static int ns_small_run(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, hipStream_t st) {
+  return a.m <= 64 ? ns_small_go<T, 2>(q, a, p, count, st) : a.m <= 96 ? ns_small_go<T, 3>(q, a, p, count, st) : ns_small_go<T, 4>(q, a, p, count, st);
 }
 
 static int ns_check(int count, int rows, int cols) {
