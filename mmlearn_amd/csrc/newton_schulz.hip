@@ -253,7 +253,7 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int NW = 2 * WN, NT = 64 * NW * KG, TM = 64 * MB, TN = 64 * WN, PB = TM * 128, STAGE = PB + TN * 128, PIECES = (TM + TN) / 8 / NW;
   constexpr bool SYM = MODE == NS_XXT || MODE == NS_POLY;
-  static_assert(TM / 8 % NW == 0 && TN / 8 % NW == 0 && (!SYM || TM == TN), "pieces divide evenly; symmetric products use square tiles");
+  static_assert(KG <= 2 && TM / 8 % NW == 0 && TN / 8 % NW == 0 && (!SYM || TM == TN), "pieces divide evenly; symmetric products use square tiles");
   const int tid = threadIdx.x, lane = tid & 63, all_waves = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kg = all_waves / NW, wave = all_waves % NW;
   const int r = lane & 31, hf = lane >> 5, wm = wave / WN, wn = wave % WN;
@@ -319,10 +319,10 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
     for (int y = 0; y < 2; ++y)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
-  const int all_k = K / 64, nk = (all_k - kg + KG - 1) / KG, turns = (all_k + KG - 1) / KG;   // this group's steps kg, kg + KG ..; turns of the workgroup
+  const int nk = K / 64 / KG;   // this group's steps: kg, kg + KG ..  (sides are padded to multiples of 128)
   for (int k = 0; k < min(max(NST - 1, 1), nk); ++k) issue(k, k);
   int stage = 0;
-  for (int k = 0; k < turns; ++k) {
+  for (int k = 0; k < nk; ++k) {
     if (NST > 1 && k + NST - 2 < nk) ns_wait_loads<(NST > 1 ? NST - 2 : 0) * PIECES>();
     else ns_wait_loads<0>();   // (nothing more is requested: the last stages arrive together)
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the stage is here, and no wave still reads the one before it
@@ -338,22 +338,20 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
 #pragma unroll
       for (int x = 0; x < MB; ++x) fp[kk & 1][x] = frag(sp, MB * wm + x, kk);
     };
-    if (KG == 1 || k < nk) {   // (the last turn may have no step for the second group)
-      read(0);
+    read(0);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        if (kk < 3) read(kk + 1);
-        __builtin_amdgcn_sched_barrier(0);
+    for (int kk = 0; kk < 4; ++kk) {
+      if (kk < 3) read(kk + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int x = 0; x < MB; ++x)
+      for (int x = 0; x < MB; ++x)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk & 1][x], fq[kk & 1][y], acc[x][y], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+        for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk & 1][x], fq[kk & 1][y], acc[x][y], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (NST == 1 && k + 1 < turns) {   // the one stage is free once all waves have read it
+    if (NST == 1 && k + 1 < nk) {   // the one stage is free once all waves have read it
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (k + 1 < nk) issue(k + 1, 0);
+      issue(k + 1, 0);
     }
   }
   // ---- epilogue: pass `pass` brings the 64 columns j of wave column wn = pass to LDS, each with the tile's TM rows i along it
