@@ -1070,7 +1070,7 @@ static int rel_check(const mmk_rel_attn* p) {
   MMK_REQUIRE(p->D == 64 || p->D == 128, "head dim must be 64 or 128");
   MMK_REQUIRE(p->B >= 0 && p->H >= 1 && p->Hk >= 1 && p->H % p->Hk == 0 && p->Lq >= 0 && p->Lk >= 0, "bad sizes");
   MMK_REQUIRE(p->Lq <= (1 << 28) && p->Lk <= (1 << 28), "sequence too long");
-  MMK_REQUIRE((int64_t)p->B * p->H * (((int64_t)std::max(p->Lq, p->Lk) + 127) / 128) < (1 << 26), "too many workgroups");
+  MMK_REQUIRE((int64_t)p->B * p->H * (((int64_t)std::max(p->Lq, p->Lk) + 127) / 128) < (1 << 24), "too many rows");   // (a launch holds 2^32 threads)
   MMK_REQUIRE(p->buckets >= 1 && p->buckets <= REL_MAX_BUCKETS && p->n_borders >= 0 && p->n_borders <= REL_MAX_BORDERS, "too many buckets");
   MMK_REQUIRE(p->near_buckets >= 1 && p->max_distance >= 1 && p->max_distance <= REL_MAX_FAR, "max_distance must be 1 .. 512");
   MMK_REQUIRE((p->bidirectional ? 2 : 1) * (p->near_buckets + p->n_borders + 1) == p->buckets, "near and logarithmic buckets do not add up");

@@ -1389,7 +1389,9 @@ def _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_ma
     p.q_strides[:], p.k_strides[:], p.v_strides[:] = _strides_bhl(q), _strides_bhl(k), _strides_bhl(v)
     p.B, p.H, p.Hk, p.Lq, p.Lk, p.D = B, H, k.shape[1], Lq, k.shape[2], D
     p.dtype, p.table_dtype = dtype_tag(q.dtype), dtype_tag(table.dtype)
-    if key_mask is not None:
+    if key_mask is None or key_mask.numel() == 0:   # (no samples, or no keys)
+        p.mask = None
+    else:
         p.mask_kind = _REL_MASKS[key_mask.dim(), key_mask.dtype]
         p.mask_stride = key_mask.stride(0) if key_mask.dim() == 2 else 0
     near, borders, n_borders = relative_buckets(table.shape[0], max_distance, bidirectional)

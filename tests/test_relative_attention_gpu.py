@@ -260,6 +260,18 @@ def test_no_rows_no_keys_no_samples():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,lk,shape,dtype", [(0, 9, (0, 9), torch.bool), (0, 9, (0,), torch.int32), (3, 0, (3, 0), torch.int64), (3, 0, (3,), torch.int64)])
+def test_masks_of_nothing(B, lk, shape, dtype):
+    q, k = (torch.randn(B, n, 2, 64, device="cuda").bfloat16().transpose(1, 2).requires_grad_() for n in (5, lk))
+    table = torch.randn(8, 2, device="cuda", requires_grad=True)
+    off = torch.zeros(B, dtype=torch.int32, device="cuda")
+    out = relative_attention(q, k, k, table, key_mask=torch.zeros(shape, dtype=dtype, device="cuda"), q_offset=off)
+    assert out.shape == (B, 5, 2, 64) and not out.any()
+    for g, t in zip(torch.autograd.grad(out, (q, k, table), torch.ones_like(out)), (q, k, table)):
+        assert g.shape == t.shape and not g.any()
+
+
+@pytest.mark.gpu
 def test_rows_more_than_32_bits_apart():
     if torch.cuda.mem_get_info()[0] < 30 << 30:
         pytest.skip("needs 22 GiB of device memory")
