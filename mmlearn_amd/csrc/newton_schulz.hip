@@ -39,7 +39,6 @@ struct NsArgs {
   int rows, cols, m, n, mp, np;   // m <= n: short and long side, padded
   int tall;                       // rows > cols: X = G^T
   int flat;                       // every src is a run of rows * cols values from an aligned address
-  int dst_vec;                    // rows of the results are whole, aligned vectors of eight
   int64_t rs, cs;                 // element strides of src
   float eps, S, inv_S;
   float ca, cb, cc;
@@ -157,7 +156,20 @@ __global__ __launch_bounds__(256) void ns_reduce_kernel(const NsArgs a, const Ns
   if (threadIdx.x == 0) a.parts[mat * NS_PARTS + blockIdx.x] = sum;
 }
 
-// X^T = G^T / (|G| + eps) as xt[0] and xl, zero beyond the matrix.  64 x 64 tiles, through LDS where G is read along the other axis.
+// values at any element's address as one vector of 16 bytes
+template <typename T>
+struct NsVec {
+  static constexpr int V = 16 / sizeof(T);
+  struct __attribute__((packed, aligned(sizeof(T)))) mem {
+    T e[V];
+  };
+  static __device__ __forceinline__ mem load(const T* p) { return *reinterpret_cast<const mem*>(p); }
+  static __device__ __forceinline__ void store(T* p, const mem& m) { *reinterpret_cast<mem*>(p) = m; }
+};
+
+// X^T = G^T / (|G| + eps) as xt[0] and xl, zero beyond the matrix.  64 x 64 tiles, through LDS where G is read along the other axis.  16-bit values of a
+// unit stride are read 16 bytes a lane (3 x 1000 x 1777 bf16: 15 us, 18 one by one); f32 ones, whose lines are whole anyway, one by one (12 x
+// 2304 x 768: 31 us, 34 in vectors).
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void ns_prepare_kernel(const NsArgs a, const NsPtrs p) {
   __shared__ double red[4];
@@ -168,18 +180,40 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const NsArgs a, const N
   const int tm = a.mp / 64, j0 = 64 * (blockIdx.x / tm), i0 = 64 * (blockIdx.x % tm);
   // read along the axis that is contiguous in memory: i (the short side) or j
   const bool by_i = MOM || (a.tall ? a.cs <= a.rs : a.rs <= a.cs);
+  const bool unit = !MOM && sizeof(T) == 2 && min(a.rs, a.cs) == 1;
+  typedef NsVec<T> vec;
+  constexpr int V = vec::V, LINE = 64 / V;   // lanes of a line of the tile
   float v[16];
 #pragma unroll
-  for (int u = 0; u < 16; ++u) {
-    const int k = w + 4 * u, i = i0 + (by_i ? l : k), j = j0 + (by_i ? k : l);
-    v[u] = i < a.m && j < a.n ? (MOM ? a.u32[mat * mn + (int64_t)j * a.mp + i] : to_f32(src[ns_src_at(a, i, j)])) : 0.f;
+  for (int u = 0; u < 16; ++u) {   // unit: vector u / V, element u % V
+    const int line = unit ? tid / LINE + (u / V) * (256 / LINE) : w + 4 * u, at = unit ? tid % LINE * V : l;
+    const int i = i0 + (by_i ? at : line), j = j0 + (by_i ? line : at);
+    if (!unit) {
+      v[u] = i < a.m && j < a.n ? (MOM ? a.u32[mat * mn + (int64_t)j * a.mp + i] : to_f32(src[ns_src_at(a, i, j)])) : 0.f;
+    } else if (u % V == 0) {
+      const bool in = i < a.m && j < a.n;
+      const int left = by_i ? a.m - i : a.n - j;
+      const T* p = src + (in ? ns_src_at(a, i, j) : 0);
+      typename vec::mem x;
+      if (in && left >= V) {
+        x = vec::load(p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x.e[e] = in && e < left ? p[e] : (T)0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[u + e] = to_f32(x.e[e]);
+    }
   }
   double sq = 0.0;
   for (int k = tid; k < ns_parts(a); k += 256) sq += a.parts[mat * NS_PARTS + k];
   sq = ns_block_sum(sq, red);
   const float inv = (float)(1.0 / (sqrt(sq) + (double)a.eps));
 #pragma unroll
-  for (int u = 0; u < 16; ++u) tile[by_i ? w + 4 * u : l][by_i ? l : w + 4 * u] = v[u] * inv * a.S;
+  for (int u = 0; u < 16; ++u) {
+    const int line = unit ? tid / LINE + (u / V) * (256 / LINE) : w + 4 * u, at = unit ? tid % LINE * V + u % V : l;
+    tile[by_i ? line : at][by_i ? at : line] = v[u] * inv * a.S;
+  }
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < 4; ++u) {   // four values a lane, four rows a wave
@@ -213,11 +247,14 @@ __device__ __forceinline__ void ns_result(const NsArgs& a, void* dst, int row, i
   if (MODE == NS_WEIGHTS) {
     const float lr = a.lr_dev ? *a.lr_dev : a.lr;
     float* w = reinterpret_cast<float*>(dst) + at;
-    if (a.dst_vec) {   // (rows are whole vectors)
-      if (col >= a.cols) return;
-      const float4 lo = *reinterpret_cast<float4*>(w), hi = *reinterpret_cast<float4*>(w + 4);
-      *reinterpret_cast<float4*>(w) = make_float4(ns_weight(a, lr, lo.x, v[0]), ns_weight(a, lr, lo.y, v[1]), ns_weight(a, lr, lo.z, v[2]), ns_weight(a, lr, lo.w, v[3]));
-      *reinterpret_cast<float4*>(w + 4) = make_float4(ns_weight(a, lr, hi.x, v[4]), ns_weight(a, lr, hi.y, v[5]), ns_weight(a, lr, hi.z, v[6]), ns_weight(a, lr, hi.w, v[7]));
+    if (col + 8 <= a.cols) {
+#pragma unroll
+      for (int q = 0; q < 8; q += 4) {
+        auto x = NsVec<float>::load(w + q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.e[e] = ns_weight(a, lr, x.e[e], v[q + e]);
+        NsVec<float>::store(w + q, x);
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -225,8 +262,11 @@ __device__ __forceinline__ void ns_result(const NsArgs& a, void* dst, int row, i
     }
   } else {
     bf16_t* o = reinterpret_cast<bf16_t*>(dst) + at;
-    if (a.dst_vec) {
-      if (col < a.cols) Vec8<bf16_t>::store(o, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
+    if (col + 8 <= a.cols) {
+      NsVec<bf16_t>::mem x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x.e[e] = (bf16_t)v[e];
+      NsVec<bf16_t>::store(o, x);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -830,14 +870,12 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
   for (int at = 0; at < q->count; at += group) {
     const int n = std::min(group, q->count - at);
     NsPtrs p = {};
-    a.dst_vec = q->cols % 8 == 0;
     a.flat = (q->col_stride == 1 && q->row_stride == q->cols) || (q->row_stride == 1 && q->col_stride == q->rows);
     for (int i = 0; i < n; ++i) {
       p.src[i] = q->src[at + i];
       p.mom[i] = q->momenta ? q->momenta[at + i] : nullptr;
       p.dst[i] = q->dst[at + i];
       a.flat &= reinterpret_cast<uintptr_t>(p.src[i]) % 16 == 0;
-      a.dst_vec &= reinterpret_cast<uintptr_t>(p.dst[i]) % 16 == 0;
     }
     const int rc = small ? MMK_DISPATCH_DTYPE(q->dtype, T, [&]() -> int { return ns_small_run<T>(q, a, p, n, (hipStream_t)stream); })
                          : ns_run(q, a, p, n, wide, (hipStream_t)stream);
