@@ -106,14 +106,26 @@ __device__ __forceinline__ s16x8 rel_operand(const f32x16& x, int s) {
   for (int e = 0; e < 8; ++e) o[e] = from_f32<T>(x[8 * s + e]);
   return __builtin_bit_cast(s16x8, o);
 }
+// two neighbouring values of an operand in f32 (bf16 taken apart by hand: through conversions of single values the packed ones get lost)
+__device__ __forceinline__ float2 rel_pair(uint32_t w, bf16_t) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 rel_pair(uint32_t w, f16_t) {
+  typedef f16_t f2 __attribute__((ext_vector_type(2)));
+  const f2 v = __builtin_bit_cast(f2, w);
+  return make_float2((float)v[0], (float)v[1]);
+}
 // what rel_operand's rounding left
 template <typename T>
 __device__ __forceinline__ s16x8 rel_operand_rest(const f32x16& x, int s, s16x8 rounded) {
   typedef T t8 __attribute__((ext_vector_type(8)));
-  const t8 hi = __builtin_bit_cast(t8, rounded);
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  const u4 w = __builtin_bit_cast(u4, rounded);
   t8 o;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = from_f32<T>(x[8 * s + e] - to_f32(hi[e]));
+  for (int e = 0; e < 4; ++e) {
+    const float2 hi = rel_pair(w[e], T());
+    o[2 * e] = from_f32<T>(x[8 * s + 2 * e] - hi.x);
+    o[2 * e + 1] = from_f32<T>(x[8 * s + 2 * e + 1] - hi.y);
+  }
   return __builtin_bit_cast(s16x8, o);
 }
 __device__ __forceinline__ f32x16 rel_zero() {
@@ -305,7 +317,7 @@ __device__ __forceinline__ void rel_store_out(const RelArgs& a, int64_t at, floa
 // 4 x 12 x 512 x 64 20 us with 32 and 23 with 64, 2 x 12 x 8192 x 64 503 and 498.  At D = 128 the LDS reads take as long as the products:
 // a fragment of 1 KiB for each, four waves, 128 bytes a cycle.)  Scores of the next tile formed under the exponentials of this one, in one
 // wave: 5 to 15 % slower than two waves that do so by themselves.  2 x 16 x 4096 x 128: 295 us, 930 TFLOP/s; 2 x 12 x 8192 x 64: 512 us, 805;
-// 256 x 12 x 77 x 64: 36 us, 3.4 TB/s.  LO: P V with P in two parts, 237 us for 2 x 16 x 4097 x 128 causal, 181 without.
+// 256 x 12 x 77 x 64: 36 us, 3.4 TB/s.  LO: P V with P in two parts, 230 us for 2 x 16 x 4097 x 128 causal, 175 without.
 template <typename T, int D, bool LO>
 __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
