@@ -98,6 +98,20 @@ def test_batches_strides_and_neighbours():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("count,rows,cols", [(22, 384, 640), (40, 640, 384), (64, 1280, 100), (64, 640, 640), (3, 130, 4000)])
+def test_batches_that_fill_the_chip_differently(count, rows, cols):
+    """Few tiles, some for every CU, many, and 256 x 256 ones."""
+    x = torch.randn(count, rows, cols, generator=torch.Generator().manual_seed(count))
+    x[count // 2] *= 1e4
+    got = orthogonalize(x.cuda()).double().cpu()
+    for i in (0, count // 2, count - 1):
+        want = oracle.orthogonalize(x[i])
+        norm, most = _tolerance(x[i], want)
+        d = got[i] - want
+        assert d.norm() <= norm and d.abs().max() <= most, (i, d.norm().item() / want.norm().item())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("steps,coefficients", [(1, NS_COEFFICIENTS), (2, (1.875, -1.25, 0.375)), (8, (1.875, -1.25, 0.375)), (6, (1.5, -0.5, 0.0))])
 def test_other_iterations(steps, coefficients):
     x = torch.randn(70, 140, generator=torch.Generator().manual_seed(3))

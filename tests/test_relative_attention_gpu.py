@@ -46,6 +46,9 @@ CASES = [
     _case(1, 2, 2, 70, 70, 64, buckets=2, far=1, bidir=False),
     _case(1, 2, 2, 40, 40, 64, offset=1 << 28),
     _case(5, 2, 2, 48, 48, 64, mask="tensor of none"),
+    # more heads than go together on an XCD, and a few left over
+    _case(3, 25, 5, 130, 130, 64, causal=True),
+    _case(2, 38, 38, 40, 70, 128, "float16", mask="lengths"),
 ]
 
 
