@@ -6,9 +6,11 @@
 // tiles on and above the diagonal are computed, their mirror image is stored with them).
 //
 // Products run on v_mfma_f32_32x32x16_f16 with f32 accumulation.  f16, not bf16: all singular values stay below 1.3, so range is no
-// matter, and its 11 bits leave 1.2e-3 to 1.7e-3 in the result where bf16 operands leave 1e-2.  X itself is kept in f32: a X enters a step
+// matter, and its 11 bits leave 5e-4 in the result where bf16 operands leave 1e-2.  X itself is kept in f32: a X enters a step
 // unrounded, and only the correction B X passes through 16 bits -- with a rounded X the small singular values of a matrix with a few
-// large ones drown in the large ones' rounding, amplified 3.4 times a step (measured: 2e-2 instead of 6e-4).  The f16 copies carry a
+// large ones drown in the large ones' rounding, amplified 3.4 times a step (measured: 2e-2 instead of 6e-4).  The diagonals of A and B, which
+// come to hold nearly all of them, are kept in f32 beside the operands and enter as A^2 = E^2 + D E + E D + D^2 and B X = E X + D X (with
+// rounded diagonals the result is off by 1.5e-3 to 1.9e-3).  The f16 copies carry a
 // power of two S ~ sqrt(max side), exact, which lifts the entries of large matrices (about 1 / S) out of f16's subnormals.
 //
 // Layout: sides padded with zeros, which the iteration keeps.  X is stored transposed, [n][m], as two f16 arrays: the operand S X rounded, and
@@ -47,8 +49,10 @@ struct NsArgs {
   float* u32;      // momentum: the update before it is normalised, [np][mp] (X^T); shares its memory with xt[1] and a16
   f16_t* xt[2];    // X^T [np][mp], times S, rounded: read and written by alternate steps
   f16_t* xl;       // what the rounding left
-  f16_t* a16;      // [mp][mp], times S
-  f16_t* b16;      // [mp][mp], times S
+  f16_t* a16;      // [mp][mp], times S, the diagonal zero
+  f16_t* b16;      // [mp][mp], times S, the diagonal zero
+  float* diag_a;   // [mp] the diagonals, times S, in f32
+  float* diag_b;
   // momentum
   float mu;
   int nesterov;
@@ -294,7 +298,7 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int NW = 2 * WN, NT = 64 * NW * KG, TM = 64 * MB, TN = 64 * WN, PB = TM * 128, STAGE = PB + TN * 128, PIECES = (TM + TN) / 8 / NW;
   constexpr bool SYM = MODE == NS_XXT || MODE == NS_POLY;
-  static_assert(KG <= 2 && TM / 8 % NW == 0 && TN / 8 % NW == 0 && (!SYM || TM == TN), "pieces divide evenly; symmetric products use square tiles");
+  static_assert(KG <= 2 && NT % (TM / 8) == 0 && TM / 8 % NW == 0 && TN / 8 % NW == 0 && (!SYM || TM == TN), "pieces divide evenly; symmetric products use square tiles");
   const int tid = threadIdx.x, lane = tid & 63, all_waves = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kg = all_waves / NW, wave = all_waves % NW;
   const int r = lane & 31, hf = lane >> 5, wm = wave / WN, wn = wave % WN;
@@ -398,6 +402,12 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
   // ---- epilogue: pass `pass` brings the 64 columns j of wave column wn = pass to LDS, each with the tile's TM rows i along it
   constexpr int PITCH = TM + 4;
   float* T = reinterpret_cast<float*>(smem);   // [64 j][PITCH]
+  float d[8];   // of this thread's columns i, the same in every turn: the diagonal of A; a + that of B
+  if (MODE != NS_XXT) {
+    const float* from = (MODE == NS_POLY ? a.diag_a : a.diag_b) + (int64_t)mat * a.mp + ti * TM + 8 * (tid % (TM / 8));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] = MODE == NS_POLY ? from[e] : fmaf(from[e], a.inv_S, a.ca);
+  }
 #pragma unroll
   for (int pass = 0; pass < WN; ++pass) {
     __syncthreads();
@@ -431,24 +441,40 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
       *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(t + 4);
       if (SYM) {
         const int64_t at = mat * mm + (int64_t)j * a.mp + i;
-        f16x8 o;
-        if (MODE == NS_XXT) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = (f16_t)(v[e] * a.inv_S);
-          *reinterpret_cast<f16x8*>(a.a16 + at) = o;
-        } else {
-          const f16x8 a8 = *reinterpret_cast<const f16x8*>(a.a16 + at);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = (f16_t)fmaf(a.cb, (float)a8[e], v[e] * (a.cc * a.inv_S));
-          *reinterpret_cast<f16x8*>(a.b16 + at) = o;
+        // S A = the product / S;  S B = b S E + c ((S E)^2 + (d_i + d_j) S E) / S beside the diagonal, b d + c ((S E)^2 + d^2) / S on it
+        const float k = MODE == NS_XXT ? a.inv_S : a.cc * a.inv_S;
+        f16x8 a8, o;
+        float dj = 0.f, y[8];
+        if (MODE == NS_POLY) {
+          a8 = *reinterpret_cast<const f16x8*>(a.a16 + at);
+          dj = a.diag_a[(int64_t)mat * a.mp + j];
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = MODE == NS_XXT ? 0.f : (float)a8[e];
+          y[e] = MODE == NS_XXT ? v[e] * k : fmaf(a.cb, x, k * fmaf(d[e] + dj, x, v[e]));
+        }
+        if (ti == tj) {
+          const int own = j - i;   // which of the eight stands on the diagonal
+          float on = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            on = e == own ? v[e] : on;
+            y[e] = e == own ? 0.f : y[e];
+          }
+          on = MODE == NS_XXT ? on * k : fmaf(a.cb, dj, k * fmaf(dj, dj, on));
+          if (own >= 0 && own < 8) (MODE == NS_XXT ? a.diag_a : a.diag_b)[(int64_t)mat * a.mp + j] = on;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (f16_t)y[e];
+        *reinterpret_cast<f16x8*>((MODE == NS_XXT ? a.a16 : a.b16) + at) = o;
         *reinterpret_cast<f16x8*>(t) = o;   // (this thread's own place: for the mirror image below)
       } else {
-        // S X' = a S X + (S B) (S X) / S
+        // S X' = (a + d / S) S X + (S B) (S X) / S with the diagonal d of S B
         const int64_t at = mat * mn + (int64_t)j * a.mp + i;
         const f16x8 h8 = *reinterpret_cast<const f16x8*>(a.xt[xt_in] + at), l8 = *reinterpret_cast<const f16x8*>(a.xl + at);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(a.ca, (float)h8[e] + (float)l8[e], v[e] * a.inv_S);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(d[e], (float)h8[e] + (float)l8[e], v[e] * a.inv_S);
         if (MODE == NS_STEP) {
           f16x8 hi, lo;
 #pragma unroll
@@ -501,7 +527,7 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
 
 // ------------------------------------------------------------------------------------------------ small matrices
 // A matrix of at most 128 x 256 never leaves its CU: one workgroup of eight waves does the whole iteration (the launches alone cost 108 us
-// for 201 x 65, this 34).  X^T is held twice: in f32 in the accumulator layout of the step product (wave w: rows 32 w .. of X^T on the
+// for 201 x 65, this 38).  X^T is held twice: in f32 in the accumulator layout of the step product (wave w: rows 32 w .. of X^T on the
 // lanes, 128 columns in 4 x 16 registers), which takes a X without any rounding, and rounded to f16 in LDS (two images of 256 rows x 64
 // columns), whose rows serve B X and whose columns, read transposed, X X^T.  A and then B stand in a third place (two images of 128 x 64).
 constexpr int NS_SMALL_M = 128, NS_SMALL_N = 256, NS_SMALL_PITCH = 129;
@@ -513,13 +539,15 @@ __device__ __forceinline__ int ns_img_at(int row, int c, int image) {
 }
 
 // MB: blocks of 32 that hold anything of the short side (at least two): the rest is zero and not computed.  The k steps of a product are unrolled,
-// so that their fragments are in flight together (201 x 65 34 us, with four blocks 39; 64 x 256 29 and 40).
+// so that their fragments are in flight together (201 x 65: 34 us, 39 with four blocks; 64 x 256: 29 and 40; the diagonals have cost 4 since).
 template <typename T, bool MOM, bool W, int MB>
 __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const NsPtrs p, int steps) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* X = smem;
   char* A = smem + NS_SMALL_X;                          // 32 KiB, inside the staging area of the first and last phase
   float* stage = reinterpret_cast<float*>(A);           // [128 j][129]
+  float* diag_a = reinterpret_cast<float*>(A + 32768);  // [128] the diagonals of A and B, times S; zero in the images
+  float* diag_b = diag_a + 128;
   const int mat = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5, fast = tid & 127, slow = tid >> 7;
   const T* src = reinterpret_cast<const T*>(p.src[mat]);
@@ -611,19 +639,43 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
     }
     // element (i, i') of the symmetric result stands in row i' (the lane) at columns i (four registers): its mirror image
     f16x4 av[2][4];
+    // (the diagonal of a block on the diagonal: lane r of the half that holds its row, register `own`)
+    const bool holds = ((r >> 2) & 1) == hf;
+    const int own = (r & 3) + 4 * (r >> 3);
+    auto on_diagonal = [&](f32x16& z) {
+      float on = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        on = e == own ? z[e] : on;
+        z[e] = e == own && holds ? 0.f : z[e];
+      }
+      return on;
+    };
     if (mine) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < 2; ++y) {
+        const int ip = 32 * (bc + y) + r;
+        if (bi == bc + y) {
+          const float on = on_diagonal(acc[y]) * a.inv_S;
+          if (holds) diag_a[ip] = on;
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) av[y][g][e] = (f16_t)(acc[y][4 * g + e] * a.inv_S);
-          *reinterpret_cast<f16x4*>(A + ns_img_at(32 * (bc + y) + r, 32 * bi + 8 * g + 4 * hf, 16384)) = av[y][g];
+          *reinterpret_cast<f16x4*>(A + ns_img_at(ip, 32 * bi + 8 * g + 4 * hf, 16384)) = av[y][g];
         }
+      }
     }
     __syncthreads();
     zero(acc[0]);
     zero(acc[1]);
+    float4 di[4];
+    float djs[2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) di[g] = *reinterpret_cast<const float4*>(diag_a + 32 * bi + 8 * g + 4 * hf);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) djs[y] = diag_a[32 * (bc + y) + r];
     if (mine) {
 #pragma unroll
       for (int k = 0; k < 2 * MB; ++k) {
@@ -636,15 +688,29 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
     }
     __syncthreads();   // all of A is read
     if (mine) {
+      const float k = a.cc * a.inv_S;
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < 2; ++y) {
+        const int ip = 32 * (bc + y) + r;
+        const float dj = djs[y];
+        if (bi == bc + y) {   // (E is zero there: what follows leaves the zero)
+          const float on = on_diagonal(acc[y]);
+          if (holds) diag_b[ip] = fmaf(a.cb, dj, k * fmaf(dj, dj, on));
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float d[4] = {di[g].x, di[g].y, di[g].z, di[g].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[y][4 * g + e] = fmaf(a.cb, (float)av[y][g][e], k * fmaf(d[e] + dj, (float)av[y][g][e], acc[y][4 * g + e]));
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           f16x4 o;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = (f16_t)fmaf(a.cb, (float)av[y][g][e], acc[y][4 * g + e] * (a.cc * a.inv_S));
-          *reinterpret_cast<f16x4*>(A + ns_img_at(32 * (bc + y) + r, 32 * bi + 8 * g + 4 * hf, 16384)) = o;
+          for (int e = 0; e < 4; ++e) o[e] = (f16_t)acc[y][4 * g + e];
+          *reinterpret_cast<f16x4*>(A + ns_img_at(ip, 32 * bi + 8 * g + 4 * hf, 16384)) = o;
         }
+      }
     }
     __syncthreads();
     if (32 * wave < a.n) {   // (rows past the matrix are zero and stay so)
@@ -660,7 +726,12 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
 #pragma unroll
       for (int b = 0; b < MB; ++b)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[b][e] = fmaf(a.ca, x[b][e], acc[b][e] * a.inv_S);
+        for (int g = 0; g < 4; ++g) {
+          const float4 d4 = *reinterpret_cast<const float4*>(diag_b + 32 * b + 8 * g + 4 * hf);
+          const float d[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[b][4 * g + e] = fmaf(fmaf(d[e], a.inv_S, a.ca), x[b][4 * g + e], acc[b][4 * g + e] * a.inv_S);
+        }
       if (s + 1 < steps) store_x();   // (a wave's rows are its own in this product)
     }
   }
@@ -710,7 +781,7 @@ static NsSize ns_size(int rows, int cols, bool wide) {
   NsSize s;
   s.mp = ns_up(std::min(rows, cols), wide ? 256 : 128);
   s.np = ns_up(std::max(rows, cols), wide ? 256 : 128);
-  s.bytes = NS_PARTS * 8 + s.mp * s.np * (2 * 2 + 2) + std::max(s.mp, s.np) * s.mp * 2 + s.mp * s.mp * 2;
+  s.bytes = NS_PARTS * 8 + s.mp * 2 * 4 + s.mp * s.np * (2 * 2 + 2) + std::max(s.mp, s.np) * s.mp * 2 + s.mp * s.mp * 2;
   return s;
 }
 // matrices of one pass: as many as 1 GiB of workspace holds, at least one
@@ -861,6 +932,8 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
     return at;
   };
   a.parts = (double*)take(NS_PARTS * 8);
+  a.diag_a = (float*)take(size.mp * 4);
+  a.diag_b = (float*)take(size.mp * 4);
   a.xt[0] = (f16_t*)take(mn * 2);
   a.xl = (f16_t*)take(mn * 2);
   // xt[1] and, behind it, a16: the un-normalised update of the momentum (4 bytes an element) is read before either is written

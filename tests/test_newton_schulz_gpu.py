@@ -1,7 +1,7 @@
 """The orthogonalised update and the optimizer built on it against float64: odd sizes, types, strides, batches, ranks; refusals.
 
 Tolerances: the products run on f16 operands.  ``_emulated`` repeats the iteration in float64 with exactly the kernel's three roundings a
-step (X, A and B to f16, X itself unrounded), which says for each input how far those carry the result; the kernel adds float32 sums
+step (X, and A and B beside their diagonals, to f16; X itself unrounded), which says for each input how far those carry the result; the kernel adds float32 sums
 and other signs of the same roundings, for which the bound is twice that, plus half a step of the bf16 result."""
 
 import copy
@@ -29,11 +29,16 @@ def _emulated(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
     def r(t):
         return (t * s).to(torch.float16).double() / s
 
+    def parts(t):      # the diagonal exact, the rest rounded
+        d = torch.diag(t.diagonal())
+        return d, r(t - d)
+
     x = x / (x.square().sum().sqrt() + eps)
     for _ in range(steps):
         h = r(x)
-        p = r(h @ h.T)
-        x = a * x + r(b * p + c * (p @ p)) @ h
+        da, ea = parts(h @ h.T)
+        db, eb = parts(b * (da + ea) + c * (da + ea) @ (da + ea))
+        x = a * x + db @ x + eb @ h
     return x.T if tall else x
 
 
