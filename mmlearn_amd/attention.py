@@ -244,26 +244,30 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
 
 
 # ------------------------------------------------------------------ attention with a learned relative position bias
+def _places(*operands: Optional[torch.Tensor]):
+    return [t if t is None else (t.data_ptr(), t.stride()) for t in operands]
+
+
 class _RelativeAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, key_mask, offsets, how):
-        q_offset = how["q_offset"] if offsets is None else offsets
-        out, out_lo, lse = K.rel_attn_fwd(q, k, v, table, how["max_distance"], how["bidirectional"], how["scale"], how["causal"], key_mask, q_offset,
-                                          any(ctx.needs_input_grad[:4]))
+        p = K.rel_attn_operands(q, k, v, table, *how[:4], key_mask, how[4] if offsets is None else offsets)
+        out, out_lo, lse = K.rel_attn_fwd(p, q, True)
         ctx.save_for_backward(q, k, v, table, key_mask, offsets, out, out_lo, lse)
-        ctx.how = how
+        ctx.how, ctx.operands, ctx.places = how, p, _places(q, k, v, table, key_mask, offsets)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, table, key_mask, offsets, out, out_lo, lse = ctx.saved_tensors
-        how = ctx.how
+        p, how = ctx.operands, ctx.how
+        if ctx.places != _places(q, k, v, table, key_mask, offsets):   # (hooks on saved tensors brought them back elsewhere)
+            p = K.rel_attn_operands(q, k, v, table, *how[:4], key_mask, how[4] if offsets is None else offsets)
         dout = dout.to(q.dtype).contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()
-        grads = K.rel_attn_bwd(q, k, v, table, how["max_distance"], how["bidirectional"], how["scale"], how["causal"], key_mask,
-                               how["q_offset"] if offsets is None else offsets, out, out_lo, lse, dout, ctx.needs_input_grad[3])
+        grads = K.rel_attn_bwd(p, q, k, table, out, out_lo, lse, dout, ctx.needs_input_grad[3])
         return (*grads, None, None, None)
 
 
@@ -320,8 +324,7 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     if any(t is not None and t.device != q.device for t in (k, v, table, key_mask, offsets)):
         raise ValueError(f"{name}: all operands must be on one device")
     scale = D ** -0.5 if scale is None else float(scale)
+    how = max_distance, bool(bidirectional), scale, bool(causal), 0 if offsets is not None else q_offset
     if not _records(q, k, v, table):
-        return K.rel_attn_fwd(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset, False)[0]
-    how = {"max_distance": max_distance, "bidirectional": bool(bidirectional), "scale": scale, "causal": bool(causal),
-           "q_offset": 0 if offsets is not None else q_offset}
+        return K.rel_attn_fwd(K.rel_attn_operands(q, k, v, table, *how[:4], key_mask, q_offset), q, False)[0]
     return _RelativeAttention.apply(q, k, v, table, key_mask, offsets, how)

@@ -1382,7 +1382,9 @@ def _strides_bhl(t: torch.Tensor):
     return b if B > 1 else 0, h if H > 1 else 0, row if L > 1 else 0
 
 
-def _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset) -> _lib.RelAttn:
+def rel_attn_operands(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int, bidirectional: bool, scale: float,
+                      causal: bool, key_mask: Optional[torch.Tensor], q_offset) -> _lib.RelAttn:
+    """What ``rel_attn_fwd`` and ``rel_attn_bwd`` of one call are told of q [B, H, Lq, D], k / v [B, Hk, Lk, D] (views), table and masks."""
     p = _lib.RelAttn()
     B, H, Lq, D = q.shape
     p.q, p.k, p.v, p.table, p.mask = ptr(q), ptr(k), ptr(v), ptr(table), ptr(key_mask)
@@ -1406,41 +1408,39 @@ def _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_ma
     return p
 
 
-def rel_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int, bidirectional: bool, scale: float,
-                 causal: bool, key_mask: Optional[torch.Tensor], q_offset, for_backward: bool):
-    """q [B, H, Lq, D], k / v [B, Hk, Lk, D] views -> out [B, Lq, H, D] contiguous and, for the backward, what its rounding left (the same
-    shape) and lse f32 [B, H, Lq], else None twice.  csrc/rel_attention.hip."""
+def rel_attn_fwd(p: _lib.RelAttn, q: torch.Tensor, for_backward: bool):
+    """-> out [B, Lq, H, D] contiguous and, for the backward, what its rounding left (the same shape) and lse f32 [B, H, Lq], else None twice.
+    csrc/rel_attention.hip."""
     require_gpu(q)
     B, H, Lq, D = q.shape
-    p = _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset)
+    lib = _lib.lib()
     with on_device_of(q):
         out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
         out_lo = torch.empty_like(out) if for_backward else None
         lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if for_backward else None
-        n = _lib.lib().mmk_rel_attn_fwd_ws_floats(C.byref(p))
+        n = lib.mmk_rel_attn_fwd_ws_floats(C.byref(p))
         ws = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
-        check(_lib.lib().mmk_rel_attn_fwd(C.byref(p), ptr(out), ptr(out_lo), ptr(lse), ptr(ws), stream()))
+        check(lib.mmk_rel_attn_fwd(C.byref(p), ptr(out), ptr(out_lo), ptr(lse), ptr(ws), stream()))
     return out, out_lo, lse
 
 
-def rel_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int, bidirectional: bool, scale: float,
-                 causal: bool, key_mask: Optional[torch.Tensor], q_offset, out: torch.Tensor, out_lo: torch.Tensor, lse: torch.Tensor,
+def rel_attn_bwd(p: _lib.RelAttn, q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, out: torch.Tensor, out_lo: torch.Tensor, lse: torch.Tensor,
                  dout: torch.Tensor, want_dtable: bool = True):
     """-> (dq, dk, dv as [B, heads, L, D] views of contiguous [B, L, heads, D] buffers, dtable or None)."""
     require_gpu(q)
     B, H, Lq, D = q.shape
     Hk, Lk = k.shape[1], k.shape[2]
     assert out.is_contiguous() and dout.is_contiguous() and out.shape == (B, Lq, H, D) == dout.shape
-    p = _rel_attn(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset)
+    lib, dt, dev = _lib.lib(), q.dtype, q.device
     with on_device_of(q):
-        dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-        dk, dv = (torch.empty((B, Lk, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+        dq = torch.empty_strided((B, H, Lq, D), (Lq * H * D, D, H * D, 1), dtype=dt, device=dev)
+        dk = torch.empty_strided((B, Hk, Lk, D), (Lk * Hk * D, D, Hk * D, 1), dtype=dt, device=dev)
+        dv = torch.empty_strided((B, Hk, Lk, D), (Lk * Hk * D, D, Hk * D, 1), dtype=dt, device=dev)
         dtable = None if not want_dtable else torch.empty_like(table) if B else torch.zeros_like(table)
         if B:
-            ws = torch.empty(max(1, _lib.lib().mmk_rel_attn_bwd_ws_floats(C.byref(p), int(want_dtable))), dtype=torch.float32, device=q.device)
-            check(_lib.lib().mmk_rel_attn_bwd(C.byref(p), ptr(out), ptr(out_lo), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws),
-                                              stream()))
-    return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), dtable
+            ws = torch.empty(max(1, lib.mmk_rel_attn_bwd_ws_floats(C.byref(p), int(want_dtable))), dtype=torch.float32, device=dev)
+            check(lib.mmk_rel_attn_bwd(C.byref(p), ptr(out), ptr(out_lo), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(ws), stream()))
+    return dq, dk, dv, dtable
 
 
 # ------------------------------------------------------------------ orthogonalised updates (Newton-Schulz)
