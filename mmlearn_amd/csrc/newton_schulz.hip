@@ -766,10 +766,12 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
 
 // ------------------------------------------------------------------------------------------------ host
 static int64_t ns_up(int64_t v, int to) { return (v + to - 1) / to * to; }
-// Tiles of 256 x 256 for the step product (and the padding they need) where they fill whole rounds of the CUs to three quarters: 1 x 4096 x
-// 4096 (256 tiles) 148 us a product against 160 with tiles of 128, 12 x 768 x 2304 (324 tiles, the second round almost empty) 75 and 61
+// Tiles of 256 x 256 for the step product where they fill whole rounds of the CUs to three quarters (1 x 4096 x 4096, 256 tiles: 148 us a
+// product against 160 with tiles of 128; 12 x 768 x 2304, 324 tiles, the second round almost empty: 75 and 61) and need no more padding, which
+// all products would carry (whole iterations with 256 / 128: 64 x 640 x 640 1220 / 702 us, 16 x 896 x 1024 551 / 452, 1 x 3968 x 4096 1520 / 1381)
 static bool ns_wide(int count, int rows, int cols) {
   const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+  if (ns_up(m, 256) != ns_up(m, 128) || ns_up(n, 256) != ns_up(n, 128)) return false;
   const int64_t tiles = count * (ns_up(m, 256) / 256) * (ns_up(n, 256) / 256);
   return tiles * 4 >= (tiles + 255) / 256 * 256 * 3;
 }

@@ -103,7 +103,7 @@ def test_batches_strides_and_neighbours():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("count,rows,cols", [(22, 384, 640), (40, 640, 384), (64, 1280, 100), (64, 640, 640), (3, 130, 4000)])
+@pytest.mark.parametrize("count,rows,cols", [(22, 384, 640), (40, 640, 384), (64, 1280, 100), (64, 640, 640), (64, 500, 510), (3, 130, 4000)])
 def test_batches_that_fill_the_chip_differently(count, rows, cols):
     """Few tiles, some for every CU, many, and 256 x 256 ones."""
     x = torch.randn(count, rows, cols, generator=torch.Generator().manual_seed(count))
