@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import kernels as K
 
@@ -175,8 +176,10 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, device=None) -
 
 
 def _records(*operands: Optional[torch.Tensor]) -> bool:
-    """Whether autograd has to record the call (an autograd function costs a single token more than its kernel)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands)
+    """Whether autograd has to see the call (an autograd function costs a single token more than its kernel): to record it, or, within a
+    level of forward-mode differentiation, to refuse operands with a tangent, which do not require grad (past the function their
+    derivative would vanish without a word)."""
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands))
 
 
 class _QKNormRotary(torch.autograd.Function):
@@ -206,8 +209,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     ``rotary``: a :func:`rotary_table` of even width ``<= D``; of a head's first ``rotary.shape[1]`` values the pairs ``(i, i + width / 2)``
     turn (``interleaved``: ``(2 i, 2 i + 1)``), the others pass.  None: no rotation.  ``positions``: int32 / int64 ``[L]`` or ``[B, L]``, rows of
     the table; None: ``0 .. L - 1``.  They are read on the device: a position outside the table makes its rows NaN.
-    Both passes may be captured into a HIP graph.  As with every autograd function, no output of an eager pass over the same leaves may be
-    alive then: it would keep the leaves' gradient nodes on that pass's stream."""
+    Forward-mode derivatives are refused.  Both passes may be captured into a HIP graph.  As with every autograd function, no output of an
+    eager pass over the same leaves may be alive then: it would keep the leaves' gradient nodes on that pass's stream."""
     K.require_gpu(q, "query")
     name = "mmlearn_amd.qk_norm_rotary"
     if not (q.dim() == k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3] and q.dtype == k.dtype
@@ -288,7 +291,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     or an int32 tensor ``[B]`` (one token against a cache: the number of keys before it).  A row that nothing is left for gives zeros and
     passes no gradient.
 
-    The table's gradient is exact to about 1e-5 of its size before it is rounded to the table's type.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive."""
+    The table's gradient is exact to about 1e-5 of its size before it is rounded to the table's type; forward-mode derivatives are
+    refused.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive."""
     K.require_gpu(q, "query")
     name = "mmlearn_amd.relative_attention"
     if not (q.dim() == k.dim() == v.dim() == 4 and q.dtype in (torch.bfloat16, torch.float16) and q.dtype == k.dtype == v.dtype):

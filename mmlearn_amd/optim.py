@@ -30,6 +30,7 @@ import math
 from typing import Any, Dict, List, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import kernels as K
@@ -211,9 +212,12 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients: Sequence[f
     """The matrices of ``update`` ``[..., rows, cols]`` (f32 / bf16 / f16, any strides, sides up to 32768) with their singular values driven towards
     1: ``X = G / (|G| + eps)``, then ``steps`` times ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``.  Returns bf16, contiguous: the
     products run on 16-bit operands (csrc/newton_schulz.hip) with f32 diagonals, whose errors of about 5e-4 are below half a step of bf16.  A matrix
-    of zeros stays zero; one that holds a NaN or an infinity becomes NaN.  The coefficients must keep singular values below about 4."""
+    of zeros stays zero; one that holds a NaN or an infinity becomes NaN.  The coefficients must keep singular values below about 4.
+    An update is no function to differentiate: the result requires no grad, and an ``update`` with a forward-mode tangent is refused."""
     require_gpu(update, "update")
     name = "mmlearn_amd.optim.orthogonalize"
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(update).tangent is not None:
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
     _check_iteration(name, steps, coefficients, eps)
     if update.dim() < 2 or update.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError(f"{name}: need a [..., rows, cols] tensor of float32, bfloat16 or float16")

@@ -4,6 +4,7 @@ Tolerances: the products run on f16 operands.  ``_emulated`` repeats the iterati
 step (X, and A and B beside their diagonals, to f16; X itself unrounded), which says for each input how far those carry the result; the kernel adds float32 sums
 and other signs of the same roundings, for which the bound is twice that, plus half a step of the bf16 result."""
 
+import contextlib
 import copy
 import ctypes
 import math
@@ -261,3 +262,18 @@ def test_refusals(monkeypatch):
         p.grad = torch.zeros_like(p)
         with pytest.raises(RuntimeError, match="dense contiguous f32"):
             Muon([p]).step()
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    from torch.autograd import forward_ad as fw
+
+    from mmlearn_amd import optim as O
+
+    monkeypatch.setattr(O, "require_gpu", lambda *a: None)
+    monkeypatch.setattr(O._lib, "on_device_of", lambda t: contextlib.nullcontext())
+    monkeypatch.setattr(O.K, "newton_schulz", lambda *a: None)
+    x = torch.zeros(4, 6)
+    with fw.dual_level():
+        assert orthogonalize(x).shape == (4, 6)
+        with pytest.raises(NotImplementedError, match="forward"):
+            orthogonalize(fw.make_dual(x, x))

@@ -249,3 +249,23 @@ def test_rotary_table_at_far_positions():
         for i in range(4):
             a = p * 10000.0 ** (-2 * i / 8)
             assert abs(t[p, i].item() - math.cos(a)) <= 2.0 ** -24 and abs(t[p, 4 + i].item() - math.sin(a)) <= 2.0 ** -24
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(monkeypatch, grad):
+    """No operand requires grad, so nothing is recorded; a tangent must not vanish all the same."""
+    from torch.autograd import forward_ad as fw
+
+    from mmlearn_amd import attention as A
+
+    monkeypatch.setattr(A.K, "require_gpu", lambda *a: None)
+    monkeypatch.setattr(A.K, "qk_norm_rotary_fwd", lambda q, k, *a: (torch.empty(q.shape), torch.empty(k.shape)))
+    ops = [torch.zeros(1, 2, 3, 4), torch.zeros(1, 2, 1, 4), torch.ones(4), torch.ones(4)]
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        assert qk_norm_rotary(*ops)[0].shape == (1, 2, 3, 4)       # nothing has a tangent
+        for n in range(4):
+            duals = [fw.make_dual(t, torch.ones_like(t)) if i == n else t for i, t in enumerate(ops)]
+            with pytest.raises((NotImplementedError, RuntimeError), match="forward|jvp"):
+                qk_norm_rotary(*duals)
+    with pytest.raises((NotImplementedError, RuntimeError), match="forward|jvp"):
+        torch.func.jvp(lambda x: qk_norm_rotary(x, x)[0], (ops[0],), (ops[0],))

@@ -394,3 +394,22 @@ def test_refusals(monkeypatch):
     ):
         with pytest.raises(ValueError):
             relative_attention(**{"q": q, "k": k, "v": k, "table": t, **bad})
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(monkeypatch, grad):
+    """No operand requires grad, so nothing is recorded; a tangent must not vanish all the same."""
+    from torch.autograd import forward_ad as fw
+
+    from mmlearn_amd import attention as A
+
+    monkeypatch.setattr(A.K, "require_gpu", lambda *a: None)
+    monkeypatch.setattr(A.K, "rel_attn_operands", lambda *a: None)
+    monkeypatch.setattr(A.K, "rel_attn_fwd", lambda p, q, record: (q.transpose(1, 2).contiguous(), None, None))
+    ops = [torch.zeros(1, 2, 3, 64, dtype=torch.bfloat16) for _ in range(3)] + [torch.zeros(32, 2)]
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        assert relative_attention(*ops).shape == (1, 3, 2, 64)     # nothing has a tangent
+        for n in range(4):
+            duals = [fw.make_dual(t, torch.ones_like(t)) if i == n else t for i, t in enumerate(ops)]
+            with pytest.raises((NotImplementedError, RuntimeError), match="forward|jvp"):
+                relative_attention(*duals)
