@@ -16,6 +16,8 @@
 // delta decides how exact the table's gradient is: dS sums to zero along a row, and an error of delta is one of every dS of the row.  With
 // o rounded (or summed from rounded P) dtable is off by 4e-3 at 512 keys, an f32 one too.  So a forward that will be differentiated sums
 // o from P in two parts, rounded and the rest, and hands the backward what the rounding of o left: delta and dtable then hold to 1e-5.
+// f16's range is narrow for dS (P is about 1 / Lk, the incoming gradient of any size) and for P of far keys, so both go through their products
+// times a power of two, which is exact and leaves with the accumulators: P times a constant, dS times one that follows its largest value.
 #include <hip/hip_ext.h>
 #include <limits.h>
 
@@ -128,6 +130,37 @@ __device__ __forceinline__ s16x8 rel_operand_rest(const f32x16& x, int s, s16x8 
   }
   return __builtin_bit_cast(s16x8, o);
 }
+// P's factor in the backward: P <= 1, and what f32 makes of a score may carry it a little above
+template <typename T>
+constexpr int REL_P_BITS = std::is_same<T, f16_t>::value ? 14 : 0;
+
+// f16: the power of two that dS of a lane's row (key) goes through its product with, a running one like the maximum of a softmax: it falls
+// when a value times it would pass 2^15, and the accumulators of that lane (and of the one 32 away, which holds the same row) fall with it.
+// Values 2^-29 of the largest so far are still normal.  bf16 has f32's range and needs none.  (2 x 16 (on 4) x 4097 x 128 causal and back: 865 us,
+// without it 825; 16 x 12 x 512 x 64: 152 both.)
+struct RelRange {
+  int bits = 60;   // (from here down f16 results of such dS are zero anyway)
+  float factor = 0x1p60f;
+  template <int N>
+  __device__ __forceinline__ void follow(const f32x16& x, f32x16 (&acc)[N]) {
+    float most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(x[e]));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const bool over = most * factor > 32768.f;
+    if (__any(over)) {
+      const int to = over ? min(bits, 15 - __builtin_amdgcn_frexp_expf(most)) : bits;   // (an infinity passes as it is)
+      const float by = __builtin_ldexpf(1.f, to - bits);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[n][e] *= by;
+      bits = to;
+      factor = __builtin_ldexpf(1.f, to);
+    }
+  }
+  __device__ __forceinline__ float undo(float mul) const { return __builtin_ldexpf(mul, -bits); }
+};
 __device__ __forceinline__ f32x16 rel_zero() {
   f32x16 z;
 #pragma unroll
@@ -692,6 +725,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int CB = D / 64, STAGE = 2 * CB * 8192, EXT = 96, VECS = REL_DIAG;
+  constexpr bool F16 = std::is_same<T, f16_t>::value;
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int nbias = (2 * (a.far + EXT) + 1 + 3) & ~3;
   float* diag = bias + nbias;   // [VECS][nbias], per half wave
@@ -720,6 +754,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelA
 
   s16x8 qf[D / 16], gf[D / 16];
   f32x16 dq[D / 32];
+  RelRange range;
   float lse, delta = 0.f, far_l = 0.f, far_r = 0.f;
   {
     const int ic = min(i, a.Lq - 1);
@@ -816,6 +851,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelA
           }
         }
       }
+      if (F16) {
+        range.follow(s, dq);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= range.factor;
+      }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         const s16x8 df = rel_operand<T>(s, st);
@@ -824,7 +864,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelA
       }
     }
   }
-  if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, nullptr, dq, a.scale, hf);
+  if (i < a.Lq) rel_store_row<T, D>(reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + h) * D, nullptr, dq, F16 ? range.undo(a.scale) : a.scale, hf);
   if (!a.dtab_part) return;
   // ---- this workgroup's sums by bucket: the far sums join their wave's vectors at its ends, the vectors are added in order, and
   // a thread per (bucket, slice) collects its distances
@@ -891,6 +931,8 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int CB = D / 64, STAGE = 2 * CB * 8192 + 512, KB = 128, EXT = 96;
+  constexpr bool F16 = std::is_same<T, f16_t>::value;
+  constexpr int BITS = REL_P_BITS<T>;
   float* bias = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5;
@@ -901,6 +943,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const Rel
   const int j_wg = kb * KB, j_wave = j_wg + 32 * wave, j = j_wave + r;
   const bool kept = j < klen && rel_mask_at(a, b, j);
   f32x16 dk[D / 32], dv[D / 32];
+  RelRange range;   // of 2^BITS dS
   s16x8 kf[D / 16], vf[D / 16];
   {
     const int jc = min(j, a.Lk - 1);
@@ -946,7 +989,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const Rel
     char* Gr = Q + CB * 8192;
     float* rows = reinterpret_cast<float*>(Q + 2 * CB * 8192);   // [lse 64][delta 64]
     wait_vmem_all();
-    if (wave < 2) rows[64 * wave + lane] = rowv;
+    if (wave < 2) rows[64 * wave + lane] = wave ? rowv : rowv - BITS;   // (P comes out times 2^BITS)
     if (hg != head) {   // (nobody reads the old bias any more once all are past this barrier)
       __syncthreads();
       rel_bias_fill<T>(a, bias, EXT, hk * a.G + hg, tid, 256);
@@ -1012,6 +1055,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const Rel
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] = kept && acc_row(e) >= imin ? dp[e] : 0.f;
       }
+      if (F16) {
+        range.follow(dp, dk);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] *= range.factor;
+      }
       if (D == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
@@ -1029,9 +1077,19 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const Rel
       for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = rel_zero();
     }
     if (S == 1) {
-      rel_store_row<T, D>(reinterpret_cast<T*>(a.dk) + at, nullptr, dk, a.scale, hf);
-      rel_store_row<T, D>(reinterpret_cast<T*>(a.dv) + at, nullptr, dv, 1.f, hf);
+      rel_store_row<T, D>(reinterpret_cast<T*>(a.dk) + at, nullptr, dk, F16 ? range.undo(__builtin_ldexpf(a.scale, -BITS)) : a.scale, hf);
+      rel_store_row<T, D>(reinterpret_cast<T*>(a.dv) + at, nullptr, dv, __builtin_ldexpf(1.f, -BITS), hf);
     } else {
+      if (F16) {
+        const float k1 = range.undo(__builtin_ldexpf(1.f, -BITS)), v1 = __builtin_ldexpf(1.f, -BITS);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            dk[dt][e] *= k1;
+            dv[dt][e] *= v1;
+          }
+      }
       const int64_t n = (int64_t)a.B * a.Lk * a.Hk * D;
       rel_store_row<D>(a.dkv_part + 2 * split * n + at, dk, hf);
       rel_store_row<D>(a.dkv_part + (2 * split + 1) * n + at, dv, hf);

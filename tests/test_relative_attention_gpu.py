@@ -413,3 +413,51 @@ def test_forward_mode_derivatives_are_refused(monkeypatch, grad):
             duals = [fw.make_dual(t, torch.ones_like(t)) if i == n else t for i, t in enumerate(ops)]
             with pytest.raises((NotImplementedError, RuntimeError), match="forward|jvp"):
                 relative_attention(*duals)
+
+
+def _exact_head(q, k, v, dout, scale, seen=None):
+    """One head without bias in float64: out, dq, dk, dv, and dS, P."""
+    z = (q @ k.T) * scale
+    if seen is not None:
+        z = z.masked_fill(~seen, float("-inf"))
+    p = torch.softmax(z, 1)
+    o = p @ v
+    ds = p * (dout @ v.T - (dout * o).sum(1, keepdim=True))
+    return o, ds @ k * scale, ds.T @ q * scale, p.T @ dout, ds, p
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lq,lk,size,peak", [(64, 4096, 1e-4, 1.0), (300, 512, 1e-5, 1.0), (96, 96, 1e4, 3.0), (1, 4096, 1e-4, 1.0), (40, 700, 1e4, 3.0),
+                                             (1100, 300, 1e-4, 1.0)])     # (several workgroups a key block)
+def test_f16_gradients_of_any_size(lq, lk, size, peak, D):
+    """dS = P (dP - delta) stays off both ends of f16's range, whatever the size of the gradient that comes in: it is rounded once relative to its
+    size, as the results are.  (Rounded as it stands it is subnormal at ordinary sizes of P and dout, and infinite beyond 65504.)"""
+    g = torch.Generator().manual_seed(lq + lk)
+    q = (peak * torch.randn(1, 1, lq, D, generator=g)).half()
+    k, v = (torch.randn(1, 1, lk, D, generator=g).half() for _ in range(2))
+    dout = (size * torch.randn(1, lq, 1, D, generator=g)).clamp(-6e4, 6e4).half()
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v, torch.zeros(32, 1))]
+    out = relative_attention(*leaves)
+    got = [t.double().cpu() for t in torch.autograd.grad(out, leaves, dout.cuda())]
+    Q, Kd, V, dO = q[0, 0].double(), k[0, 0].double(), v[0, 0].double(), dout[0, :, 0].double()
+    scale = D ** -0.5
+    o, dq, dk, dv, ds, p = _exact_head(Q, Kd, V, dO, scale)
+    u = 2.0 ** -11
+    # a score's f32 sums (D products, scale, maximum, exponential, softmax's sum), as a relative error of P; delta from an o in two parts of f16
+    es = 2.0 ** -24 * ((D + 8) * (Q.abs() @ Kd.abs().T).amax(1, keepdim=True) * scale + lk / 16 + 32)
+    edelta = (dO.abs() * (u * u * o.abs() + (u * u + es) * (p @ V.abs()) + 2.0 ** -25)).sum(1, keepdim=True)
+    e32 = 2 * es * ds.abs() + p * edelta + p * 2.0 ** -24 * (D + 8) * (dO.abs() @ V.abs().T + (dO * o).abs().sum(1, keepdim=True))
+    bounds = {"dq": ((u * ds.abs() + e32) @ Kd.abs() * scale, dq), "dk": ((u * ds.abs() + e32).T @ Q.abs() * scale, dk),
+              "dv": (((u + 2 * es) * p).T @ dO.abs(), dv)}
+    for (name, (err, want)), x in zip(bounds.items(), got):
+        x = x[0, 0]
+        fits = want.abs() < 6e4     # (a gradient of this size can itself be past f16's end, which is infinite and no fault)
+        assert torch.isfinite(x[fits]).all() and fits.double().mean() > 0.99, name
+        x = torch.where(fits, x, want)
+        # the result is rounded once: half a step of its own size, or of f16's smallest values
+        over = ((x - want).abs() - 1.01 * err - 1.01 * (u * want.abs() + 2.0 ** -25)).max().item()
+        assert over <= 0, (name, over, ((x - want).norm() / want.norm()).item())
+        # independent roundings: of dS (P) before the product, of the result after it
+        once = (want.half().double() - want).norm()
+        assert (x - want).norm() <= 2 * (once + u * want.norm()), (name, ((x - want).norm() / want.norm()).item())
