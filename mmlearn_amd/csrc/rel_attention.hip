@@ -130,6 +130,11 @@ __device__ __forceinline__ s16x8 rel_operand_rest(const f32x16& x, int s, s16x8 
   }
   return __builtin_bit_cast(s16x8, o);
 }
+// The forward's P is relative to a maximum that is at most 2^8 too low; in f16 it is carried 2^7 higher, to 2^15 at most, so that keys far below
+// the first one are still there when there are many of them: each is off by 2^-32 of the first at most, 2^20 of them by half a step of the
+// result (the softmax's sum is of the same values; lse takes the factor out again).
+template <typename T>
+constexpr int REL_FWD_BITS = std::is_same<T, f16_t>::value ? 7 : 0;
 // P's factor in the backward: P <= 1, and what f32 makes of a score may carry it a little above
 template <typename T>
 constexpr int REL_P_BITS = std::is_same<T, f16_t>::value ? 14 : 0;
@@ -457,14 +462,16 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
     }
-    const float nm = m == -INFINITY ? 0.f : -m;
+    const float nm = m == -INFINITY ? 0.f : REL_FWD_BITS<T> - m;
+    float lt = 0.f;   // (a tile's sum by itself: single keys far below the sum so far would not move it)
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[t][e] = att_exp2(s[t][e] + nm);
-        l += s[t][e];
+        lt += s[t][e];
       }
+    l += lt;
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
       const s16x8 pf = rel_operand<T>(s[st >> 1], st & 1);
@@ -482,7 +489,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
   if (i < a.Lq) {
     const int64_t row = (((int64_t)b * a.Lq + i) * a.H + h) * D;
     rel_store_row<T, D>(reinterpret_cast<T*>(a.out) + row, LO ? reinterpret_cast<T*>(a.out_lo) + row : nullptr, o, sum > 0.f ? 1.f / sum : sum, hf);
-    if (a.lse && hf == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : m + log2f(sum);
+    if (a.lse && hf == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : m - REL_FWD_BITS<T> + log2f(sum);
   }
 }
 
@@ -588,12 +595,14 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
     }
-    const float nm = m == -INFINITY ? 0.f : -m;
+    const float nm = m == -INFINITY ? 0.f : REL_FWD_BITS<T> - m;
+    float lt = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       s[e] = att_exp2(s[e] + nm);
-      l += s[e];
+      lt += s[e];
     }
+    l += lt;
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const s16x8 pf = rel_operand<T>(s, st);
@@ -649,7 +658,7 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
       const int ro = blk * 32 + rr, go = ro / a.Lq, io = ro - go * a.Lq, ho = hk * a.G + go;
       const float f = ll > 0.f ? 1.f / ll : ll;
       rel_store_out<T>(a, (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-      if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm + log2f(ll);
+      if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm - REL_FWD_BITS<T> + log2f(ll);
     }
   }
 }
@@ -680,7 +689,7 @@ __global__ __launch_bounds__(256) void rel_join_kernel(const RelArgs a) {
   }
   const float f = ll > 0.f ? 1.f / ll : ll;
   rel_store_out<T>(a, (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm + log2f(ll);
+  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm - REL_FWD_BITS<T> + log2f(ll);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, dtable

@@ -2,6 +2,7 @@
 anything behind them, offsets, strides; gradients (table included) against the definition's and against differences; refusals."""
 
 import ctypes
+import math
 import os
 import subprocess
 
@@ -461,3 +462,24 @@ def test_f16_gradients_of_any_size(lq, lk, size, peak, D):
         # independent roundings: of dS (P) before the product, of the result after it
         once = (want.half().double() - want).norm()
         assert (x - want).norm() <= 2 * (once + u * want.norm()), (name, ((x - want).norm() / want.norm()).item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [1, 3, 130])
+def test_f16_many_keys_far_below_the_first(lq):
+    """2^20 keys, each 2^-26 of the first one's weight: together 1.5 % of the result, and none of them lost below f16's smallest values."""
+    lk = 1 << 20
+    far = 26 * math.log(2.0)
+    q = torch.zeros(1, 1, lq, 64)
+    q[..., 0] = 8.0                                       # scale 1 / 8: the score is k[0]
+    k, v = torch.zeros(1, 1, lk, 64), torch.ones(1, 1, lk, 64)
+    k[:, :, 0, 0], v[:, :, 0] = far, 0.0
+    q, k, v = (t.half().cuda() for t in (q, k, v))
+    weight = math.exp(-k[0, 0, 0, 0].double().item())     # of each of the others
+    want = (lk - 1) * weight / (1 + (lk - 1) * weight)
+    table = torch.zeros(32, 1, device="cuda")
+    for grad in (False, True):
+        out = relative_attention(q.requires_grad_(grad), k, v, table).double()
+        # half a step of the result, and of P; the f32 sum of the weights: 2^14 tiles added to 1, each off by 2^-24 at most.  Times 2^7 a weight
+        # is 32.2 times f16's smallest value 2^-24: each is off by half of that at most, 2^-25 / 2^7 of the largest one's weight
+        assert (out - want).abs().max().item() <= want * (2 * 2.0 ** -11 + 2.0 ** -10) + lk * 2.0 ** -32, (grad, out.mean().item(), want)
