@@ -578,7 +578,7 @@ int mmk_qk_norm_rotary_bwd(const void* q, const void* k, const void* qw, const v
  * first near_buckets hold one distance each, the next n_borders + 1 begin at near_buckets, borders[0], borders[1], .. (HOST memory,
  * ascending); all distances from max_distance (1 .. 512) on fall into one bucket.  table: [buckets][H], f32 or the operands' type.
  * mask: one of MMK_REL_MASK_* -- LEN: int [B] leading keys are kept; 8 / 32 / 64: [B, Lk] integers of that width with batch stride
- * mask_stride, nonzero = kept.  Masked keys and values may hold anything.  q_offsets (int32 [B], device) overrides q_offset.
+ * mask_stride, nonzero = kept.  Masked keys and values may hold anything, with `causal` those behind the last query too.  q_offsets (int32 [B], device) overrides q_offset.
  * ws: mmk_rel_attn_fwd_ws_floats() floats.
  * Backward: out / out_lo / dout [B, Lq, H, D] contiguous; dq / dk / dv contiguous [B, L, heads, D]; dtable [buckets][H] in table_dtype, NULL: not
  * wanted; ws: mmk_rel_attn_bwd_ws_floats() floats.  All sums in a fixed order. */

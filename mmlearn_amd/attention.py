@@ -287,9 +287,10 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     ``max_distance`` (above the number of single distances where there are more than two, at most 512), beyond which all distances share the last one.
 
     ``key_mask``: ``[B, Lk]`` bool / uint8 / int32 / int64 with nonzero = attended, or int32 / int64 ``[B]`` numbers of leading keys.  What masked
-    keys and values hold does not matter.  ``causal``: only keys ``j <= i + q_offset``.  ``q_offset``: position of query 0 among the keys, an int
-    or an int32 tensor ``[B]`` (one token against a cache: the number of keys before it).  A row that nothing is left for gives zeros and
-    passes no gradient.
+    keys and values hold does not matter.  ``causal``: only keys ``j <= i + q_offset``; what stands behind the last query (the free places of a
+    cache) does not matter either, but a NaN or an infinity in a key or value of the queries' own stretch may reach earlier rows near it.
+    ``q_offset``: position of query 0 among the keys, an int or an int32 tensor ``[B]`` (one token against a cache: the number of keys before
+    it).  A row that nothing is left for gives zeros and passes no gradient.
 
     The table's gradient is exact to about 1e-5 of its size before it is rounded to the table's type; forward-mode derivatives are
     refused.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive."""

@@ -210,11 +210,13 @@ __device__ __forceinline__ int rel_offset(const RelArgs& a, int b) {
   const int o = a.off_ptr ? a.off_ptr[b] : a.off;
   return __builtin_amdgcn_readfirstlane(min(max(o, -(1 << 29)), 1 << 29));   // (distances stay within 32 bits; far beyond every bucket border)
 }
-// how many leading keys of the sample can be kept at all
-__device__ __forceinline__ int rel_key_len(const RelArgs& a, int b) {
+// how many leading keys of the sample can be kept at all.  Causal: none behind the last query, whatever stands there (the places of a cache
+// that are not filled yet)
+__device__ __forceinline__ int rel_key_len(const RelArgs& a, int b, int off) {
   int64_t n = a.Lk;
   if (a.mask_kind == MMK_REL_MASK_LEN32) n = reinterpret_cast<const int32_t*>(a.mask)[b];
   if (a.mask_kind == MMK_REL_MASK_LEN64) n = reinterpret_cast<const int64_t*>(a.mask)[b];
+  if (a.causal) n = min(n, (int64_t)a.Lq + off);
   return __builtin_amdgcn_readfirstlane((int)(n < 0 ? 0 : n < a.Lk ? n : a.Lk));
 }
 // whether the mask keeps key j (1 where there is no per-key mask); j may lie past the end
@@ -367,7 +369,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
   const RelPlace pl = rel_place(blockIdx.x, nqb, a.B * a.H);
   const int bh = pl.head, b = bh / a.H, h = bh - b * a.H;
   const int qb = a.causal ? nqb - 1 - pl.rank : pl.rank;   // causal: the longest rows first
-  const int off = rel_offset(a, b), klen = rel_key_len(a, b);
+  const int off = rel_offset(a, b), klen = rel_key_len(a, b, off);
   const int i_wg = qb * 128, i_wave = i_wg + 32 * wave, i = i_wave + r;
   int nkt = (klen + 63) / 64;
   if (a.causal) {
@@ -512,13 +514,11 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
   const int rows = a.G * a.Lq, row = blk * 32 + r;
   const int rc = min(row, rows - 1), g = rc / a.Lq, i = rc - g * a.Lq, h = hk * a.G + g;
   const int g0 = blk * 32 / a.Lq, g1 = min(blk * 32 + 31, rows - 1) / a.Lq;   // heads of this block
-  const int off = rel_offset(a, b), klen = rel_key_len(a, b), ip = i + off;
+  const int off = rel_offset(a, b), klen = rel_key_len(a, b, off), ip = i + off;
   for (int gg = g0; gg <= g1; ++gg) rel_bias_fill<T>(a, bias_all + (gg - g0) * nb, EXT, hk * a.G + gg, tid, 256);
   const float* bias = bias_all + (g - g0) * nb + a.far + EXT;
   // tiles of this split: the sample's own length is divided, so that short samples do not leave splits idle
-  int last = klen - 1;
-  if (a.causal) last = min(last, a.Lq - 1 + off);
-  const int tiles = last < 0 ? 0 : last / 32 + 1, per = (tiles + a.splits - 1) / a.splits;
+  const int tiles = (klen + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
   const int t0 = split * per + wave, t1 = min((split + 1) * per, tiles);
   const T* kp = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
@@ -744,7 +744,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelA
   const RelPlace pl = rel_place(blockIdx.x, nqb, a.B * a.H);
   const int bh = pl.head, b = bh / a.H, h = bh - b * a.H;
   const int qb = a.causal ? nqb - 1 - pl.rank : pl.rank;
-  const int off = rel_offset(a, b), klen = rel_key_len(a, b);
+  const int off = rel_offset(a, b), klen = rel_key_len(a, b, off);
   const int i_wg = qb * 128, i_wave = i_wg + 32 * wave, i = i_wave + r;
   int nkt = (klen + 63) / 64;
   if (a.causal) {
@@ -948,7 +948,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const Rel
   const int nkb = (a.Lk + KB - 1) / KB, S = a.dkv_splits;
   const RelPlace pl = rel_place(blockIdx.x, nkb * S, a.B * a.Hk);
   const int kb = pl.rank / S, split = pl.rank - kb * S, b = pl.head / a.Hk, hk = pl.head - b * a.Hk;
-  const int off = rel_offset(a, b), klen = rel_key_len(a, b);
+  const int off = rel_offset(a, b), klen = rel_key_len(a, b, off);
   const int j_wg = kb * KB, j_wave = j_wg + 32 * wave, j = j_wave + r;
   const bool kept = j < klen && rel_mask_at(a, b, j);
   f32x16 dk[D / 32], dv[D / 32];

@@ -483,3 +483,37 @@ def test_f16_many_keys_far_below_the_first(lq):
         # half a step of the result, and of P; the f32 sum of the weights: 2^14 tiles added to 1, each off by 2^-24 at most.  Times 2^7 a weight
         # is 32.2 times f16's smallest value 2^-24: each is off by half of that at most, 2^-25 / 2^7 of the largest one's weight
         assert (out - want).abs().max().item() <= want * (2 * 2.0 ** -11 + 2.0 ** -10) + lk * 2.0 ** -32, (grad, out.mean().item(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,dtype", [(64, "bfloat16"), (128, "float16")])
+@pytest.mark.parametrize("lq,used,tensor", [(1, 37, True), (3, 64, False), (1, 200, False), (70, 61, True), (200, 0, False)])
+def test_causal_keys_behind_the_last_query_may_hold_anything(lq, used, tensor, D, dtype):
+    """A cache of fixed size that nobody has filled beyond the newest token: causal alone keeps those places out."""
+    g = torch.Generator().manual_seed(lq)
+    lk, n = 300, used + lq
+    dt = getattr(torch, dtype)
+    q, k, v = (torch.randn(2, h, s, D, generator=g).to(dt).cuda() for h, s in ((4, lq), (2, n), (2, n)))
+    dout = torch.randn(2, lq, 4, D, generator=g).to(dt).cuda()
+    table = torch.randn(32, 4, generator=g).cuda()
+    off = torch.full((2,), used, dtype=torch.int32, device="cuda") if tensor else used
+
+    def run(k, v):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v, table)]
+        out = relative_attention(*leaves, causal=True, q_offset=off)
+        with torch.no_grad():
+            plain = relative_attention(*leaves, causal=True, q_offset=off)
+        return out.detach(), plain, *torch.autograd.grad(out, leaves, dout)
+
+    want = run(k, v)
+    for junk in (float("nan"), float("inf")):
+        big = [torch.full((2, 2, lk, D), junk, dtype=dt, device="cuda") for _ in range(2)]
+        for b, t in zip(big, (k, v)):
+            b[:, :, :n] = t
+        got = run(*big)
+        for name, a, b in zip(("out", "out without gradient", "dq", "dk", "dv", "dtable"), got, want):
+            if name in ("dk", "dv"):
+                assert not a[:, :, n:].any(), name     # (any() is true for a NaN)
+                a = a[:, :, :n]
+            # (another number of keys may divide the sums differently)
+            assert torch.isfinite(a).all() and (a.double() - b.double()).norm() <= 4 * torch.finfo(dt).eps * b.double().norm(), name
