@@ -241,9 +241,11 @@ class Muon(torch.optim.Optimizer):
         ``w <- w (1 - lr weight_decay) - lr adjust orthogonalize(u)``
 
     with ``adjust = sqrt(max(1, rows / cols))`` (``adjust_lr_fn`` None or ``"original"``) or ``0.2 sqrt(max(rows, cols))``
-    (``"match_rms_adamw"``: the update's root mean square is that of AdamW, whose learning rates then carry over).  Arguments, formulas and
-    state (``momentum_buffer``) as in ``torch.optim.Muon``; parameters are dense contiguous f32 matrices on the GPU.  Momentum,
-    normalisation and the step of the weights are part of the launches; all matrices of one shape run as one batch.
+    (``"match_rms_adamw"``: the update's root mean square is that of AdamW, whose learning rates then carry over).  Arguments as in
+    ``torch.optim.Muon``, updates too but for ``eps``, which acts on the larger ``u`` and is added to its norm; parameters are dense contiguous
+    f32 matrices on the GPU.  ``momentum_buffer`` is the sum M above, ``torch.optim.Muon`` keeps the mean ``(1 - momentum) M``: ``load_state_dict``
+    converts a state that comes from there (its groups have no ``capturable``); the other way, multiply the buffers by ``1 - momentum``.
+    Momentum, normalisation and the step of the weights are part of the launches; all matrices of one shape run as one batch.
 
     ``capturable=True``: the learning rate is read from a device word (``lr_device(g)``), so a captured step follows it.  A captured step
     bakes in the addresses of weights, gradients and momenta: run one eager step before capturing and keep the gradients
@@ -266,6 +268,18 @@ class Muon(torch.optim.Optimizer):
         for p in self.param_groups[-1]["params"]:
             if p.dim() != 2:
                 raise ValueError(f"mmlearn_amd.optim.Muon takes matrices; got a parameter of shape {tuple(p.shape)}")
+
+    def load_state_dict(self, state_dict) -> None:
+        means = ["capturable" not in group for group in state_dict["param_groups"]]
+        if any(mean and not 0 <= group["momentum"] < 1 for mean, group in zip(means, state_dict["param_groups"])):
+            raise ValueError("mmlearn_amd.optim.Muon: a state of torch.optim.Muon needs a momentum below 1")
+        super().load_state_dict(state_dict)
+        for group, mean in zip(self.param_groups, means):
+            if mean:
+                group["capturable"] = self.defaults["capturable"]
+                for p in group["params"]:
+                    if "momentum_buffer" in self.state.get(p, {}):   # (not in place: the state dict may hold the other optimizer's own tensors)
+                        self.state[p]["momentum_buffer"] = self.state[p]["momentum_buffer"].float() / (1 - group["momentum"])
 
     @torch.no_grad()
     def step(self, closure=None):

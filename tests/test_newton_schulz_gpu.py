@@ -277,3 +277,67 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
         assert orthogonalize(x).shape == (4, 6)
         with pytest.raises(NotImplementedError, match="forward"):
             orthogonalize(fw.make_dual(x, x))
+
+
+def _torch_muon_state(start, grads, **how):
+    """A state of ``torch.optim.Muon`` after steps on the CPU, and the weights they lead to."""
+    params = [torch.nn.Parameter(t.clone()) for t in start]
+    opt = torch.optim.Muon(params, **how)
+    for gs in grads:
+        for p, g in zip(params, gs):
+            p.grad = g.clone()
+        opt.step()
+    return opt, params
+
+
+@pytest.mark.parametrize("momentum", [0.95, 0.0])
+def test_a_state_of_torch_muon_is_converted(momentum):
+    g = torch.Generator().manual_seed(21)
+    start = [torch.randn(5, 7, generator=g), torch.randn(6, 4, generator=g)]
+    grads = [[torch.randn(t.shape, generator=g) for t in start] for _ in range(4)]
+    theirs, params = _torch_muon_state(start, grads, lr=0.02, momentum=momentum)
+    before = [theirs.state[p]["momentum_buffer"].clone() for p in params]
+    idle = torch.nn.Parameter(torch.zeros(2, 2))
+    mine = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    opt = Muon(mine, lr=0.5, capturable=True)
+    opt.load_state_dict(theirs.state_dict())
+    for i, p in enumerate(mine):
+        m = torch.zeros(start[i].shape, dtype=torch.float64)
+        for gs in grads:
+            m = momentum * m + gs[i].double()
+        # theirs: a subtraction, a product and a sum in float32 a step; then the factor 1 / (1 - momentum) = 20, itself of float32
+        assert (opt.state[p]["momentum_buffer"].double() - m).abs().max() <= 4 * 4 * 2.0 ** -24 * m.abs().max() / (1 - momentum)
+        assert torch.equal(theirs.state[params[i]]["momentum_buffer"], before[i])
+    assert opt.param_groups[0]["lr"] == 0.02 and opt.param_groups[0]["capturable"] is True
+    # a state of this class stays as it is
+    other = Muon([torch.nn.Parameter(p.detach().clone()) for p in params] + [idle])
+    sd = opt.state_dict()
+    sd["param_groups"][0]["params"].append(2)
+    other.load_state_dict(sd)
+    for p, r in zip(mine, other.param_groups[0]["params"]):
+        assert torch.equal(opt.state[p]["momentum_buffer"], other.state[r]["momentum_buffer"])
+    Muon([idle]).load_state_dict(torch.optim.Muon([idle]).state_dict())     # (nothing in it yet)
+    with pytest.raises(ValueError, match="momentum"):
+        Muon([idle]).load_state_dict(torch.optim.Muon([idle], momentum=1.0).state_dict())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_continues_from_a_state_of_torch_muon(nesterov):
+    g = torch.Generator().manual_seed(22)
+    start = [0.1 * torch.randn(40, 60, generator=g), 0.1 * torch.randn(130, 70, generator=g)]
+    grads = [[1e-2 * torch.randn(t.shape, generator=g) for t in start] for _ in range(4)]
+    theirs, params = _torch_muon_state(start, grads, lr=0.02, momentum=0.95, nesterov=nesterov, weight_decay=0.0)
+    mine = [torch.nn.Parameter(p.detach().clone().cuda()) for p in params]
+    opt = Muon(mine)
+    opt.load_state_dict(theirs.state_dict())
+    last = [1e-2 * torch.randn(t.shape, generator=g) for t in start]
+    for p, x in zip(mine, last):
+        p.grad = x.cuda()
+    opt.step()
+    for i, p in enumerate(mine):
+        buf = torch.zeros(start[i].shape, dtype=torch.float64)
+        for gs in grads:
+            buf = 0.95 * buf + gs[i].double()
+        want, _, tol = _muon_oracle(params[i].detach().double(), buf, last[i].double(), 0.02, 0.0, 0.95, nesterov, False)
+        assert (p.detach().double().cpu() - want).abs().max() <= tol + 4 * 2.0 ** -24
