@@ -314,16 +314,17 @@ class Muon(torch.optim.Optimizer):
         word = None
         if group.get("capturable", False):
             word, seen = self._lr_words.get((gi, device), (None, None))
-            if word is None or (not capturing and seen != group["lr"]):
-                if capturing:
-                    raise RuntimeError("mmlearn_amd.optim.Muon(capturable=True): run one eager step before capturing")
+            if capturing and word is None:
+                raise RuntimeError("mmlearn_amd.optim.Muon(capturable=True): run one eager step before capturing")
+            # the number, not the object: a scheduler fills a tensor in place (eager steps only: a capture reads nothing on the host)
+            if not capturing and seen != float(group["lr"]):
                 word = torch.empty(1, dtype=torch.float32, device=device) if word is None else word
                 word.fill_(float(group["lr"]))
-                self._lr_words[gi, device] = (word, group["lr"])
+                self._lr_words[gi, device] = (word, float(group["lr"]))
         adjust = 0.2 * math.sqrt(max(rows, cols)) if group["adjust_lr_fn"] == "match_rms_adamw" else math.sqrt(max(1.0, rows / cols))
         K.newton_schulz([p.grad.data_ptr() for p in plist], [p.data_ptr() for p in plist], rows, cols, strides, dtype, device, group["ns_steps"],
                         group["ns_coefficients"], group["eps"], [self.state[p]["momentum_buffer"].data_ptr() for p in plist], group["momentum"],
-                        group["nesterov"], True, float(group["lr"]), adjust, group["weight_decay"], word)
+                        group["nesterov"], True, float(group["lr"]) if word is None else 0.0, adjust, group["weight_decay"], word)
         torch.autograd.graph.increment_version(plist)
 
     def lr_device(self, group_index: int = 0, device=None) -> torch.Tensor:

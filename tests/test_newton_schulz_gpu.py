@@ -341,3 +341,33 @@ def test_continues_from_a_state_of_torch_muon(nesterov):
             buf = 0.95 * buf + gs[i].double()
         want, _, tol = _muon_oracle(params[i].detach().double(), buf, last[i].double(), 0.02, 0.0, 0.95, nesterov, False)
         assert (p.detach().double().cpu() - want).abs().max() <= tol + 4 * 2.0 ** -24
+
+
+def _on_the_host(monkeypatch, calls):
+    """Muon's host side without a GPU: every launch is written down."""
+    from mmlearn_amd import optim as O
+
+    monkeypatch.setattr(O, "require_gpu", lambda *a: None)
+    monkeypatch.setattr(O._lib, "on_device_of", lambda t: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(O.K, "newton_schulz", lambda src, dst, rows, cols, *a: calls.append((rows, cols, a[-4], None if a[-1] is None else a[-1].item())))
+
+
+@pytest.mark.parametrize("tensor", [True, False])
+def test_capturable_eager_steps_follow_a_learning_rate_filled_in_place(monkeypatch, tensor):
+    calls = []
+    _on_the_host(monkeypatch, calls)
+    p = torch.nn.Parameter(torch.zeros(3, 4))
+    opt = Muon([p], lr=torch.tensor(0.5) if tensor else 0.5, capturable=True)
+    for lr in (0.5, 0.25, 0.25, 0.125):
+        if tensor:
+            opt.param_groups[0]["lr"].fill_(lr)
+        else:
+            opt.param_groups[0]["lr"] = lr
+        p.grad = torch.ones_like(p)
+        opt.step()
+        assert calls[-1][3] == lr and opt.lr_device().item() == lr
+    plain = Muon([p], lr=torch.tensor(0.5))
+    plain.param_groups[0]["lr"].fill_(0.25)
+    plain.step()
+    assert calls[-1][2:] == (0.25, None)
