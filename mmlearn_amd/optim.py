@@ -266,8 +266,11 @@ class Muon(torch.optim.Optimizer):
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
         for p in self.param_groups[-1]["params"]:
-            if p.dim() != 2:
-                raise ValueError(f"mmlearn_amd.optim.Muon takes matrices; got a parameter of shape {tuple(p.shape)}")
+            wrong = (f"takes matrices; got a parameter of shape {tuple(p.shape)}" if p.dim() != 2 else
+                     f"takes sides up to 32768; got a parameter of shape {tuple(p.shape)}" if p.numel() and max(p.shape) > 32768 else None)
+            if wrong:
+                self.param_groups.pop()
+                raise ValueError(f"mmlearn_amd.optim.Muon {wrong}")
 
     def load_state_dict(self, state_dict) -> None:
         means = ["capturable" not in group for group in state_dict["param_groups"]]
@@ -287,32 +290,42 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # everything that can be refused is, before any weight moves
+        batches: Dict[Any, List[torch.Tensor]] = {}
         for gi, group in enumerate(self.param_groups):
-            batches: Dict[Any, List[torch.Tensor]] = {}
             for p in group["params"]:
                 if p.grad is None or p.numel() == 0:
                     continue
                 require_gpu(p)
                 if p.dtype != torch.float32 or not p.is_contiguous() or p.grad.is_sparse:
                     raise RuntimeError("mmlearn_amd.optim.Muon supports dense contiguous f32 parameters")
-                batches.setdefault((p.device, tuple(p.shape), p.grad.dtype, p.grad.stride()), []).append(p)
-            for (device, (rows, cols), dtype, strides), plist in batches.items():
-                with _lib.on_device_of(plist[0]):
-                    self._step_batch(gi, group, plist, rows, cols, strides, dtype, device)
+                dtype_tag(p.grad.dtype)
+                batches.setdefault((gi, p.device, tuple(p.shape), p.grad.dtype, p.grad.stride()), []).append(p)
+        words = [self._prepare_batch(gi, self.param_groups[gi], plist, device) for (gi, device, *_), plist in batches.items()]
+        for ((gi, device, (rows, cols), dtype, strides), plist), word in zip(batches.items(), words):
+            group = self.param_groups[gi]
+            adjust = 0.2 * math.sqrt(max(rows, cols)) if group["adjust_lr_fn"] == "match_rms_adamw" else math.sqrt(max(1.0, rows / cols))
+            with _lib.on_device_of(plist[0]):
+                K.newton_schulz([p.grad.data_ptr() for p in plist], [p.data_ptr() for p in plist], rows, cols, strides, dtype, device, group["ns_steps"],
+                                group["ns_coefficients"], group["eps"], [self.state[p]["momentum_buffer"].data_ptr() for p in plist], group["momentum"],
+                                group["nesterov"], True, float(group["lr"]) if word is None else 0.0, adjust, group["weight_decay"], word)
+            torch.autograd.graph.increment_version(plist)
         return loss
 
-    def _step_batch(self, gi, group, plist, rows, cols, strides, dtype, device) -> None:
-        capturing = torch.cuda.is_current_stream_capturing()
-        for p in plist:
-            st = self.state[p]
-            buf = st.get("momentum_buffer")
-            if buf is None or buf.dtype != torch.float32 or not buf.is_contiguous() or buf.device != p.device:
-                if capturing:
-                    raise RuntimeError("mmlearn_amd.optim.Muon: run one eager step before capturing")
-                st["momentum_buffer"] = (torch.zeros_like(p, memory_format=torch.contiguous_format) if buf is None
-                                         else buf.to(device=p.device, dtype=torch.float32).contiguous())
-        word = None
-        if group.get("capturable", False):
+    def _prepare_batch(self, gi, group, plist, device):
+        """The momenta of a batch, and the device word of its learning rate or None."""
+        with _lib.on_device_of(plist[0]):
+            capturing = torch.cuda.is_current_stream_capturing()
+            for p in plist:
+                st = self.state[p]
+                buf = st.get("momentum_buffer")
+                if buf is None or buf.dtype != torch.float32 or not buf.is_contiguous() or buf.device != p.device:
+                    if capturing:
+                        raise RuntimeError("mmlearn_amd.optim.Muon: run one eager step before capturing")
+                    st["momentum_buffer"] = (torch.zeros_like(p, memory_format=torch.contiguous_format) if buf is None
+                                             else buf.to(device=p.device, dtype=torch.float32).contiguous())
+            if not group.get("capturable", False):
+                return None
             word, seen = self._lr_words.get((gi, device), (None, None))
             if capturing and word is None:
                 raise RuntimeError("mmlearn_amd.optim.Muon(capturable=True): run one eager step before capturing")
@@ -321,11 +334,7 @@ class Muon(torch.optim.Optimizer):
                 word = torch.empty(1, dtype=torch.float32, device=device) if word is None else word
                 word.fill_(float(group["lr"]))
                 self._lr_words[gi, device] = (word, float(group["lr"]))
-        adjust = 0.2 * math.sqrt(max(rows, cols)) if group["adjust_lr_fn"] == "match_rms_adamw" else math.sqrt(max(1.0, rows / cols))
-        K.newton_schulz([p.grad.data_ptr() for p in plist], [p.data_ptr() for p in plist], rows, cols, strides, dtype, device, group["ns_steps"],
-                        group["ns_coefficients"], group["eps"], [self.state[p]["momentum_buffer"].data_ptr() for p in plist], group["momentum"],
-                        group["nesterov"], True, float(group["lr"]) if word is None else 0.0, adjust, group["weight_decay"], word)
-        torch.autograd.graph.increment_version(plist)
+            return word
 
     def lr_device(self, group_index: int = 0, device=None) -> torch.Tensor:
         """The device word a captured step reads its learning rate from (``capturable=True``, after the first eager step)."""

@@ -371,3 +371,25 @@ def test_capturable_eager_steps_follow_a_learning_rate_filled_in_place(monkeypat
     plain.param_groups[0]["lr"].fill_(0.25)
     plain.step()
     assert calls[-1][2:] == (0.25, None)
+
+
+def test_a_refused_step_moves_nothing(monkeypatch):
+    calls = []
+    _on_the_host(monkeypatch, calls)
+    good = torch.nn.Parameter(torch.zeros(3, 4))
+    for other in (torch.nn.Parameter(torch.zeros(4, 5).t()), torch.nn.Parameter(torch.zeros(4, 5).bfloat16()), torch.nn.Parameter(torch.zeros(32768, 1))):
+        for p in (good, other):
+            p.grad = torch.ones_like(p)
+        opt = Muon([{"params": [good]}, {"params": [other]}])
+        if other.shape == (32768, 1):
+            opt.step()
+            assert [c[:2] for c in calls] == [(3, 4), (32768, 1)]
+            continue
+        with pytest.raises(RuntimeError, match="dense contiguous f32"):
+            opt.step()
+        assert not calls and not opt.state
+    # a matrix too wide for the kernels is refused where it is added, and leaves nothing behind
+    for shape, why in (((32769, 1), "32768"), ((2, 40000), "32768"), ((3,), "matrices")):
+        with pytest.raises(ValueError, match=why):
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(shape))]})
+        assert len(opt.param_groups) == 2
