@@ -16,6 +16,7 @@
 // Layout: sides padded with zeros, which the iteration keeps.  X is stored transposed, [n][m], as two f16 arrays: the operand S X rounded, and
 // the rest S X - that (together 22 bits, kept between steps).  A step moves 8 bytes an element: the transposed copy serves both products
 // -- B X takes its rows, X X^T contracts along its columns with transposed LDS reads -- and its epilogue is in place.
+#include <float.h>
 #include <hip/hip_ext.h>
 
 #include <algorithm>
@@ -896,6 +897,7 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
   MMK_REQUIRE(q != nullptr, "no arguments");
   if (int rc = ns_check(q->count, q->rows, q->cols)) return rc;
   MMK_REQUIRE(q->steps >= 1 && q->steps <= 32, "1 to 32 steps");
+  MMK_REQUIRE(q->eps >= FLT_MIN, "eps must be a normal positive number");   // (1 / eps has to be finite: zeros are divided by it)
   MMK_REQUIRE(!q->momenta || q->dtype == MMK_F32 || q->dtype == MMK_BF16 || q->dtype == MMK_F16, "unsupported dtype");
   if (q->count == 0) return 0;
   const bool small = ns_small(q->rows, q->cols);

@@ -203,8 +203,8 @@ def _check_iteration(name: str, steps: int, coefficients: Sequence[float], eps: 
         raise ValueError(f"{name}: 1 to 32 Newton-Schulz steps")
     if len(coefficients) != 3 or not all(math.isfinite(c) and abs(c) <= 64 for c in coefficients):
         raise ValueError(f"{name}: three finite coefficients of at most 64 in size")
-    if not (math.isfinite(eps) and eps > 0):
-        raise ValueError(f"{name}: eps must be positive")
+    if not (math.isfinite(eps) and eps >= 2.0 ** -126):   # (1 / eps has to be finite in float32: zeros are divided by it)
+        raise ValueError(f"{name}: eps must be positive, a normal number of float32")
 
 
 @torch.no_grad()

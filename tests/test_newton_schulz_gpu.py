@@ -393,3 +393,28 @@ def test_a_refused_step_moves_nothing(monkeypatch):
         with pytest.raises(ValueError, match=why):
             opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(shape))]})
         assert len(opt.param_groups) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(20, 30), (130, 260)])
+def test_zeros_stay_zero_at_the_smallest_eps(shape):
+    x = torch.zeros(2, *shape, device="cuda")
+    x[1] = 1.0
+    got = orthogonalize(x, eps=2.0 ** -126)
+    assert not got[0].any() and torch.isfinite(got).all()
+
+
+def test_an_eps_that_float32_cannot_divide_by_is_refused(monkeypatch):
+    from mmlearn_amd import _lib
+    from mmlearn_amd import optim as O
+
+    monkeypatch.setattr(O, "require_gpu", lambda *a: None)
+    monkeypatch.setattr(O.K, "newton_schulz", lambda *a: pytest.fail("reached the kernel"))
+    for eps in (1e-39, 1e-60, 2.0 ** -149):
+        with pytest.raises(ValueError, match="eps"):
+            orthogonalize(torch.zeros(4, 6), eps=eps)
+        with pytest.raises(ValueError, match="eps"):
+            Muon([torch.nn.Parameter(torch.zeros(3, 3))], eps=eps)
+        args = _lib.NewtonSchulz()
+        args.count, args.rows, args.cols, args.steps, args.eps = 0, 4, 6, 5, eps
+        assert _lib.lib().mmk_newton_schulz(ctypes.byref(args), None, None) != 0
