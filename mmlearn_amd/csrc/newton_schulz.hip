@@ -594,11 +594,11 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
     if (tid < o) red[tid] += red[tid + o];
     __syncthreads();
   }
-  const float scale = (float)(1.0 / (sqrt(red[0]) + (double)a.eps)) * a.S;   // (the product with S is exact)
+  const float inv = (float)(1.0 / (sqrt(red[0]) + (double)a.eps));
 #pragma unroll
   for (int b = 0; b < MB; ++b)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[b][e] *= scale;
+    for (int e = 0; e < 16; ++e) x[b][e] = x[b][e] * inv * a.S;   // (in this order: inv S may be past f32's end)
   auto store_x = [&]() {
 #pragma unroll
     for (int b = 0; b < MB; ++b)
