@@ -1154,7 +1154,8 @@ static int rel_check(const mmk_rel_attn* p) {
   MMK_REQUIRE(p->D == 64 || p->D == 128, "head dim must be 64 or 128");
   MMK_REQUIRE(p->B >= 0 && p->H >= 1 && p->Hk >= 1 && p->H % p->Hk == 0 && p->Lq >= 0 && p->Lk >= 0, "bad sizes");
   MMK_REQUIRE(p->Lq <= (1 << 28) && p->Lk <= (1 << 28), "sequence too long");
-  MMK_REQUIRE((int64_t)p->B * p->H * (((int64_t)std::max(p->Lq, p->Lk) + 127) / 128) < (1 << 24), "too many rows");   // (a launch holds 2^32 threads)
+  // a launch holds 2^32 threads: the forward's workgroups take 128 queries of a head each, however many keys there are
+  MMK_REQUIRE((int64_t)p->B * p->H * std::max<int64_t>(1, ((int64_t)p->Lq + 127) / 128) < (1 << 24), "too many query rows");
   MMK_REQUIRE(p->buckets >= 1 && p->buckets <= REL_MAX_BUCKETS && p->n_borders >= 0 && p->n_borders <= REL_MAX_BORDERS, "too many buckets");
   MMK_REQUIRE(p->near_buckets >= 1 && p->max_distance >= 1 && p->max_distance <= REL_MAX_FAR, "max_distance must be 1 .. 512");
   MMK_REQUIRE((p->bidirectional ? 2 : 1) * (p->near_buckets + p->n_borders + 1) == p->buckets, "near and logarithmic buckets do not add up");
@@ -1166,6 +1167,13 @@ static int rel_check(const mmk_rel_attn* p) {
   MMK_REQUIRE(p->q_strides[2] <= (1 << 23) && p->k_strides[2] <= (1 << 23) && p->v_strides[2] <= (1 << 23), "row stride too large");
   MMK_REQUIRE(p->mask_kind >= MMK_REL_MASK_NONE && p->mask_kind <= MMK_REL_MASK_64 && (p->mask_kind == 0) == (p->mask == nullptr), "bad mask");
   for (const void* x : {p->q, p->k, p->v}) MMK_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "operands must be 16-byte aligned");
+  return 0;
+}
+
+// the backward's, beside those, 128 keys of a key head (divided only where they are few)
+static int rel_check_bwd(const mmk_rel_attn* p) {
+  if (int rc = rel_check(p)) return rc;
+  MMK_REQUIRE((int64_t)p->B * p->Hk * (((int64_t)p->Lk + 127) / 128) < (1 << 24), "too many key rows");
   return 0;
 }
 
@@ -1306,13 +1314,13 @@ int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, void* out_lo, float* lse,
 }
 
 int64_t mmk_rel_attn_bwd_ws_floats(const mmk_rel_attn* p, int want_dtable) {
-  if (rel_check(p)) return -1;
+  if (rel_check_bwd(p)) return -1;
   return rel_dkv_floats(p) + (int64_t)p->B * p->H * p->Lq + (want_dtable ? (int64_t)p->B * p->H * rel_dq_blocks(p) * p->buckets : 0);
 }
 
 int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const void* out_lo, const float* lse, const void* dout, void* dq, void* dk, void* dv,
                      void* dtable, float* ws, void* stream) {
-  if (int rc = rel_check(p)) return rc;
+  if (int rc = rel_check_bwd(p)) return rc;
   MMK_REQUIRE(p->Lk == 0 || (dk && dv), "missing operand");
   MMK_REQUIRE(p->Lq == 0 || (p->q && out && out_lo && lse && dout && dq && ws && p->table), "missing operand");
   if (p->B == 0) {

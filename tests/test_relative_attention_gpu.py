@@ -517,3 +517,43 @@ def test_causal_keys_behind_the_last_query_may_hold_anything(lq, used, tensor, D
                 a = a[:, :, :n]
             # (another number of keys may divide the sums differently)
             assert torch.isfinite(a).all() and (a.double() - b.double()).norm() <= 4 * torch.finfo(dt).eps * b.double().norm(), name
+
+
+def _described(B, H, Hk, Lq, Lk, D):
+    """The C description of a call on operands that nobody reads."""
+    from mmlearn_amd import _lib
+
+    def flat(heads, rows):
+        return torch.zeros(D, dtype=torch.bfloat16).as_strided((B, heads, rows, D), (0, 0, 0, 1))
+
+    p = K.rel_attn_operands(flat(H, Lq), flat(Hk, Lk), flat(Hk, Lk), torch.zeros(32, H), 128, True, D ** -0.5, False, None, 0)
+    return p, _lib.lib()
+
+
+@pytest.mark.parametrize("B,H,Hk,Lq,Lk", [(64, 32, 1, 1, 1 << 20), (1, 2, 1, 130, 1 << 28), (1, 8, 8, 1, 1 << 28)])
+def test_many_keys_are_not_many_rows(B, H, Hk, Lq, Lk):
+    """What a launch holds is counted in queries; the length of a cache does not enter the forward's."""
+    p, lib = _described(B, H, Hk, Lq, Lk, 64)
+    assert lib.mmk_rel_attn_fwd_ws_floats(ctypes.byref(p)) >= 0, lib.mmk_last_error()
+    assert (lib.mmk_rel_attn_bwd_ws_floats(ctypes.byref(p), 1) >= 0) == (B * Hk * Lk // 128 < 1 << 24)
+    p, lib = _described(1 << 16, 1 << 8, 1, 1, 5, 64)     # 2^24 workgroups of 256 threads
+    assert lib.mmk_rel_attn_fwd_ws_floats(ctypes.byref(p)) == -1 and b"query rows" in lib.mmk_last_error()
+
+
+@pytest.mark.gpu
+def test_a_batch_of_very_long_caches():
+    """64 samples x 32 query heads against 2^20 keys (which all samples share here, by a stride of zero)."""
+    g = torch.Generator().manual_seed(3)
+    n = 1 << 20
+    k, v = (torch.randn(1, 1, n, 64, generator=g).bfloat16().cuda() for _ in range(2))
+    q = torch.randn(64, 32, 1, 64, generator=g).bfloat16().cuda()
+    table = torch.randn(32, 32, generator=g).cuda()
+    got = relative_attention(q, k.expand(64, -1, -1, -1), v.expand(64, -1, -1, -1), table, q_offset=n - 1)
+    for b in (0, 40, 63):
+        bias = torch.zeros(32, n, dtype=torch.float64, device="cuda") + table[15].double()[:, None]
+        rel = oracle.bucket_map(1, 300, 299, 32, 128, True)[0].cuda()
+        bias[:, -300:] = table.double()[rel].T
+        p = torch.softmax((q[b, :, 0].double() @ k[0, 0].double().T) / 8 + bias, -1)
+        want = p @ v[0, 0].double()
+        # P and the result are each rounded once, with independent signs over the keys
+        assert (got[b, 0].double() - want).norm() <= 2 * 2.0 ** -8 * want.norm(), b
