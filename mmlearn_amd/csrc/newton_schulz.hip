@@ -902,6 +902,8 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
   if (q->count == 0) return 0;
   const bool small = ns_small(q->rows, q->cols);
   MMK_REQUIRE(q->src && q->dst && (ws || small), "missing operand");
+  MMK_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "the workspace must be 16-byte aligned");
+  for (int i = 0; i < q->count; ++i) MMK_REQUIRE(q->src[i] && q->dst[i] && (!q->momenta || q->momenta[i]), "missing operand");
   NsArgs a = {};
   a.rows = q->rows;
   a.cols = q->cols;

@@ -381,6 +381,7 @@ int mmk_qk_norm_rotary_fwd(const void* q, const void* k, const void* qw, const v
   void* y[2] = {qo, ko};
   const int64_t* st[2] = {q_strides, k_strides};
   for (int i = 0; i < 2; ++i) {
+    MMK_REQUIRE(st[i] && (a.s[i].H == 0 || (x[i] && y[i])), "missing operand");
     a.s[i].x = x[i];
     a.s[i].w = w[i];
     a.s[i].y = y[i];
@@ -413,6 +414,7 @@ int mmk_qk_norm_rotary_bwd(const void* q, const void* k, const void* qw, const v
   const int64_t* gst[2] = {dq_strides, dk_strides};
   for (int i = 0; i < 2; ++i) {
     QkSide& s = a.s[i];
+    MMK_REQUIRE(st[i] && gst[i] && (s.H == 0 || (x[i] && g[i] && dx[i])), "missing operand");
     s.x = x[i];
     s.w = w[i];
     s.dy = g[i];

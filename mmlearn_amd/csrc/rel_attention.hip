@@ -1157,7 +1157,8 @@ static int rel_check(const mmk_rel_attn* p) {
   // a launch holds 2^32 threads: the forward's workgroups take 128 queries of a head each, however many keys there are
   MMK_REQUIRE((int64_t)p->B * p->H * std::max<int64_t>(1, ((int64_t)p->Lq + 127) / 128) < (1 << 24), "too many query rows");
   MMK_REQUIRE(p->buckets >= 1 && p->buckets <= REL_MAX_BUCKETS && p->n_borders >= 0 && p->n_borders <= REL_MAX_BORDERS, "too many buckets");
-  MMK_REQUIRE(p->near_buckets >= 1 && p->max_distance >= 1 && p->max_distance <= REL_MAX_FAR, "max_distance must be 1 .. 512");
+  MMK_REQUIRE(p->n_borders == 0 || p->borders, "missing borders");
+  MMK_REQUIRE(p->near_buckets >= 1 && p->near_buckets <= REL_MAX_BUCKETS && p->max_distance >= 1 && p->max_distance <= REL_MAX_FAR, "max_distance must be 1 .. 512");
   MMK_REQUIRE((p->bidirectional ? 2 : 1) * (p->near_buckets + p->n_borders + 1) == p->buckets, "near and logarithmic buckets do not add up");
   for (int i = 0; i < 3; ++i) {
     MMK_REQUIRE(p->q_strides[i] % 8 == 0 && p->k_strides[i] % 8 == 0 && p->v_strides[i] % 8 == 0, "strides must be multiples of 8 elements");
@@ -1270,7 +1271,7 @@ static int rel_backward(const mmk_rel_attn* p, RelArgs& a, void* dtable, hipStre
       MMK_LAUNCH_CHECK();
     }
   }
-  if (a.dtab_part) {
+  if (dtable) {   // (no queries: no partials, and no workspace for them)
     const int n = a.Lq > 0 ? nqb : 0;
     if (p->table_dtype == MMK_F32)
       hipLaunchKernelGGL(rel_dtable_kernel<float>, dim3(a.H), dim3(256), 0, st, a.dtab_part, (float*)dtable, a.B, a.H, n, a.buckets);
@@ -1305,6 +1306,8 @@ int mmk_rel_attn_fwd(const mmk_rel_attn* p, void* out, void* out_lo, float* lse,
   if ((int64_t)p->B * p->Lq == 0) return 0;
   MMK_REQUIRE(p->q && out && (p->Lk == 0 || (p->k && p->v)) && p->table, "missing operand");
   MMK_REQUIRE(mmk_rel_attn_fwd_ws_floats(p) == 0 || ws, "missing workspace");
+  for (const void* x : {(const void*)out, (const void*)out_lo, (const void*)ws})
+    MMK_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "outputs and the workspace must be 16-byte aligned");
   RelArgs a = rel_args(p);
   a.out = out;
   a.out_lo = out_lo;
@@ -1321,8 +1324,11 @@ int64_t mmk_rel_attn_bwd_ws_floats(const mmk_rel_attn* p, int want_dtable) {
 int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const void* out_lo, const float* lse, const void* dout, void* dq, void* dk, void* dv,
                      void* dtable, float* ws, void* stream) {
   if (int rc = rel_check_bwd(p)) return rc;
-  MMK_REQUIRE(p->Lk == 0 || (dk && dv), "missing operand");
-  MMK_REQUIRE(p->Lq == 0 || (p->q && out && out_lo && lse && dout && dq && ws && p->table), "missing operand");
+  MMK_REQUIRE(p->Lk == 0 || (dk && dv && p->k && p->v), "missing operand");
+  MMK_REQUIRE(p->Lq == 0 || (p->q && out && out_lo && lse && dout && dq && p->table), "missing operand");
+  MMK_REQUIRE(ws || mmk_rel_attn_bwd_ws_floats(p, dtable != nullptr) == 0, "missing workspace");
+  for (const void* x : {out, out_lo, dout, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)ws})
+    MMK_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "gradients and the workspace must be 16-byte aligned");
   if (p->B == 0) {
     if (!dtable) return 0;
     MMK_REQUIRE(false, "the table's gradient of no samples is the caller's zero");

@@ -109,3 +109,56 @@ def test_the_driver_build_entry_point_passes(built):
     src = open(g.__file__).read()
     assert "_lib.ABI_VERSION" in src and built.lib().mmk_abi_version() == built.ABI_VERSION
 
+
+def _error(built, rc):
+    return rc, built.lib().mmk_last_error().decode()
+
+
+def test_missing_operands_of_the_tower_operators_are_refused_on_the_host(built):
+    """A null pointer comes back as an error; nothing is launched with it (the addresses here belong to nobody)."""
+    import ctypes as C
+
+    lib, at, st = built.lib(), 1 << 20, (C.c_int64 * 3)(64, 64, 64)
+    # mmk_qk_norm_rotary_fwd / _bwd
+    q, k, qo, ko = at, at, at, at
+    for hole in range(6):
+        a = [x if i != hole else None for i, x in enumerate((q, k, qo, ko, st, st))]
+        rc, why = _error(built, lib.mmk_qk_norm_rotary_fwd(a[0], a[1], None, None, None, 0, None, 0, 0, a[2], a[3], 1, 1, 1, 1, 64, 0, 0, a[4], a[5], 1e-6, 1, 1, None))
+        assert rc == -1 and "missing operand" in why, (hole, why)
+    for hole in range(10):
+        a = [x if i != hole else None for i, x in enumerate((at, at, at, at, at, at, st, st, st, st))]
+        rc, why = _error(built, lib.mmk_qk_norm_rotary_bwd(a[0], a[1], None, None, None, 0, None, 0, 0, a[2], a[3], a[4], a[5], None, None, None, None, 1, 1, 1, 1, 64, 0, 0,
+                                                          a[6], a[7], a[8], a[9], 1e-6, 1, 1, None))
+        assert rc == -1 and "missing operand" in why, (hole, why)
+    # mmk_newton_schulz
+    for hole in range(4):
+        p = built.NewtonSchulz()
+        arrays = [(C.c_void_p * 2)(at, None if hole == i else at) for i in range(3)]
+        p.src, p.dst, p.momenta = (C.cast(x, C.c_void_p) for x in arrays)
+        p.count, p.rows, p.cols, p.steps, p.eps, p.weights, p.row_stride, p.col_stride = 2, 300, 300, 5, 1e-7, 1, 300, 1
+        rc, why = _error(built, lib.mmk_newton_schulz(C.byref(p), at + 8 if hole == 3 else at, None))
+        assert rc == -1 and ("aligned" if hole == 3 else "missing operand") in why, (hole, why)
+    # mmk_rel_attn_fwd / _bwd
+    def described(Lq=200, **how):
+        p = built.RelAttn()
+        borders = (C.c_int32 * 1)(3)
+        p.q, p.k, p.v, p.table, p.borders = at, at, at, at, C.cast(borders, C.c_void_p)
+        p.B, p.H, p.Hk, p.Lq, p.Lk, p.D, p.dtype, p.table_dtype = 1, 1, 1, Lq, 200, 64, 1, 1
+        p.buckets, p.near_buckets, p.n_borders, p.max_distance = 4, 2, 1, 8
+        for n, x in how.items():
+            setattr(p, n, x)
+        return p
+
+    for how in (dict(q=None), dict(k=None), dict(v=None), dict(table=None), dict(borders=None)):
+        rc, why = _error(built, lib.mmk_rel_attn_fwd(C.byref(described(**how)), at, None, None, at, None))
+        assert rc == -1 and "missing" in why, (how, why)
+        rc, why = _error(built, lib.mmk_rel_attn_bwd(C.byref(described(**how)), *[at] * 9, None))
+        assert rc == -1 and "missing" in why, (how, why)
+    for hole in (0, 1, 2, 3, 4, 5, 6, 8):     # (7: the table's gradient may be unwanted)
+        rc, why = _error(built, lib.mmk_rel_attn_bwd(C.byref(described()), *[at if i != hole else None for i in range(9)], None))
+        assert rc == -1 and "missing" in why, (hole, why)
+    for hole in (0, 1, 3, 4, 5, 6, 8):
+        rc, why = _error(built, lib.mmk_rel_attn_bwd(C.byref(described()), *[at if i != hole else at + 8 for i in range(9)], None))
+        assert rc == -1 and "aligned" in why, (hole, why)
+    rc, why = _error(built, lib.mmk_rel_attn_fwd(C.byref(described(near_buckets=2**31 - 1, n_borders=0)), at, None, None, at, None))
+    assert rc == -1

@@ -557,3 +557,15 @@ def test_a_batch_of_very_long_caches():
         want = p @ v[0, 0].double()
         # P and the result are each rounded once, with independent signs over the keys
         assert (got[b, 0].double() - want).norm() <= 2 * 2.0 ** -8 * want.norm(), b
+
+
+@pytest.mark.gpu
+def test_the_table_gradient_of_no_queries_needs_no_workspace():
+    from mmlearn_amd import _lib
+
+    q, kv = (torch.zeros(1, 2, n, 64, dtype=torch.bfloat16, device="cuda") for n in (0, 0))
+    table, dtable = torch.zeros(32, 2, device="cuda"), torch.full((32, 2), 3.0, device="cuda")
+    p, lib = K.rel_attn_operands(q, kv, kv, table, 128, True, 0.125, False, None, 0), _lib.lib()
+    assert lib.mmk_rel_attn_bwd_ws_floats(ctypes.byref(p), 1) == 0
+    _lib.check(lib.mmk_rel_attn_bwd(ctypes.byref(p), *[None] * 7, dtable.data_ptr(), None, _lib.stream()))
+    assert not dtable.any()
