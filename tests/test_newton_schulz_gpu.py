@@ -418,3 +418,29 @@ def test_an_eps_that_float32_cannot_divide_by_is_refused(monkeypatch):
         args = _lib.NewtonSchulz()
         args.count, args.rows, args.cols, args.steps, args.eps = 0, 4, 6, 5, eps
         assert _lib.lib().mmk_newton_schulz(ctypes.byref(args), None, None) != 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,rows,cols", [(3, 300, 129), (3, 129, 301), (22, 384, 640), (40, 640, 380), (64, 500, 510), (70, 130, 140), (2, 512, 5000)])
+def test_muon_steps_of_batches(count, rows, cols):
+    """Two steps (momenta that are not zero) of several equal matrices at once: few tiles, some for every CU, many, 256 x 256 ones, more matrices than
+    one launch takes; columns that fit no vector."""
+    g = torch.Generator().manual_seed(count)
+    start = 0.1 * torch.randn(count, rows, cols, generator=g)
+    params = [torch.nn.Parameter(t.cuda()) for t in start]
+    opt = Muon(params, lr=0.02, weight_decay=0.1, momentum=0.9)
+    which = sorted({0, count // 2, count - 1})
+    want = {i: start[i].double() for i in which}
+    bufs, slack = {i: torch.zeros(rows, cols, dtype=torch.float64) for i in which}, dict.fromkeys(which, 0.0)
+    for step in range(2):
+        grads = 1e-2 * torch.randn(count, rows, cols, generator=g)
+        grads[count // 2] *= 1e3
+        for p, x in zip(params, grads):
+            p.grad = x.cuda()
+        opt.step()
+        for i in which:
+            want[i], bufs[i], tol = _muon_oracle(want[i], bufs[i], grads[i].double(), 0.02, 0.1, 0.9, True, False)
+            slack[i] += tol
+            assert (params[i].detach().double().cpu() - want[i]).abs().max() <= slack[i] + 4 * 2.0 ** -24, (step, i)
+            b = opt.state[params[i]]["momentum_buffer"].double().cpu()
+            assert (b - bufs[i]).abs().max() <= (step + 1) * 2.0 ** -23 * bufs[i].abs().max(), (step, i)

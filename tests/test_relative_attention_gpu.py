@@ -569,3 +569,52 @@ def test_the_table_gradient_of_no_queries_needs_no_workspace():
     assert lib.mmk_rel_attn_bwd_ws_floats(ctypes.byref(p), 1) == 0
     _lib.check(lib.mmk_rel_attn_bwd(ctypes.byref(p), *[None] * 7, dtable.data_ptr(), None, _lib.stream()))
     assert not dtable.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1.0, 0.03, -0.2, 0.0])
+@pytest.mark.parametrize("lq,dtype,train", [(1, "bfloat16", False), (150, "bfloat16", True), (70, "float16", True)])
+def test_scales(lq, dtype, train, scale):
+    """T5-type towers take scale = 1."""
+    c = _case(2, 4, 2, lq, 190, 64, dtype, "f32")
+    dev, _, _, _ = _inputs(c, 5)
+    dev[0] = dev[0] / 4       # (scores of a few units at scale 1)
+    leaves = [t.detach().requires_grad_(train) for t in dev[:4]]
+    out = relative_attention(*leaves, scale=scale)
+    a = [t.detach().double().cpu().requires_grad_(train) for t in dev[:4]]
+    want = oracle.relative_attention(*a, scale=scale)
+    # P, dS and the results are each rounded once, with independent signs: a few half steps of the type in the norm
+    tol = 6 * torch.finfo(dev[0].dtype).eps
+    assert (out.detach().double().cpu() - want.detach()).norm() <= tol * want.detach().norm()
+    if train:
+        got = torch.autograd.grad(out, leaves, dev[4])
+        for name, x, w in zip(("dq", "dk", "dv", "dtable"), got, torch.autograd.grad(want, a, dev[4].double().cpu())):
+            if scale == 0.0 and name in ("dq", "dk"):
+                assert not x.any()
+            else:
+                assert (x.double().cpu() - w).norm() <= tol * w.norm(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("train", [False, True])
+def test_a_serving_batch_with_offsets_of_its_own(train):
+    """Each sample's new tokens stand behind its own cache: lengths and offsets a sample, a few tokens each."""
+    g = torch.Generator().manual_seed(31)
+    used = torch.tensor([0, 5, 63, 64, 250, 296], dtype=torch.int32)
+    B, lq, lk = len(used), 4, 300
+    q = torch.randn(B, lq, 8, 64, generator=g).bfloat16().cuda().transpose(1, 2)
+    k, v = (torch.full((B, lk, 2, 64), float("nan"), dtype=torch.bfloat16) for _ in range(2))
+    for b, n in enumerate((used + lq).tolist()):
+        k[b, :n], v[b, :n] = (torch.randn(n, 2, 64, generator=g).bfloat16() for _ in range(2))
+    table = torch.randn(32, 8, generator=g)
+    keep = torch.arange(lk)[None] < (used + lq)[:, None]
+    dout = torch.randn(B, lq, 8, 64, generator=g).bfloat16()
+    leaves = [t.requires_grad_(train) for t in (q, k.cuda().transpose(1, 2), v.cuda().transpose(1, 2), table.cuda())]
+    out = relative_attention(*leaves, bidirectional=False, causal=True, key_mask=(used + lq).cuda(), q_offset=used.cuda())
+    a = [torch.nan_to_num(t.detach().double().cpu()).requires_grad_(train) for t in leaves]
+    want = oracle.relative_attention(*a, bidirectional=False, causal=True, keep=keep, q_offset=used.tolist())
+    tol = 6 * 2.0 ** -7
+    assert (out.detach().double().cpu() - want.detach()).norm() <= tol * want.detach().norm()
+    if train:
+        for x, w in zip(torch.autograd.grad(out, leaves, dout.cuda()), torch.autograd.grad(want, a, dout.double())):
+            assert torch.isfinite(x).all() and (x.double().cpu() - w).norm() <= tol * w.norm()
