@@ -61,7 +61,7 @@ struct RelArgs {
   int dkv_splits;
   // split forward
   float* part;               // partial results of the key splits
-  int splits, row_blocks;
+  int splits;
   int borders[REL_MAX_BORDERS];   // smallest distance of the 2nd, 3rd, .. logarithmic bucket
 };
 
@@ -496,7 +496,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward, few rows
-// One workgroup per (sample, key head, block of 32 rows, split of the keys).  Row = query head of the group x query; all rows of a block
+// One workgroup per (sample, key head, split of the keys).  Row = query head of the group x query, 32 at most; all of them
 // share every key tile, so the keys are read once for the whole group.  The four waves walk tiles of 32 keys of their own, each through
 // LDS of its own without barriers, and are joined at the end; splits are joined by rel_join_kernel.  Bound by the K / V bytes: 716 MB in
 // 140 us, 5.1 TB/s.
@@ -509,14 +509,13 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
   char* mine = smem + wave * 2 * STAGE;
   float* bias_all = reinterpret_cast<float*>(smem + 8 * STAGE);
   const int nb = 2 * (a.far + EXT) + 1;
-  const int split = blockIdx.x % a.splits, blk = (blockIdx.x / a.splits) % a.row_blocks, bk = blockIdx.x / a.splits / a.row_blocks;
+  const int split = blockIdx.x % a.splits, bk = blockIdx.x / a.splits;
   const int b = bk / a.Hk, hk = bk - b * a.Hk;
-  const int rows = a.G * a.Lq, row = blk * 32 + r;
-  const int rc = min(row, rows - 1), g = rc / a.Lq, i = rc - g * a.Lq, h = hk * a.G + g;
-  const int g0 = blk * 32 / a.Lq, g1 = min(blk * 32 + 31, rows - 1) / a.Lq;   // heads of this block
+  const int rows = a.G * a.Lq;
+  const int rc = min(r, rows - 1), g = rc / a.Lq, i = rc - g * a.Lq, h = hk * a.G + g;
   const int off = rel_offset(a, b), klen = rel_key_len(a, b, off), ip = i + off;
-  for (int gg = g0; gg <= g1; ++gg) rel_bias_fill<T>(a, bias_all + (gg - g0) * nb, EXT, hk * a.G + gg, tid, 256);
-  const float* bias = bias_all + (g - g0) * nb + a.far + EXT;
+  for (int gg = 0; gg < a.G; ++gg) rel_bias_fill<T>(a, bias_all + gg * nb, EXT, hk * a.G + gg, tid, 256);
+  const float* bias = bias_all + g * nb + a.far + EXT;
   // tiles of this split: the sample's own length is divided, so that short samples do not leave splits idle
   const int tiles = (klen + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
   const int t0 = split * per + wave, t1 = min((split + 1) * per, tiles);
@@ -631,8 +630,7 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
       *reinterpret_cast<float4*>(ob + (wave * 32 + r) * (D + 4) + 32 * dt + 8 * q4 + 4 * hf) =
           make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
   __syncthreads();
-  const int n_rows = min(32, rows - blk * 32);
-  for (int x = tid; x < n_rows * (D / 4); x += 256) {
+  for (int x = tid; x < rows * (D / 4); x += 256) {
     const int rr = x / (D / 4), d = 4 * (x - rr * (D / 4));
     float mm = -INFINITY, ll = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -649,13 +647,13 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
       acc.z += f * v4.z;
       acc.w += f * v4.w;
     }
-    const int64_t prow = ((int64_t)bk * a.row_blocks + blk) * 32 + rr;
+    const int64_t prow = (int64_t)bk * 32 + rr;
     if (a.splits > 1) {
       float* p = a.part + (prow * a.splits + split) * (D + 4);   // [.., D] sums, then (m, l)
       *reinterpret_cast<float4*>(p + d) = acc;
       if (d == 0) *reinterpret_cast<float2*>(p + D) = make_float2(mm, ll);
     } else {
-      const int ro = blk * 32 + rr, go = ro / a.Lq, io = ro - go * a.Lq, ho = hk * a.G + go;
+      const int go = rr / a.Lq, io = rr - go * a.Lq, ho = hk * a.G + go;
       const float f = ll > 0.f ? 1.f / ll : ll;
       rel_store_out<T>(a, (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
       if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm - REL_FWD_BITS<T> + log2f(ll);
@@ -673,7 +671,7 @@ __global__ __launch_bounds__(256) void rel_join_kernel(const RelArgs a) {
   const int bk = (int)(row / rows), ro = (int)(row - (int64_t)bk * rows);
   if (bk >= a.B * a.Hk) return;
   const int b = bk / a.Hk, hk = bk - b * a.Hk, go = ro / a.Lq, io = ro - go * a.Lq, ho = hk * a.G + go;
-  const float* p = a.part + ((int64_t)bk * a.row_blocks * 32 + ro) * a.splits * (D + 4);
+  const float* p = a.part + ((int64_t)bk * 32 + ro) * a.splits * (D + 4);
   float mm = -INFINITY, ll = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, p[s * (D + 4) + D]);
@@ -1236,7 +1234,6 @@ template <typename T, int D>
 static int rel_forward(const mmk_rel_attn* p, RelArgs& a, hipStream_t st) {
   if (rel_few_rows(p)) {
     a.splits = rel_splits(p);
-    a.row_blocks = 1;
     if (int rc = rel_launch(rel_split_kernel<T, D>, MMK_K_REL_ATTN_FWD, (int64_t)a.B * a.Hk * a.splits, (int)rel_split_lds(p), REL_LDS, a, st))
       return rc;
     if (a.splits == 1) return 0;
