@@ -612,10 +612,10 @@ int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const void* out_lo,
 /* Orthogonalised update of `count` matrices [rows, cols] of one shape by a quintic Newton-Schulz iteration (the step of a Muon-type
  * optimizer; beside mmk_adamw_update, which serves TrainingTask.configure_optimizers, mmlearn/tasks/base.py:72-155):
  *   X = G / (|G|_F + eps);  `steps` times  A = X X^T, X <- coef[0] X + (coef[1] A + coef[2] A^2) X   (G transposed where rows > cols).
- * src / momenta / dst: HOST arrays of `count` device addresses.  src: elements of `dtype` at row_stride / col_stride.  momenta (NULL: G = src):
- * f32 [rows][cols] contiguous buffers, moved on first: M <- momentum M + src, G = nesterov ? src + momentum M : M.  dst: bf16 [rows][cols]
- * results; with `weights`, f32 [rows][cols] weights that are stepped instead: W <- W (1 - lr weight_decay) - lr adjust X, lr from *lr_dev
- * (device) where that is given.  Sides up to 32768.  ws: mmk_newton_schulz_ws_bytes() bytes, 16-byte aligned. */
+ * src / momenta / dst: HOST arrays of `count` device addresses.  src: elements of `dtype` at row_stride / col_stride.  weights = 0: G = src, momenta
+ * NULL, dst: bf16 [rows][cols] results.  weights = 1, the whole step of an optimizer: momenta are f32 [rows][cols] contiguous buffers, moved on
+ * first: M <- momentum M + src, G = nesterov ? src + momentum M : M; dst: f32 [rows][cols] weights, W <- W (1 - lr weight_decay) - lr adjust X, lr
+ * from *lr_dev (device) where that is given.  eps: a normal positive number.  Sides up to 32768.  ws: mmk_newton_schulz_ws_bytes() bytes, 16-byte aligned. */
 typedef struct {
   const void* const* src;
   void* const* momenta;

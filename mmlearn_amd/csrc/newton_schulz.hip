@@ -539,9 +539,9 @@ __device__ __forceinline__ int ns_img_at(int row, int c, int image) {
   return (c >> 6) * image + row * 128 + ((((c & 63) >> 3) ^ img_swz(row)) << 4) + (c & 7) * 2;
 }
 
-// MB: blocks of 32 that hold anything of the short side (at least two): the rest is zero and not computed.  The k steps of a product are unrolled,
+// MUON: the momentum is moved on first and the weights at last.  MB: blocks of 32 that hold anything of the short side (at least two): the rest is zero and not computed.  The k steps of a product are unrolled,
 // so that their fragments are in flight together (201 x 65: 34 us, 39 with four blocks; 64 x 256: 29 and 40; the diagonals have cost 4 since).
-template <typename T, bool MOM, bool W, int MB>
+template <typename T, bool MUON, int MB>
 __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const NsPtrs p, int steps) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* X = smem;
@@ -552,7 +552,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
   const int mat = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hf = lane >> 5, fast = tid & 127, slow = tid >> 7;
   const T* src = reinterpret_cast<const T*>(p.src[mat]);
-  float* mom = MOM ? reinterpret_cast<float*>(p.mom[mat]) : nullptr;
+  float* mom = MUON ? reinterpret_cast<float*>(p.mom[mat]) : nullptr;
   const int halves = a.n > 128 ? 2 : 1;
   f32x16 x[MB];
   double sum = 0.0;
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
         float v = 0.f;
         if (i < a.m && j < a.n) {
           v = to_f32(src[ns_src_at(a, i, j)]);
-          if (MOM) {
+          if (MUON) {
             float* at = mom + (a.tall ? (int64_t)j * a.cols + i : (int64_t)i * a.cols + j);
             float m = *at;
             v = ns_momentum(a, m, v);
@@ -737,7 +737,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
     }
   }
   // ---- result, half by half through LDS
-  const float lr = W && a.lr_dev ? *a.lr_dev : a.lr;
+  const float lr = MUON && a.lr_dev ? *a.lr_dev : a.lr;
   for (int half = 0; half < halves; ++half) {
     __syncthreads();
     if (wave >> 2 == half) {
@@ -754,7 +754,7 @@ __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const 
       if (i < a.m && j < a.n) {
         const int64_t at = a.tall ? (int64_t)j * a.cols + i : (int64_t)i * a.cols + j;
         const float v = stage[jl * NS_SMALL_PITCH + i];
-        if (W) {
+        if (MUON) {
           float* w = reinterpret_cast<float*>(p.dst[mat]) + at;
           *w = ns_weight(a, lr, *w, v);
         } else {
@@ -866,8 +866,7 @@ static int ns_small_go(const mmk_newton_schulz_args* q, const NsArgs& a, const N
     MMK_LAUNCH_CHECK();
     return 0;
   };
-  if (q->momenta) return q->weights ? go(ns_small_kernel<T, true, true, MB>) : go(ns_small_kernel<T, true, false, MB>);
-  return q->weights ? go(ns_small_kernel<T, false, true, MB>) : go(ns_small_kernel<T, false, false, MB>);
+  return q->weights ? go(ns_small_kernel<T, true, MB>) : go(ns_small_kernel<T, false, MB>);
 }
 template <typename T>
 static int ns_small_run(const mmk_newton_schulz_args* q, const NsArgs& a, const NsPtrs& p, int count, hipStream_t st) {
@@ -898,7 +897,7 @@ int mmk_newton_schulz(const mmk_newton_schulz_args* q, void* ws, void* stream) {
   if (int rc = ns_check(q->count, q->rows, q->cols)) return rc;
   MMK_REQUIRE(q->steps >= 1 && q->steps <= 32, "1 to 32 steps");
   MMK_REQUIRE(q->eps >= FLT_MIN, "eps must be a normal positive number");   // (1 / eps has to be finite: zeros are divided by it)
-  MMK_REQUIRE(!q->momenta || q->dtype == MMK_F32 || q->dtype == MMK_BF16 || q->dtype == MMK_F16, "unsupported dtype");
+  MMK_REQUIRE((q->momenta != nullptr) == (q->weights != 0), "an optimizer's step has momenta and weights, an update neither");
   if (q->count == 0) return 0;
   const bool small = ns_small(q->rows, q->cols);
   MMK_REQUIRE(q->src && q->dst && (ws || small), "missing operand");

@@ -1448,8 +1448,8 @@ def newton_schulz(src: Sequence[int], dst: Sequence[int], rows: int, cols: int, 
                   device: torch.device, steps: int, coefficients: Sequence[float], eps: float, momenta: Optional[Sequence[int]] = None,
                   momentum: float = 0.0, nesterov: bool = False, weights: bool = False, lr: float = 0.0, adjust: float = 1.0,
                   weight_decay: float = 0.0, lr_dev: Optional[torch.Tensor] = None) -> None:
-    """Device addresses of equally shaped matrices -> their orthogonalised updates (bf16 at ``dst``), or with ``weights`` the step of the f32
-    weights at ``dst``; ``momenta``: f32 buffers moved on first.  ``device`` is the current one.  csrc/newton_schulz.hip."""
+    """Device addresses of equally shaped matrices -> their orthogonalised updates (bf16 at ``dst``), or with ``weights`` and ``momenta`` (f32 buffers,
+    moved on first) the step of the f32 weights at ``dst``.  ``device`` is the current one.  csrc/newton_schulz.hip."""
     n = len(src)
     array = C.c_void_p * max(n, 1)
     p = _lib.NewtonSchulz()

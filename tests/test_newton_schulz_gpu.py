@@ -444,3 +444,14 @@ def test_muon_steps_of_batches(count, rows, cols):
             assert (params[i].detach().double().cpu() - want[i]).abs().max() <= slack[i] + 4 * 2.0 ** -24, (step, i)
             b = opt.state[params[i]]["momentum_buffer"].double().cpu()
             assert (b - bufs[i]).abs().max() <= (step + 1) * 2.0 ** -23 * bufs[i].abs().max(), (step, i)
+
+
+def test_momenta_and_weights_go_together():
+    from mmlearn_amd import _lib
+
+    at = (ctypes.c_void_p * 1)(1 << 20)
+    for momenta, weights in ((None, 1), (ctypes.cast(at, ctypes.c_void_p), 0)):
+        p = _lib.NewtonSchulz()
+        p.src = p.dst = ctypes.cast(at, ctypes.c_void_p)
+        p.count, p.rows, p.cols, p.steps, p.eps, p.momenta, p.weights = 1, 8, 8, 5, 1e-7, momenta, weights
+        assert _lib.lib().mmk_newton_schulz(ctypes.byref(p), None, None) == -1 and b"momenta and weights" in _lib.lib().mmk_last_error()
