@@ -292,6 +292,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     ``q_offset``: position of query 0 among the keys, an int or an int32 tensor ``[B]`` (one token against a cache: the number of keys before
     it).  A row that nothing is left for gives zeros and passes no gradient.
 
+    A call that autograd records sums its result from weights in two 16-bit parts, one that it does not from weights rounded once (with few rows a
+    key head both do the former): the same value within the type's rounding, not bit for bit.
     The table's gradient is exact to about 1e-5 of its size before it is rounded to the table's type; forward-mode derivatives are
     refused.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive."""
     K.require_gpu(q, "query")

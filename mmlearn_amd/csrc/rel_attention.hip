@@ -16,6 +16,8 @@
 // delta decides how exact the table's gradient is: dS sums to zero along a row, and an error of delta is one of every dS of the row.  With
 // o rounded (or summed from rounded P) dtable is off by 4e-3 at 512 keys, an f32 one too.  So a forward that will be differentiated sums
 // o from P in two parts, rounded and the rest, and hands the backward what the rounding of o left: delta and dtable then hold to 1e-5.
+// Where nothing will be differentiated the prompt kernel rounds P once -- o is then off by 2.3e-3 of its size in bf16 where its own rounding is
+// 1.7e-3, and the second product would make it a third slower (230 us for 175) --; the few-rows kernel always takes both parts.
 // f16's range is narrow for dS (P is about 1 / Lk, the incoming gradient of any size) and for P of far keys, so both go through their products
 // times a power of two, which is exact and leaves with the accumulators: P times a constant, dS times one that follows its largest value.
 #include <hip/hip_ext.h>
@@ -605,12 +607,12 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const s16x8 pf = rel_operand<T>(s, st);
+      const s16x8 pl = rel_operand_rest<T>(s, st, pf);   // (in two parts always: under the loads it costs less than 1 %)
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_mfma<T>(rel_tr_frag(V + (dt >> 1) * IMG, il, st * 2048, dt & 1), pf, o[dt]);
-      if (a.out_lo) {
-        const s16x8 pl = rel_operand_rest<T>(s, st, pf);
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) o[dt] = rel_mfma<T>(rel_tr_frag(V + (dt >> 1) * IMG, il, st * 2048, dt & 1), pl, o[dt]);
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const s16x8 vf = rel_tr_frag(V + (dt >> 1) * IMG, il, st * 2048, dt & 1);
+        o[dt] = rel_mfma<T>(vf, pf, o[dt]);
+        o[dt] = rel_mfma<T>(vf, pl, o[dt]);
       }
     }
   }

@@ -618,3 +618,17 @@ def test_a_serving_batch_with_offsets_of_its_own(train):
     if train:
         for x, w in zip(torch.autograd.grad(out, leaves, dout.cuda()), torch.autograd.grad(want, a, dout.double())):
             assert torch.isfinite(x).all() and (x.double().cpu() - w).norm() <= tol * w.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("lq,lk,G", [(1, 1, 1), (1, 700, 4), (5, 3000, 6), (32, 90, 1)])
+def test_few_rows_give_one_result_with_and_without_gradients(lq, lk, G, dtype):
+    g = torch.Generator().manual_seed(lk)
+    q, k, v = (torch.randn(2, h, n, 128, generator=g).to(getattr(torch, dtype)).cuda() for h, n in ((2 * G, lq), (2, lk), (2, lk)))
+    table = torch.randn(32, 2 * G, generator=g).cuda()
+    plain = relative_attention(q, k, v, table, q_offset=lk - lq)
+    assert torch.equal(plain, relative_attention(q.requires_grad_(True), k, v, table, q_offset=lk - lq).detach())
+    want = oracle.relative_attention(*(t.detach().double().cpu() for t in (q, k, v, table)), q_offset=lk - lq)
+    # P in two parts is off by u^2: the result's one rounding (u at most, u / sqrt(3) in the mean square) is nearly all there is
+    assert (plain.double().cpu() - want).norm() <= 0.75 * torch.finfo(q.dtype).eps / 2 * want.norm()
