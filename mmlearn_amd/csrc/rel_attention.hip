@@ -137,6 +137,12 @@ __device__ __forceinline__ s16x8 rel_operand_rest(const f32x16& x, int s, s16x8 
 // result (the softmax's sum is of the same values; lse takes the factor out again).
 template <typename T>
 constexpr int REL_FWD_BITS = std::is_same<T, f16_t>::value ? 7 : 0;
+// exp2(s - m + bits): where a backward follows, s - m by itself first, which is exactly 0 at the maximum -- a row with one key then has exactly the
+// weight 2^bits there, o = v and dS = 0 (see rel_dq_kernel) --, else with the shift in m, one addition less
+template <typename T, bool EXACT>
+__device__ __forceinline__ float rel_weight(float s, float m) {
+  return EXACT && REL_FWD_BITS<T> ? att_exp2((s - m) + REL_FWD_BITS<T>) : att_exp2(s - m);
+}
 // P's factor in the backward: P <= 1, and what f32 makes of a score may carry it a little above
 template <typename T>
 constexpr int REL_P_BITS = std::is_same<T, f16_t>::value ? 14 : 0;
@@ -466,13 +472,13 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
     }
-    const float nm = m == -INFINITY ? 0.f : REL_FWD_BITS<T> - m;
+    const float top = m == -INFINITY ? 0.f : LO ? m : m - REL_FWD_BITS<T>;
     float lt = 0.f;   // (a tile's sum by itself: single keys far below the sum so far would not move it)
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[t][e] = att_exp2(s[t][e] + nm);
+        s[t][e] = rel_weight<T, LO>(s[t][e], top);
         lt += s[t][e];
       }
     l += lt;
@@ -493,7 +499,7 @@ __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
   if (i < a.Lq) {
     const int64_t row = (((int64_t)b * a.Lq + i) * a.H + h) * D;
     rel_store_row<T, D>(reinterpret_cast<T*>(a.out) + row, LO ? reinterpret_cast<T*>(a.out_lo) + row : nullptr, o, sum > 0.f ? 1.f / sum : sum, hf);
-    if (a.lse && hf == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : m - REL_FWD_BITS<T> + log2f(sum);
+    if (a.lse && hf == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : m + (log2f(sum) - REL_FWD_BITS<T>);
   }
 }
 
@@ -596,11 +602,11 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
     }
-    const float nm = m == -INFINITY ? 0.f : REL_FWD_BITS<T> - m;
+    const float top = m == -INFINITY ? 0.f : m;
     float lt = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      s[e] = att_exp2(s[e] + nm);
+      s[e] = rel_weight<T, true>(s[e], top);
       lt += s[e];
     }
     l += lt;
@@ -658,7 +664,7 @@ __global__ __launch_bounds__(256, 1) void rel_split_kernel(const RelArgs a) {
       const int go = rr / a.Lq, io = rr - go * a.Lq, ho = hk * a.G + go;
       const float f = ll > 0.f ? 1.f / ll : ll;
       rel_store_out<T>(a, (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-      if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm - REL_FWD_BITS<T> + log2f(ll);
+      if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm + (log2f(ll) - REL_FWD_BITS<T>);
     }
   }
 }
@@ -689,7 +695,7 @@ __global__ __launch_bounds__(256) void rel_join_kernel(const RelArgs a) {
   }
   const float f = ll > 0.f ? 1.f / ll : ll;
   rel_store_out<T>(a, (((int64_t)b * a.Lq + io) * a.H + ho) * D + d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm - REL_FWD_BITS<T> + log2f(ll);
+  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + ho) * a.Lq + io] = ll == 0.f ? INFINITY : mm + (log2f(ll) - REL_FWD_BITS<T>);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, dtable
@@ -724,7 +730,8 @@ __device__ __forceinline__ void rel_diagonals(const f32x16& s, float (&d)[3]) {
 }
 
 // As the forward, with the query on the lane: dS^T needs lse and delta of the lane alone, and dQ^T += K^T dS^T takes it from the
-// accumulators.  dtable: rel_diagonals sums a near tile along its diagonals in registers, and each half wave adds the sums to a
+// accumulators.  delta is the diagonal of O dO^T, formed by the instructions and in the order of dP = V dO^T, and what o's rounding left times dO:
+// where one key has all of a row's weight (o = v), dP - delta is exactly zero, as dS is.  dtable: rel_diagonals sums a near tile along its diagonals in registers, and each half wave adds the sums to a
 // vector over the distances of its own (plain LDS reads and writes in a fixed order; LDS float atomics took 175 cycles a wave
 // instruction, which made this kernel 3.5 times slower).  Tiles beyond max_distance add to two registers.
 // D = 64 leaves room for three workgroups a CU, in registers and in LDS (16 documents of 512 rows, 12 heads: 41 us instead of 57
@@ -772,15 +779,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelA
     const T* gp = reinterpret_cast<const T*>(a.dout) + orow;
     const T* op = reinterpret_cast<const T*>(a.o) + orow;
     const T* lp = reinterpret_cast<const T*>(a.o_lo) + orow;
+    f32x16 od = rel_zero();
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       typedef T t8 __attribute__((ext_vector_type(8)));
       qf[kk] = *reinterpret_cast<const s16x8*>(qp + 16 * kk);
       gf[kk] = *reinterpret_cast<const s16x8*>(gp + 16 * kk);
-      const t8 g8 = __builtin_bit_cast(t8, gf[kk]), o8 = *reinterpret_cast<const t8*>(op + 16 * kk), l8 = *reinterpret_cast<const t8*>(lp + 16 * kk);
+      od = rel_mfma<T>(*reinterpret_cast<const s16x8*>(op + 16 * kk), gf[kk], od);
+      const t8 g8 = __builtin_bit_cast(t8, gf[kk]), l8 = *reinterpret_cast<const t8*>(lp + 16 * kk);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf(to_f32(g8[e]), to_f32(o8[e]) + to_f32(l8[e]), delta);
+      for (int e = 0; e < 8; ++e) delta = fmaf(to_f32(g8[e]), to_f32(l8[e]), delta);
     }
+    const int own = ((r >> 2) & 1) == hf ? (r & 3) + 4 * (r >> 3) : -1;   // the register that holds (r, r)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) delta += e == own ? od[e] : 0.f;
     delta += rel_other_half(delta);
     const int64_t at = ((int64_t)b * a.H + h) * a.Lq + ic;
     lse = i < a.Lq ? a.lse[at] : INFINITY;

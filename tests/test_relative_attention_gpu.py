@@ -632,3 +632,40 @@ def test_few_rows_give_one_result_with_and_without_gradients(lq, lk, G, dtype):
     want = oracle.relative_attention(*(t.detach().double().cpu() for t in (q, k, v, table)), q_offset=lk - lq)
     # P in two parts is off by u^2: the result's one rounding (u at most, u / sqrt(3) in the mean square) is nearly all there is
     assert (plain.double().cpu() - want).norm() <= 0.75 * torch.finfo(q.dtype).eps / 2 * want.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("B,H,Hk,lq,lk,D,mask", [(3, 4, 2, 1, 1, 64, None), (2, 2, 1, 200, 1, 128, None), (4, 6, 3, 70, 40, 64, "one"), (2, 4, 4, 3, 500, 128, "one"),
+                                                (1, 1, 1, 1200, 1, 64, None)])
+def test_rows_with_one_key_pass_no_gradient_through_their_scores(B, H, Hk, lq, lk, D, mask, dtype):
+    """A softmax over one key is 1 whatever its score: dq, dk and the table's gradient are zero, not small."""
+    g = torch.Generator().manual_seed(lq + lk)
+    dt = getattr(torch, dtype)
+    q, k, v = (2 * torch.randn(B, h, n, D, generator=g).to(dt).cuda() for h, n in ((H, lq), (Hk, lk), (Hk, lk)))
+    table, dout = torch.randn(32, H, generator=g).cuda(), torch.randn(B, lq, H, D, generator=g).to(dt).cuda()
+    which = torch.randint(0, lk, (B,), generator=g)
+    keep = None if mask is None else (torch.arange(lk)[None] == which[:, None]).cuda()
+    leaves = [t.requires_grad_(True) for t in (q, k, v, table)]
+    out = relative_attention(*leaves, key_mask=keep, q_offset=7)
+    dq, dk, dv, dtable = torch.autograd.grad(out, leaves, dout)
+    rows = v.detach()[torch.arange(B), :, which].repeat_interleave(H // Hk, 1)[:, None]      # [B, 1, H, D]
+    assert torch.equal(out.detach(), rows.expand(-1, lq, -1, -1))
+    assert not dq.any() and not dk.any() and not dtable.any(), (dq.abs().max().item(), dk.abs().max().item(), dtable.abs().max().item())
+    want = dout.double().sum(1).view(B, Hk, H // Hk, D).sum(2)
+    got = dv.double()[torch.arange(B), :, which]
+    # P in 16 bits is 1 (f32 carries it 1e-6 off at most); sums of lq H / Hk rows in f32
+    assert (got - want).abs().max() <= torch.finfo(dt).eps * want.abs().max() + 2.0 ** -20 * dout.abs().max() * lq
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("L", [40, 300])
+def test_the_first_causal_row_passes_no_gradient_through_its_score(L, dtype):
+    dt = getattr(torch, dtype)
+    g = torch.Generator().manual_seed(L)
+    q, k, v = (torch.randn(2, 4, L, 64, generator=g).to(dt).cuda().requires_grad_(True) for _ in range(3))
+    table = torch.randn(32, 4, generator=g).cuda()
+    out = relative_attention(q, k, v, table, causal=True)
+    dq, = torch.autograd.grad(out, q, torch.randn(2, L, 4, 64, generator=g).to(dt).cuda())
+    assert not dq[:, :, 0].any() and dq[:, :, 1:].any()
