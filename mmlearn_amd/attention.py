@@ -210,7 +210,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     turn (``interleaved``: ``(2 i, 2 i + 1)``), the others pass.  None: no rotation.  ``positions``: int32 / int64 ``[L]`` or ``[B, L]``, rows of
     the table; None: ``0 .. L - 1``.  They are read on the device: a position outside the table makes its rows NaN.
     Forward-mode derivatives are refused.  Both passes may be captured into a HIP graph.  As with every autograd function, no output of an
-    eager pass over the same leaves may be alive then: it would keep the leaves' gradient nodes on that pass's stream."""
+    eager pass over the same leaves may be alive then: it would keep the leaves' gradient nodes on that pass's stream.
+    ``torch.compile`` does not trace the call: the graph breaks around it."""
+    if torch.compiler.is_dynamo_compiling():
+        return _qk_norm_rotary_untraced(q, k, q_weight, k_weight, rotary, positions, interleaved, eps)
     K.require_gpu(q, "query")
     name = "mmlearn_amd.qk_norm_rotary"
     if not (q.dim() == k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3] and q.dtype == k.dtype
@@ -244,6 +247,9 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     if not _records(q, k, q_weight, k_weight):
         return K.qk_norm_rotary_fwd(q, k, q_weight, k_weight, rotary, positions, interleaved, eps)
     return _QKNormRotary.apply(q, k, q_weight, k_weight, rotary, positions, bool(interleaved), float(eps))
+
+
+_qk_norm_rotary_untraced = torch.compiler.disable(qk_norm_rotary)
 
 
 # ------------------------------------------------------------------ attention with a learned relative position bias
@@ -295,7 +301,10 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     A call that autograd records sums its result from weights in two 16-bit parts, one that it does not from weights rounded once (with few rows a
     key head both do the former): the same value within the type's rounding, not bit for bit.
     The table's gradient is exact to about 1e-5 of its size before it is rounded to the table's type; forward-mode derivatives are
-    refused.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive."""
+    refused.  A HIP graph may hold both passes if no output of an eager pass over the same leaves is alive.  ``torch.compile`` does not trace the
+    call: the graph breaks around it."""
+    if torch.compiler.is_dynamo_compiling():   # (the kernels' descriptions are ctypes structures, which a resumed trace takes for their classes)
+        return _relative_attention_untraced(q, k, v, table, max_distance, bidirectional, scale, causal, key_mask, q_offset)
     K.require_gpu(q, "query")
     name = "mmlearn_amd.relative_attention"
     if not (q.dim() == k.dim() == v.dim() == 4 and q.dtype in (torch.bfloat16, torch.float16) and q.dtype == k.dtype == v.dtype):
@@ -335,3 +344,6 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     if not _records(q, k, v, table):
         return K.rel_attn_fwd(K.rel_attn_operands(q, k, v, table, *how[:4], key_mask, q_offset), q, False)[0]
     return _RelativeAttention.apply(q, k, v, table, key_mask, offsets, how)
+
+
+_relative_attention_untraced = torch.compiler.disable(relative_attention)

@@ -207,13 +207,15 @@ def _check_iteration(name: str, steps: int, coefficients: Sequence[float], eps: 
         raise ValueError(f"{name}: eps must be positive, a normal number of float32")
 
 
+@torch.compiler.disable
 @torch.no_grad()
 def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients: Sequence[float] = NS_COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
     """The matrices of ``update`` ``[..., rows, cols]`` (f32 / bf16 / f16, any strides, sides up to 32768) with their singular values driven towards
     1: ``X = G / (|G| + eps)``, then ``steps`` times ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``.  Returns bf16, contiguous: the
     products run on 16-bit operands (csrc/newton_schulz.hip) with f32 diagonals, whose errors of about 5e-4 are below half a step of bf16.  A matrix
     of zeros stays zero; one that holds a NaN or an infinity becomes NaN.  The coefficients must keep singular values below about 4.
-    An update is no function to differentiate: the result requires no grad, and an ``update`` with a forward-mode tangent is refused."""
+    An update is no function to differentiate: the result requires no grad, and an ``update`` with a forward-mode tangent is refused.
+    ``torch.compile`` does not trace the call."""
     require_gpu(update, "update")
     name = "mmlearn_amd.optim.orthogonalize"
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(update).tangent is not None:
@@ -284,6 +286,7 @@ class Muon(torch.optim.Optimizer):
                     if "momentum_buffer" in self.state.get(p, {}):   # (not in place: the state dict may hold the other optimizer's own tensors)
                         self.state[p]["momentum_buffer"] = self.state[p]["momentum_buffer"].float() / (1 - group["momentum"])
 
+    @torch.compiler.disable
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -103,3 +103,33 @@ def test_token_by_token_gives_the_whole_sequence():
         y = F.linear(o.flatten(2), block.proj.bfloat16())
         # the same roundings but for the order of sums, which may turn a rounding of P, of o and of y the other way
         assert (y[:, 0].double() - whole[:, i].double()).norm() <= 4 * 2.0 ** -8 * whole[:, i].double().norm(), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_training_step_is_the_eager_one(backend):
+    """``torch.compile`` breaks its graph around the operators and the optimizer's step and computes what the eager step does."""
+    x, dy, lengths, _ = _inputs()
+    lengths = lengths.cuda()
+
+    def step(block, opt):
+        y = block(x, lengths)
+        y.backward(dy)
+        opt.step()
+        opt.zero_grad()
+        return y.detach()
+
+    torch._dynamo.reset()
+    results = []
+    for compiled in (False, True):
+        block = Block().cuda()
+        opt = Muon([block.qkv, block.proj], lr=0.05)
+        run = torch.compile(step, backend=backend) if compiled else step
+        results.append([run(block, opt) for _ in range(3)] + [block.qkv.detach(), block.proj.detach(), block.bias.grad])
+    for a, b in zip(*results):
+        assert (a is None and b is None) or torch.equal(a, b)
+    held = torch.randn(40, 50, device="cuda")
+    from mmlearn_amd.optim import orthogonalize
+
+    assert torch.equal(torch.compile(lambda t: orthogonalize(2 * t), backend=backend)(held), orthogonalize(2 * held))
+    torch._dynamo.reset()
