@@ -265,6 +265,10 @@ class Muon(torch.optim.Optimizer):
                                       eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn, capturable=bool(capturable)))
         self._lr_words: Dict[Any, Any] = {}
 
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        self.__dict__.setdefault("_lr_words", {})   # (a copy or an unpickled optimizer has none yet; load_state_dict keeps what captures read)
+
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
         for p in self.param_groups[-1]["params"]:

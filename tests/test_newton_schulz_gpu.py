@@ -9,6 +9,7 @@ import copy
 import ctypes
 import math
 import os
+import pickle
 import subprocess
 
 import pytest
@@ -455,3 +456,21 @@ def test_momenta_and_weights_go_together():
         p.src = p.dst = ctypes.cast(at, ctypes.c_void_p)
         p.count, p.rows, p.cols, p.steps, p.eps, p.momenta, p.weights = 1, 8, 8, 5, 1e-7, momenta, weights
         assert _lib.lib().mmk_newton_schulz(ctypes.byref(p), None, None) == -1 and b"momenta and weights" in _lib.lib().mmk_last_error()
+
+
+def test_copies_of_the_optimizer_work(monkeypatch):
+    calls = []
+    _on_the_host(monkeypatch, calls)
+    p = torch.nn.Parameter(torch.zeros(3, 4))
+    opt = Muon([p], lr=0.5, capturable=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        other.param_groups[0]["lr"] = 0.25
+        other.param_groups[0]["params"][0].grad = torch.ones_like(p)
+        other.step()
+        assert calls[-1][3] == 0.25 and other.lr_device().item() == 0.25 and opt.lr_device().item() == 0.5
+    word = opt.lr_device()
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    opt.step()
+    assert opt.lr_device() is word and word.item() == 0.5     # (a captured step reads this word)
