@@ -991,6 +991,9 @@ def launch_ranks(n: int, argv: list[str]) -> int:
                 if code != 0 and rc == 0:
                     rc = code if code > 0 else 1
                     print(f"[bench] rank {r} exited with code {code}; stopping the other ranks", file=sys.stderr)
+                    until = time.monotonic() + 5.0     # most fail for the same reason a moment later: let them say so
+                    while time.monotonic() < until and any(procs[q].poll() is None for q in live):
+                        time.sleep(0.05)
                     for q in live:
                         procs[q].terminate()
             time.sleep(0.05)
