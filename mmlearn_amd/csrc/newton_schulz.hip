@@ -6,15 +6,16 @@
 // tiles on and above the diagonal are computed, their mirror image is stored with them).
 //
 // Products run on v_mfma_f32_32x32x16_f16 with f32 accumulation.  f16, not bf16: all singular values stay below 1.3, so range is no
-// matter, and its 11 bits leave 5e-4 in the result where bf16 operands leave 1e-2.  X itself is kept in f32: a X enters a step
-// unrounded, and only the correction B X passes through 16 bits -- with a rounded X the small singular values of a matrix with a few
+// matter, and its 11 bits leave 5e-4 in the result where bf16 operands leave 1e-2.  X itself is kept in more: in f32 where it stays on chip, else
+// in two f16 parts (layout below).  a X enters a step from there, and only the correction B X passes through 16 bits -- with a rounded X the small singular values of a matrix with a few
 // large ones drown in the large ones' rounding, amplified 3.4 times a step (measured: 2e-2 instead of 6e-4).  The diagonals of A and B, which
 // come to hold nearly all of them, are kept in f32 beside the operands and enter as A^2 = E^2 + D E + E D + D^2 and B X = E X + D X (with
 // rounded diagonals the result is off by 1.5e-3 to 1.9e-3).  The f16 copies carry a
 // power of two S ~ sqrt(max side), exact, which lifts the entries of large matrices (about 1 / S) out of f16's subnormals.
 //
 // Layout: sides padded with zeros, which the iteration keeps.  X is stored transposed, [n][m], as two f16 arrays: the operand S X rounded, and
-// the rest S X - that (together 22 bits, kept between steps).  A step moves 8 bytes an element: the transposed copy serves both products
+// the rest S X - that, kept between steps: together 22 bits where the rest is a normal f16, else S X to 2^-25
+// (about 19 bits of the first X of a 4096 x 4096 matrix, where S X is near 2^-6).  A step moves 8 bytes an element: the transposed copy serves both products
 // -- B X takes its rows, X X^T contracts along its columns with transposed LDS reads -- and its epilogue is in place.
 #include <float.h>
 #include <hip/hip_ext.h>
@@ -292,7 +293,8 @@ __device__ __forceinline__ void ns_result(const NsArgs& a, void* dst, int row, i
 // instead of eight.
 // KG groups of waves take the K steps in turn, each with a ring of its own, and their accumulators are added in LDS on the way out (always in
 // the same order): a workgroup that is alone on its CU then has two waves on each SIMD, and half the barriers.
-// Step product of 4096 x 4096: 145 us, 948 TFLOP/s (its epilogue moves 134 MB, 27 us, with nothing to run under); X X^T: 99 us, 715.
+// Step product of 4096 x 4096: 138 us, 995 TFLOP/s (its epilogue moves 134 MB, 27 us, with nothing to run under); X X^T: 92 us, 770.  The last step
+// as the step of the weights: 158 us (12 x 2304 x 768: 90, and 57 without the weights); the momentum pass 56 us on average of the two.
 // The accumulators leave through LDS as f32, 64 columns at a time, so that all global accesses of the epilogue are whole rows of 16 bytes a lane.
 template <int MODE, int MB, int WN, int NST, int KG>
 __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs a, const NsPtrs p, int xt_in, int tiles) {
@@ -528,7 +530,7 @@ __global__ __launch_bounds__(128 * WN * KG, 2) void ns_gemm_kernel(const NsArgs 
 
 // ------------------------------------------------------------------------------------------------ small matrices
 // A matrix of at most 128 x 256 never leaves its CU: one workgroup of eight waves does the whole iteration (the launches alone cost 108 us
-// for 201 x 65, this 38).  X^T is held twice: in f32 in the accumulator layout of the step product (wave w: rows 32 w .. of X^T on the
+// for 201 x 65, this 41).  X^T is held twice: in f32 in the accumulator layout of the step product (wave w: rows 32 w .. of X^T on the
 // lanes, 128 columns in 4 x 16 registers), which takes a X without any rounding, and rounded to f16 in LDS (two images of 256 rows x 64
 // columns), whose rows serve B X and whose columns, read transposed, X X^T.  A and then B stand in a third place (two images of 128 x 64).
 constexpr int NS_SMALL_M = 128, NS_SMALL_N = 256, NS_SMALL_PITCH = 129;
@@ -540,7 +542,7 @@ __device__ __forceinline__ int ns_img_at(int row, int c, int image) {
 }
 
 // MUON: the momentum is moved on first and the weights at last.  MB: blocks of 32 that hold anything of the short side (at least two): the rest is zero and not computed.  The k steps of a product are unrolled,
-// so that their fragments are in flight together (201 x 65: 34 us, 39 with four blocks; 64 x 256: 29 and 40; the diagonals have cost 4 since).
+// so that their fragments are in flight together (201 x 65: 41 us; three blocks instead of four saved 5 of it, two at 64 x 256 11).
 template <typename T, bool MUON, int MB>
 __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const NsPtrs p, int steps) {
   extern __shared__ __attribute__((aligned(16))) char smem[];

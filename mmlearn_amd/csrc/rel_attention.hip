@@ -17,7 +17,7 @@
 // o rounded (or summed from rounded P) dtable is off by 4e-3 at 512 keys, an f32 one too.  So a forward that will be differentiated sums
 // o from P in two parts, rounded and the rest, and hands the backward what the rounding of o left: delta and dtable then hold to 1e-5.
 // Where nothing will be differentiated the prompt kernel rounds P once -- o is then off by 2.3e-3 of its size in bf16 where its own rounding is
-// 1.7e-3, and the second product would make it a third slower (230 us for 175) --; the few-rows kernel always takes both parts.
+// 1.7e-3, and the second product would make it 40 % slower (233 us for 166) --; the few-rows kernel always takes both parts.
 // f16's range is narrow for dS (P is about 1 / Lk, the incoming gradient of any size) and for P of far keys, so both go through their products
 // times a power of two, which is exact and leaves with the accumulators: P times a constant, dS times one that follows its largest value.
 #include <hip/hip_ext.h>
@@ -149,8 +149,8 @@ constexpr int REL_P_BITS = std::is_same<T, f16_t>::value ? 14 : 0;
 
 // f16: the power of two that dS of a lane's row (key) goes through its product with, a running one like the maximum of a softmax: it falls
 // when a value times it would pass 2^15, and the accumulators of that lane (and of the one 32 away, which holds the same row) fall with it.
-// Values 2^-29 of the largest so far are still normal.  bf16 has f32's range and needs none.  (2 x 16 (on 4) x 4097 x 128 causal and back: 865 us,
-// without it 825; 16 x 12 x 512 x 64: 152 both.)
+// Values 2^-29 of the largest so far are still normal.  bf16 has f32's range and needs none.  (2 x 16 (on 4) x 4097 x 128 causal and back: 874 us,
+// without it 830; 16 x 12 x 512 x 64: 152 both.)
 struct RelRange {
   int bits = 60;   // (from here down f16 results of such dS are zero anyway)
   float factor = 0x1p60f;
@@ -364,8 +364,8 @@ __device__ __forceinline__ void rel_store_out(const RelArgs& a, int64_t at, floa
 // unit -- exponential, bias, maximum, sum: twice the cycles of the products at D = 64 -- bounds it and finer workgroups fill the chip better:
 // 4 x 12 x 512 x 64 20 us with 32 and 23 with 64, 2 x 12 x 8192 x 64 503 and 498.  At D = 128 the LDS reads take as long as the products:
 // a fragment of 1 KiB for each, four waves, 128 bytes a cycle.)  Scores of the next tile formed under the exponentials of this one, in one
-// wave: 5 to 15 % slower than two waves that do so by themselves.  2 x 16 x 4096 x 128: 295 us, 930 TFLOP/s; 2 x 12 x 8192 x 64: 512 us, 805;
-// 256 x 12 x 77 x 64: 36 us, 3.4 TB/s.  LO: P V with P in two parts, 230 us for 2 x 16 x 4097 x 128 causal, 175 without.
+// wave: 5 to 15 % slower than two waves that do so by themselves.  2 x 16 x 4096 x 128: 281 us, 978 TFLOP/s (f16 298); 2 x 12 x 8192 x 64: 496 us, 831
+// (f16 523); 256 x 12 x 77 x 64: 36 us, 3.4 TB/s.  LO: P V with P in two parts, 233 us for 2 x 16 x 4097 x 128 causal, 166 without.
 template <typename T, int D, bool LO>
 __global__ __launch_bounds__(256, 2) void rel_fwd_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -735,7 +735,7 @@ __device__ __forceinline__ void rel_diagonals(const f32x16& s, float (&d)[3]) {
 // vector over the distances of its own (plain LDS reads and writes in a fixed order; LDS float atomics took 175 cycles a wave
 // instruction, which made this kernel 3.5 times slower).  Tiles beyond max_distance add to two registers.
 // D = 64 leaves room for three workgroups a CU, in registers and in LDS (16 documents of 512 rows, 12 heads: 41 us instead of 57
-// with two, the dK / dV kernel below 45 instead of 61).  At D = 128 bound as the forward: 2 x 16 x 4097 x 128 causal 280 us, 735 TFLOP/s.
+// with two, the dK / dV kernel below 42 instead of 61).  At D = 128 bound as the forward: 2 x 16 x 4097 x 128 causal 284 us, 725 TFLOP/s (f16 328).
 constexpr int REL_DIAG = 8;   // vectors over the distances
 template <typename T, int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dq_kernel(const RelArgs a) {
@@ -947,7 +947,7 @@ __global__ __launch_bounds__(256) void rel_dtable_kernel(const float* part, W* d
 // The key on the lane: a wave keeps K and V of its 32 keys as operands, walks the query tiles of all heads of the group, and sums dK^T
 // and dV^T of the group in its accumulators.  With few key blocks (few key heads) or unequal ones (causal: the first keys see all rows, the
 // last few) the walk is divided among `dkv_splits` workgroups, whose f32 sums rel_dkv_join_kernel adds in order.
-// 2 x 16 (on 4) x 4097 x 128 causal: 369 us, 745 TFLOP/s, and 23 us for the join.
+// 2 x 16 (on 4) x 4097 x 128 causal: 370 us, 743 TFLOP/s (f16 412), and 23 us for the join.
 template <typename T, int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void rel_dkv_kernel(const RelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
