@@ -279,13 +279,16 @@ class Muon(torch.optim.Optimizer):
                 raise ValueError(f"mmlearn_amd.optim.Muon {wrong}")
 
     def load_state_dict(self, state_dict) -> None:
+        for group in state_dict["param_groups"]:   # (torch.optim.Muon takes more than this class does)
+            _check_iteration("mmlearn_amd.optim.Muon", group["ns_steps"], group["ns_coefficients"], group["eps"])
+            if not 0 <= group["momentum"] < 1:
+                raise ValueError("mmlearn_amd.optim.Muon: momentum must be at least 0 and below 1")
         means = ["capturable" not in group for group in state_dict["param_groups"]]
-        if any(mean and not 0 <= group["momentum"] < 1 for mean, group in zip(means, state_dict["param_groups"])):
-            raise ValueError("mmlearn_amd.optim.Muon: a state of torch.optim.Muon needs a momentum below 1")
+        capturable = [group.get("capturable", False) for group in self.param_groups]
         super().load_state_dict(state_dict)
-        for group, mean in zip(self.param_groups, means):
+        for group, mean, own in zip(self.param_groups, means, capturable):
             if mean:
-                group["capturable"] = self.defaults["capturable"]
+                group["capturable"] = own
                 for p in group["params"]:
                     if "momentum_buffer" in self.state.get(p, {}):   # (not in place: the state dict may hold the other optimizer's own tensors)
                         self.state[p]["momentum_buffer"] = self.state[p]["momentum_buffer"].float() / (1 - group["momentum"])

@@ -310,6 +310,9 @@ def test_a_state_of_torch_muon_is_converted(momentum):
         assert (opt.state[p]["momentum_buffer"].double() - m).abs().max() <= 4 * 4 * 2.0 ** -24 * m.abs().max() / (1 - momentum)
         assert torch.equal(theirs.state[params[i]]["momentum_buffer"], before[i])
     assert opt.param_groups[0]["lr"] == 0.02 and opt.param_groups[0]["capturable"] is True
+    mixed = Muon([{"params": [torch.nn.Parameter(p.detach().clone()) for p in params], "capturable": True}])     # (a group's own choice)
+    mixed.load_state_dict(theirs.state_dict())
+    assert mixed.param_groups[0]["capturable"] is True
     # a state of this class stays as it is
     other = Muon([torch.nn.Parameter(p.detach().clone()) for p in params] + [idle])
     sd = opt.state_dict()
@@ -320,6 +323,9 @@ def test_a_state_of_torch_muon_is_converted(momentum):
     Muon([idle]).load_state_dict(torch.optim.Muon([idle]).state_dict())     # (nothing in it yet)
     with pytest.raises(ValueError, match="momentum"):
         Muon([idle]).load_state_dict(torch.optim.Muon([idle], momentum=1.0).state_dict())
+    for how in (dict(ns_steps=40), dict(eps=1e-50)):     # refused here, not in the middle of a step
+        with pytest.raises(ValueError):
+            Muon([idle]).load_state_dict(torch.optim.Muon([idle], **how).state_dict())
 
 
 @pytest.mark.gpu
