@@ -578,7 +578,8 @@ int mmk_qk_norm_rotary_bwd(const void* q, const void* k, const void* qw, const v
  * first near_buckets hold one distance each, the next n_borders + 1 begin at near_buckets, borders[0], borders[1], .. (HOST memory,
  * ascending); all distances from max_distance (1 .. 512) on fall into one bucket.  table: [buckets][H], f32 or the operands' type.
  * mask: one of MMK_REL_MASK_* -- LEN: int [B] leading keys are kept; 8 / 32 / 64: [B, Lk] integers of that width with batch stride
- * mask_stride, nonzero = kept.  Masked keys and values may hold anything, with `causal` those behind the last query too.  q_offsets (int32 [B], device) overrides q_offset.
+ * mask_stride, nonzero = kept.  Masked keys and values may hold anything, with `causal` those behind the last query too.  q_offsets (int32
+ * [B], device) overrides q_offset.
  * ws: mmk_rel_attn_fwd_ws_floats() floats.
  * Backward: out / out_lo / dout [B, Lq, H, D] contiguous; dq / dk / dv contiguous [B, L, heads, D]; dtable [buckets][H] in table_dtype, NULL: not
  * wanted; ws: mmk_rel_attn_bwd_ws_floats() floats.  All sums in a fixed order. */
@@ -615,7 +616,8 @@ int mmk_rel_attn_bwd(const mmk_rel_attn* p, const void* out, const void* out_lo,
  * src / momenta / dst: HOST arrays of `count` device addresses.  src: elements of `dtype` at row_stride / col_stride.  weights = 0: G = src, momenta
  * NULL, dst: bf16 [rows][cols] results.  weights = 1, the whole step of an optimizer: momenta are f32 [rows][cols] contiguous buffers, moved on
  * first: M <- momentum M + src, G = nesterov ? src + momentum M : M; dst: f32 [rows][cols] weights, W <- W (1 - lr weight_decay) - lr adjust X, lr
- * from *lr_dev (device) where that is given.  eps: a normal positive number.  Sides up to 32768.  ws: mmk_newton_schulz_ws_bytes() bytes, 16-byte aligned. */
+ * from *lr_dev (device) where that is given.  eps: a normal positive number.  Sides up to 32768.  ws: mmk_newton_schulz_ws_bytes() bytes,
+ * 16-byte aligned. */
 typedef struct {
   const void* const* src;
   void* const* momenta;

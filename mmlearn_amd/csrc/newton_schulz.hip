@@ -7,15 +7,16 @@
 //
 // Products run on v_mfma_f32_32x32x16_f16 with f32 accumulation.  f16, not bf16: all singular values stay below 1.3, so range is no
 // matter, and its 11 bits leave 5e-4 in the result where bf16 operands leave 1e-2.  X itself is kept in more: in f32 where it stays on chip, else
-// in two f16 parts (layout below).  a X enters a step from there, and only the correction B X passes through 16 bits -- with a rounded X the small singular values of a matrix with a few
-// large ones drown in the large ones' rounding, amplified 3.4 times a step (measured: 2e-2 instead of 6e-4).  The diagonals of A and B, which
+// in two f16 parts (layout below).  a X enters a step from there, and only the correction B X passes through 16 bits -- with a rounded X the
+// small singular values of a matrix with a few large ones drown in the large ones' rounding, amplified 3.4 times a step (measured: 2e-2 instead of 6e-4).  The diagonals of A and B, which
 // come to hold nearly all of them, are kept in f32 beside the operands and enter as A^2 = E^2 + D E + E D + D^2 and B X = E X + D X (with
 // rounded diagonals the result is off by 1.5e-3 to 1.9e-3).  The f16 copies carry a
 // power of two S ~ sqrt(max side), exact, which lifts the entries of large matrices (about 1 / S) out of f16's subnormals.
 //
 // Layout: sides padded with zeros, which the iteration keeps.  X is stored transposed, [n][m], as two f16 arrays: the operand S X rounded, and
 // the rest S X - that, kept between steps: together 22 bits where the rest is a normal f16, else S X to 2^-25
-// (about 19 bits of the first X of a 4096 x 4096 matrix, where S X is near 2^-6).  A step moves 8 bytes an element: the transposed copy serves both products
+// (about 19 bits of the first X of a 4096 x 4096 matrix, where S X is near 2^-6).  A step moves 8 bytes an element: the transposed copy serves
+// both products
 // -- B X takes its rows, X X^T contracts along its columns with transposed LDS reads -- and its epilogue is in place.
 #include <float.h>
 #include <hip/hip_ext.h>
@@ -541,8 +542,8 @@ __device__ __forceinline__ int ns_img_at(int row, int c, int image) {
   return (c >> 6) * image + row * 128 + ((((c & 63) >> 3) ^ img_swz(row)) << 4) + (c & 7) * 2;
 }
 
-// MUON: the momentum is moved on first and the weights at last.  MB: blocks of 32 that hold anything of the short side (at least two): the rest is zero and not computed.  The k steps of a product are unrolled,
-// so that their fragments are in flight together (201 x 65: 41 us; three blocks instead of four saved 5 of it, two at 64 x 256 11).
+// MUON: the momentum is moved on first and the weights at last.  MB: blocks of 32 that hold anything of the short side (at least two): the rest
+// is zero and not computed.  The k steps of a product are unrolled, so that their fragments are in flight together (201 x 65: 41 us; three blocks instead of four saved 5 of it, two at 64 x 256 11).
 template <typename T, bool MUON, int MB>
 __global__ __launch_bounds__(512, 2) void ns_small_kernel(const NsArgs a, const NsPtrs p, int steps) {
   extern __shared__ __attribute__((aligned(16))) char smem[];

@@ -731,7 +731,8 @@ __device__ __forceinline__ void rel_diagonals(const f32x16& s, float (&d)[3]) {
 
 // As the forward, with the query on the lane: dS^T needs lse and delta of the lane alone, and dQ^T += K^T dS^T takes it from the
 // accumulators.  delta is the diagonal of O dO^T, formed by the instructions and in the order of dP = V dO^T, and what o's rounding left times dO:
-// where one key has all of a row's weight (o = v), dP - delta is exactly zero, as dS is.  dtable: rel_diagonals sums a near tile along its diagonals in registers, and each half wave adds the sums to a
+// where one key has all of a row's weight (o = v), dP - delta is exactly zero, as dS is.
+// dtable: rel_diagonals sums a near tile along its diagonals in registers, and each half wave adds the sums to a
 // vector over the distances of its own (plain LDS reads and writes in a fixed order; LDS float atomics took 175 cycles a wave
 // instruction, which made this kernel 3.5 times slower).  Tiles beyond max_distance add to two registers.
 // D = 64 leaves room for three workgroups a CU, in registers and in LDS (16 documents of 512 rows, 12 heads: 41 us instead of 57
@@ -1170,7 +1171,8 @@ static int rel_check(const mmk_rel_attn* p) {
   MMK_REQUIRE((int64_t)p->B * p->H * std::max<int64_t>(1, ((int64_t)p->Lq + 127) / 128) < (1 << 24), "too many query rows");
   MMK_REQUIRE(p->buckets >= 1 && p->buckets <= REL_MAX_BUCKETS && p->n_borders >= 0 && p->n_borders <= REL_MAX_BORDERS, "too many buckets");
   MMK_REQUIRE(p->n_borders == 0 || p->borders, "missing borders");
-  MMK_REQUIRE(p->near_buckets >= 1 && p->near_buckets <= REL_MAX_BUCKETS && p->max_distance >= 1 && p->max_distance <= REL_MAX_FAR, "max_distance must be 1 .. 512");
+  MMK_REQUIRE(p->near_buckets >= 1 && p->near_buckets <= REL_MAX_BUCKETS, "1 to 256 single distances a side");
+  MMK_REQUIRE(p->max_distance >= 1 && p->max_distance <= REL_MAX_FAR, "max_distance must be 1 .. 512");
   MMK_REQUIRE((p->bidirectional ? 2 : 1) * (p->near_buckets + p->n_borders + 1) == p->buckets, "near and logarithmic buckets do not add up");
   for (int i = 0; i < 3; ++i) {
     MMK_REQUIRE(p->q_strides[i] % 8 == 0 && p->k_strides[i] % 8 == 0 && p->v_strides[i] % 8 == 0, "strides must be multiples of 8 elements");
